@@ -170,6 +170,37 @@ int lbmk_layernorm(const void* x, void* y, const float* gamma, const float* beta
                    int rows, int C, float eps, void* stream);
 
 /* ------------------------------------------------------------------------
+ * RMS norm of every query / key head and the rotation by the token's position, in one pass:
+ *   y = R(pos) (w * x * rsqrt(mean(x^2) + eps)),  mean over the D channels of one head.
+ * No counterpart in the reference (its denoisers neither norm q / k nor rotate them); stands next to lbmk_layernorm.
+ *   q, q_out : [B][N][ldq / ldqo], Hq heads of D channels;  k, k_out likewise with Hk heads; bf16, or f32 (f32 = 1).
+ *              q_out may be q and k_out k (each row is read before it is written).
+ *   wq, wk   : [D] gains, bf16 or f32 (w_f32 = 1), NULL: ones
+ *   table    : f32 [positions][rot / 2 / axes][2], cosine and sine;  pos : int32 [B][N][axes].  Pair j of the rot / 2
+ *              rotated ones takes axis j / F and column j mod F (F = rot / 2 / axes); it is channels (j, j + rot / 2), or
+ *              (2 j, 2 j + 1) when interleaved = 1.  Channels from rot on are not rotated.  A position outside
+ *              [0, positions) gives NaN in the pairs that take it.
+ * D: 8 ... 256, a multiple of 8; rot: a multiple of 8; rows and batches start on 16 bytes.
+ * Backward: dq_out / dk_out are the gradients of the outputs, q_out / k_out receive the gradients of q / k (they may be
+ * dq_out / dk_out); dwq / dwk receive the gains' gradients in their dtype (NULL: not wanted), summed in a fixed order;
+ * scratch holds lbmk_norm_rope_bwd_scratch_floats(D) floats.
+ * ---------------------------------------------------------------------- */
+typedef struct lbmk_norm_rope_desc {
+  const void *q, *k, *wq, *wk, *dq_out, *dk_out;
+  void *q_out, *k_out;
+  const float* table;
+  const int32_t* pos;
+  int32_t B, N, Hq, Hk, D, rot, axes, positions;
+  int32_t ldq, ldk, ldqo, ldko, lddq, lddk;
+  int64_t sq, sk, sqo, sko, sdq, sdk;
+  int32_t f32, w_f32, interleaved;
+  float eps;
+} lbmk_norm_rope_desc;
+int lbmk_norm_rope(const lbmk_norm_rope_desc* d, void* stream);
+int64_t lbmk_norm_rope_bwd_scratch_floats(int D);
+int lbmk_norm_rope_bwd(const lbmk_norm_rope_desc* d, float* scratch, void* dwq, void* dwk, void* stream);
+
+/* ------------------------------------------------------------------------
  * Flash-style attention forward, softmax(q k^T * scale) v, no mask.
  * Replaces F.scaled_dot_product_attention inside diffusers' AttnProcessor2_0
  * (self-attention attn1/attn2 of BasicTransformerBlock; the reference passes

@@ -54,6 +54,14 @@ class IgemmDesc(C.Structure):
     ]
 
 
+class NormRopeDesc(C.Structure):
+    _fields_ = [(n, vp) for n in ("q", "k", "wq", "wk", "dq_out", "dk_out", "q_out", "k_out", "table", "pos")] + \
+               [(n, i32) for n in ("B", "N", "Hq", "Hk", "D", "rot", "axes", "positions",
+                                   "ldq", "ldk", "ldqo", "ldko", "lddq", "lddk")] + \
+               [(n, i64) for n in ("sq", "sk", "sqo", "sko", "sdq", "sdk")] + \
+               [("f32", i32), ("w_f32", i32), ("interleaved", i32), ("eps", f32)]
+
+
 # name -> (restype, argtypes); mirrors include/lbmk.h one to one
 SIGNATURES = {
     "lbmk_version": (i32, []),
@@ -70,6 +78,9 @@ SIGNATURES = {
     "lbmk_groupnorm_static_max_floats": (i64, []),
     "lbmk_groupnorm_static": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, f32, i32, vp]),
     "lbmk_layernorm": (i32, [vp, vp, vp, vp, i32, i32, f32, vp]),
+    "lbmk_norm_rope": (i32, [C.POINTER(NormRopeDesc), vp]),
+    "lbmk_norm_rope_bwd_scratch_floats": (i64, [i32]),
+    "lbmk_norm_rope_bwd": (i32, [C.POINTER(NormRopeDesc), vp, vp, vp, vp]),
     "lbmk_flash_attn_fwd": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, i32,
                                   i64, i64, i64, i64, f32, vp, vp]),
     "lbmk_flash_attn_bwd": (i32, [vp] * 13 + [i32] * 9 + [i64] * 6 + [f32, vp]),

@@ -258,6 +258,25 @@ class LayerNormFn(torch.autograd.Function):
         return (dx, *_cast_pair(dg, db, wdt), None, None, None)
 
 
+class QKNormRopeFn(torch.autograd.Function):
+    """Head norms of q and k with the position rotation (ops.qk_norm_rope); the backward pass recomputes the statistics
+    from the saved inputs."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, head_dim, table, positions, eps, interleaved):
+        ctx.save_for_backward(q, k, q_weight, k_weight, table, positions)
+        ctx.cfg = (head_dim, eps, interleaved)
+        return ops.qk_norm_rope(q, k, head_dim, q_weight, k_weight, table, positions, eps=eps, interleaved=interleaved)
+
+    @staticmethod
+    def backward(ctx, dq_out, dk_out):
+        q, k, wq, wk, table, positions = ctx.saved_tensors
+        head_dim, eps, interleaved = ctx.cfg
+        dq, dk, dwq, dwk = ops.qk_norm_rope_bwd(q, k, ops.token_rows_ready(dq_out), ops.token_rows_ready(dk_out), head_dim, wq, wk, table,
+                                                positions, eps=eps, interleaved=interleaved)
+        return dq, dk, dwq, dwk, None, None, None, None, None
+
+
 class SiluFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x):

@@ -1,0 +1,453 @@
+// RMS norm of every query / key head and the rotation by the token's position, one pass, forward and backward.
+//
+//   xh = x * rsqrt(mean(x^2) + eps)      y = R(pos) (w * xh)        (mean over the D channels of one head)
+//   g  = R(pos)^T dy     dw = sum over tokens and heads of g * xh     dx = rsqrt(..) * (g w - xh * mean(g w xh))
+//
+// R rotates `rot` leading channels in pairs: (j, j + rot/2), or (2j, 2j+1) when `interleaved`; pair j takes its angle from
+// axis j / F of the token's position (F = rot / 2 / axes) and column j mod F of the table of cosines and sines.  The
+// angles' far positions lose bits in f32, so the table is built once, in 64 bits, on the host side.
+//
+// Bound by memory: 4 bytes per element forward, 6 backward (bf16) and some 10 / 25 operations.  A head is held by
+// L = 2^k lanes, each with the TWO chunks of VEC channels that the rotation pairs up, so the rotation needs no exchange
+// between lanes and the norm a log2(L)-step butterfly.  The lanes of a group walk heads of ONE token, so its cosines and
+// sines are read once and stay in registers; four heads are loaded before the first is used, to have enough bytes in
+// flight.  All statistics and gradient sums are f32; each output is rounded once.
+#include "common.h"
+
+namespace {
+
+constexpr int NR_THREADS = 256;
+constexpr int NR_BATCH = 4;        // heads in flight per lane group
+
+struct NormRope {
+  const void *x[2], *w[2], *dy[2];
+  void* y[2];                      // forward: outputs; backward: dx
+  const float2* table;             // [P][F] (cos, sin)
+  const int32_t* pos;              // [tokens][axes]
+  float* partial;                  // backward: [grid][2][D]
+  int64_t sx[2], sdy[2], sy[2];    // batch strides (elements)
+  int ldx[2], lddy[2], ldy[2];     // token strides
+  int H[2];
+  int D, rot, axes, F, P, tokens, N, w_f32, w_wide, gpt;
+  float eps;
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ void nr_load(const T* p, float (&v)[VEC]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 4) {
+      const f32x4 a = *(const f32x4*)(p + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[i + e] = a[e];
+    }
+  } else if constexpr (VEC == 8) {
+    const u16x8 a = *(const u16x8*)p;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = bf2f(a.v[e]);
+  } else {
+    const u16x4 a = *(const u16x4*)p;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = bf2f(a.v[e]);
+  }
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void nr_store(T* p, const float (&v)[VEC]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 4) *(f32x4*)(p + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
+  } else if constexpr (VEC == 8) {
+    u16x8 a;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a.v[e] = f2bf(v[e]);
+    *(u16x8*)p = a;
+  } else {
+    u16x4 a;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a.v[e] = f2bf(v[e]);
+    *(u16x4*)p = a;
+  }
+}
+
+// The two chunks of unit u (channel offsets; -1: none).  Paired halves: units below rot / 2 / VEC hold the chunks that
+// the rotation combines; the others, and every unit of the interleaved form, two neighbouring chunks.
+template <int VEC, bool INTER>
+__device__ __forceinline__ void nr_chunks(int u, int D, int rot, int& a, int& b, bool& turns_a, bool& turns_b) {
+  const int h = INTER ? 0 : rot / 2 / VEC;
+  if (u < h) {
+    a = u * VEC;
+    b = a + rot / 2;
+    turns_a = turns_b = true;
+    return;
+  }
+  a = (2 * u) * VEC;               // paired halves: 2 h chunks precede, units h, h+1, ... take the rest two by two
+  b = a + VEC;
+  if (a >= D) a = -1;
+  if (b >= D) b = -1;
+  turns_a = INTER && a >= 0 && a < rot;
+  turns_b = INTER && b >= 0 && b < rot;
+}
+
+// cosine / sine of the lane's pairs: VEC of them for two paired chunks, VEC / 2 per chunk when interleaved
+template <int VEC, bool INTER>
+__device__ __forceinline__ void nr_angles(const NormRope& d, int64_t token, int a, int b, bool ta, bool tb, float (&c)[VEC],
+                                          float (&s)[VEC]) {
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    c[e] = 1.f;
+    s[e] = 0.f;
+    const bool turns = INTER ? (e < VEC / 2 ? ta : tb) : ta;
+    if (!turns) continue;
+    const int j = INTER ? (e < VEC / 2 ? a / 2 + e : b / 2 + e - VEC / 2) : a + e;
+    const int ax = j / d.F;
+    const int p = d.pos[token * d.axes + ax];
+    if ((unsigned)p < (unsigned)d.P) {
+      const float2 cs = d.table[(int64_t)p * d.F + (j - ax * d.F)];
+      c[e] = cs.x;
+      s[e] = cs.y;
+    } else {
+      c[e] = s[e] = __builtin_nanf("");     // a position outside the table: never a silent wrong angle
+    }
+  }
+}
+
+// rotate (va, vb) by the angle (sign = 1) or back (sign = -1)
+template <int VEC, bool INTER>
+__device__ __forceinline__ void nr_rotate(float (&va)[VEC], float (&vb)[VEC], const float (&c)[VEC], const float (&s)[VEC], bool ta,
+                                          bool tb, float sign) {
+  if constexpr (INTER) {
+#pragma unroll
+    for (int e = 0; e < VEC; e += 2) {
+      const float ca = c[e / 2], sa = sign * s[e / 2], cb = c[VEC / 2 + e / 2], sb = sign * s[VEC / 2 + e / 2];
+      const float x0 = va[e], x1 = va[e + 1], y0 = vb[e], y1 = vb[e + 1];
+      if (ta) {
+        va[e] = x0 * ca - x1 * sa;
+        va[e + 1] = x1 * ca + x0 * sa;
+      }
+      if (tb) {
+        vb[e] = y0 * cb - y1 * sb;
+        vb[e + 1] = y1 * cb + y0 * sb;
+      }
+    }
+  } else if (ta) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float x0 = va[e], x1 = vb[e];
+      va[e] = x0 * c[e] - x1 * (sign * s[e]);
+      vb[e] = x1 * c[e] + x0 * (sign * s[e]);
+    }
+  }
+}
+
+template <int L>
+__device__ __forceinline__ float nr_sum(float v) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+template <typename T, int VEC, bool INTER, int L, bool BWD>
+__global__ __launch_bounds__(NR_THREADS) void norm_rope_kernel(NormRope d) {
+  constexpr int GROUPS = NR_THREADS / L;
+  const int t = threadIdx.x, u = t % L, group = t / L;
+  const int tpb = GROUPS / d.gpt;                       // tokens per block and step
+  const int sub = group % d.gpt;                        // this group's first head
+  int ca, cb;
+  bool ta, tb;
+  nr_chunks<VEC, INTER>(u, d.D, d.rot, ca, cb, ta, tb);
+  const int pa = ca < 0 ? 0 : ca, pb = cb < 0 ? 0 : cb; // idle chunks read channel 0 and count as zeros
+
+  float w[2][2][VEC], dw[BWD ? 2 : 1][2][VEC];
+#pragma unroll
+  for (int z = 0; z < 2; ++z)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      w[z][0][e] = w[z][1][e] = 1.f;
+      if (BWD) dw[z][0][e] = dw[z][1][e] = 0.f;
+    }
+#pragma unroll
+  for (int z = 0; z < 2; ++z) {
+    if (!d.w[z]) continue;
+    if (d.w_wide && d.w_f32) {
+      nr_load<float, VEC>((const float*)d.w[z] + pa, w[z][0]);
+      nr_load<float, VEC>((const float*)d.w[z] + pb, w[z][1]);
+    } else if (d.w_wide) {
+      nr_load<bf16_t, VEC>((const bf16_t*)d.w[z] + pa, w[z][0]);
+      nr_load<bf16_t, VEC>((const bf16_t*)d.w[z] + pb, w[z][1]);
+    } else {                       // a parameter's slot in a flat buffer need not start on 16 bytes
+      for (int e = 0; e < VEC; ++e) {
+        w[z][0][e] = d.w_f32 ? ((const float*)d.w[z])[pa + e] : bf2f(((const bf16_t*)d.w[z])[pa + e]);
+        w[z][1][e] = d.w_f32 ? ((const float*)d.w[z])[pb + e] : bf2f(((const bf16_t*)d.w[z])[pb + e]);
+      }
+    }
+  }
+  const float inv_d = 1.f / (float)d.D;
+
+  for (int64_t t0 = (int64_t)blockIdx.x * tpb; t0 < d.tokens; t0 += (int64_t)gridDim.x * tpb) {
+    const int64_t token = t0 + group / d.gpt;
+    const bool live = token < d.tokens;                 // groups past the end keep step with the butterflies, reading token 0
+    const int64_t tk = live ? token : 0;
+    const int64_t bb = tk / d.N, nn = tk - bb * d.N;
+    float c[VEC], s[VEC];
+    nr_angles<VEC, INTER>(d, tk, ca, cb, ta, tb, c, s);
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+      const T* xr = (const T*)d.x[z] + bb * d.sx[z] + nn * d.ldx[z];
+      const T* gr = BWD ? (const T*)d.dy[z] + bb * d.sdy[z] + nn * d.lddy[z] : nullptr;
+      T* yr = (T*)d.y[z] + bb * d.sy[z] + nn * d.ldy[z];
+      constexpr int NB = BWD ? NR_BATCH / 2 : NR_BATCH;
+      for (int h0 = sub; h0 < d.H[z]; h0 += NB * d.gpt) {
+        float xa[NB][VEC], xb[NB][VEC], ga[BWD ? NB : 1][VEC], gb[BWD ? NB : 1][VEC];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          const int h = h0 + i * d.gpt;
+          const int hc = h < d.H[z] ? h : sub;          // a head of this group's own: in bounds
+          nr_load<T, VEC>(xr + hc * d.D + pa, xa[i]);
+          nr_load<T, VEC>(xr + hc * d.D + pb, xb[i]);
+          if constexpr (BWD) {
+            nr_load<T, VEC>(gr + hc * d.D + pa, ga[i]);
+            nr_load<T, VEC>(gr + hc * d.D + pb, gb[i]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          const int h = h0 + i * d.gpt;
+          const bool put = live && h < d.H[z];
+          float qa = 0.f, qb = 0.f;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            qa = fmaf(xa[i][e], xa[i][e], qa);
+            qb = fmaf(xb[i][e], xb[i][e], qb);
+          }
+          // (a select, not a product: what an idle lane reads twice may be infinite)
+          const float ms = nr_sum<L>((ca < 0 ? 0.f : qa) + (cb < 0 ? 0.f : qb)) * inv_d;
+          const float rstd = __builtin_amdgcn_rsqf(ms + d.eps);
+          if constexpr (!BWD) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              xa[i][e] = xa[i][e] * rstd * w[z][0][e];
+              xb[i][e] = xb[i][e] * rstd * w[z][1][e];
+            }
+            nr_rotate<VEC, INTER>(xa[i], xb[i], c, s, ta, tb, 1.f);
+            if (put && ca >= 0) nr_store<T, VEC>(yr + h * d.D + ca, xa[i]);
+            if (put && cb >= 0) nr_store<T, VEC>(yr + h * d.D + cb, xb[i]);
+          } else {
+            nr_rotate<VEC, INTER>(ga[i], gb[i], c, s, ta, tb, -1.f);
+            float da = 0.f, db = 0.f;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              xa[i][e] *= rstd;
+              xb[i][e] *= rstd;
+              if (put) {
+                dw[z][0][e] = fmaf(ga[i][e], xa[i][e], dw[z][0][e]);
+                dw[z][1][e] = fmaf(gb[i][e], xb[i][e], dw[z][1][e]);
+              }
+              ga[i][e] *= w[z][0][e];
+              gb[i][e] *= w[z][1][e];
+              da = fmaf(ga[i][e], xa[i][e], da);
+              db = fmaf(gb[i][e], xb[i][e], db);
+            }
+            const float m = nr_sum<L>((ca < 0 ? 0.f : da) + (cb < 0 ? 0.f : db)) * inv_d;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              xa[i][e] = rstd * (ga[i][e] - xa[i][e] * m);
+              xb[i][e] = rstd * (gb[i][e] - xb[i][e] * m);
+            }
+            if (put && ca >= 0) nr_store<T, VEC>(yr + h * d.D + ca, xa[i]);
+            if (put && cb >= 0) nr_store<T, VEC>(yr + h * d.D + cb, xb[i]);
+          }
+        }
+      }
+    }
+  }
+
+  if constexpr (BWD) {
+    // the groups' sums of one block, in a fixed order: butterflies over the groups of a wave, then its four waves
+    __shared__ float part[NR_THREADS / 64][2][256];
+    const int wave = t >> 6;
+#pragma unroll
+    for (int z = 0; z < 2; ++z)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        float a = dw[z][0][e], b = dw[z][1][e];
+#pragma unroll
+        for (int o = L; o < 64; o <<= 1) {
+          a += __shfl_xor(a, o, 64);
+          b += __shfl_xor(b, o, 64);
+        }
+        if ((t & 63) < L) {
+          if (ca >= 0) part[wave][z][ca + e] = a;
+          if (cb >= 0) part[wave][z][cb + e] = b;
+        }
+      }
+    __syncthreads();
+    for (int i = t; i < 2 * d.D; i += NR_THREADS) {
+      const int z = i / d.D, ch = i - z * d.D;
+      float v = 0.f;
+#pragma unroll
+      for (int k = 0; k < NR_THREADS / 64; ++k) v += part[k][z][ch];
+      d.partial[((int64_t)blockIdx.x * 2 + z) * d.D + ch] = v;
+    }
+  }
+}
+
+// dw[z][ch] = sum over blocks of partial[block][z][ch], 16 columns per workgroup, 16 strips of blocks added in order
+__global__ __launch_bounds__(256) void norm_rope_dw_kernel(const float* __restrict__ partial, int blocks, int D, void* dwq, void* dwk,
+                                                          int out_f32) {
+  __shared__ float sums[16][17];
+  const int col = blockIdx.x * 16 + (threadIdx.x & 15), strip = threadIdx.x >> 4;
+  float v = 0.f;
+  if (col < 2 * D)
+    for (int b = strip; b < blocks; b += 16) v += partial[(int64_t)b * 2 * D + col];
+  sums[strip][threadIdx.x & 15] = v;
+  __syncthreads();
+  if (strip == 0 && col < 2 * D) {
+    float a = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) a += sums[k][threadIdx.x];
+    void* dst = col < D ? dwq : dwk;
+    if (!dst) return;
+    const int ch = col < D ? col : col - D;
+    if (out_f32) ((float*)dst)[ch] = a;
+    else ((bf16_t*)dst)[ch] = f2bf(a);
+  }
+}
+
+int nr_vec(int D, int rot, int interleaved) { return interleaved || (rot / 2) % 8 == 0 ? 8 : 4; }
+
+int nr_lanes(int D, int vec) {
+  const int units = (D / vec + 1) / 2;
+  int l = 1;
+  while (l < units) l <<= 1;
+  return l;
+}
+
+// blocks of a launch: each reads the weights once (and, backward, writes 2 D partial sums), so a few per CU walk the tokens
+int nr_blocks(int tokens, int tpb, int limit) {
+  const int64_t need = ((int64_t)tokens + tpb - 1) / tpb;
+  return (int)(need < limit ? need : limit);
+}
+
+constexpr int NR_BLOCKS = 2048, NR_BWD_BLOCKS = 1024;
+
+template <typename T, int VEC, bool INTER, bool BWD>
+void nr_launch(NormRope& d, int L, int blocks, hipStream_t s) {
+#define NR(l) hipLaunchKernelGGL((norm_rope_kernel<T, VEC, INTER, l, BWD>), dim3(blocks), dim3(NR_THREADS), 0, s, d)
+  switch (L) {
+    case 1: NR(1); break;
+    case 2: NR(2); break;
+    case 4: NR(4); break;
+    case 8: NR(8); break;
+    case 16: NR(16); break;
+    default: NR(32); break;
+  }
+#undef NR
+}
+
+int nr_run(NormRope& d, int f32, int interleaved, bool bwd, hipStream_t s) {
+  const int vec = nr_vec(d.D, d.rot, interleaved), L = nr_lanes(d.D, vec), groups = NR_THREADS / L;
+  // lane groups per token: with many tokens four or five heads per group, so that the token's angles are read once for
+  // several heads; with few tokens as many groups as there are heads
+  const int heads = d.H[0] > d.H[1] ? d.H[0] : d.H[1];
+  const int per = (int64_t)d.tokens * heads >= 65536 ? NR_BATCH : 1;
+  int gpt = 1;
+  while (gpt < groups && gpt * per < heads) gpt <<= 1;
+  d.gpt = gpt;
+  const int blocks = nr_blocks(d.tokens, groups / gpt, bwd ? NR_BWD_BLOCKS : NR_BLOCKS);
+#define NR_T(T)                                                        \
+  do {                                                                 \
+    if (interleaved) {                                                 \
+      if (bwd) nr_launch<T, 8, true, true>(d, L, blocks, s);           \
+      else nr_launch<T, 8, true, false>(d, L, blocks, s);              \
+    } else if (vec == 8) {                                             \
+      if (bwd) nr_launch<T, 8, false, true>(d, L, blocks, s);          \
+      else nr_launch<T, 8, false, false>(d, L, blocks, s);             \
+    } else {                                                           \
+      if (bwd) nr_launch<T, 4, false, true>(d, L, blocks, s);          \
+      else nr_launch<T, 4, false, false>(d, L, blocks, s);             \
+    }                                                                  \
+  } while (0)
+  if (f32) NR_T(float);
+  else NR_T(bf16_t);
+#undef NR_T
+  return blocks;
+}
+
+int nr_check(const lbmk_norm_rope_desc* p, bool bwd) {
+  LBMK_REQUIRE(p, "norm_rope: null descriptor");
+  LBMK_REQUIRE(p->D >= 8 && p->D <= 256 && p->D % 8 == 0, "norm_rope: head_dim %d (8 ... 256, a multiple of 8)", p->D);
+  LBMK_REQUIRE(p->rot >= 0 && p->rot <= p->D && p->rot % 8 == 0, "norm_rope: %d rotated channels of %d (a multiple of 8)", p->rot, p->D);
+  LBMK_REQUIRE(p->B >= 0 && p->N >= 0 && (int64_t)p->B * p->N < (1ll << 31), "norm_rope: batch %d, tokens %d", p->B, p->N);
+  LBMK_REQUIRE(p->Hq >= 0 && p->Hk >= 0 && p->Hq <= 65536 && p->Hk <= 65536, "norm_rope: heads %d, %d", p->Hq, p->Hk);
+  if (p->rot > 0) {
+    LBMK_REQUIRE(p->axes >= 1 && (p->rot / 2) % p->axes == 0, "norm_rope: %d pairs over %d axes", p->rot / 2, p->axes);
+  }
+  const int row = p->f32 ? 4 : 8;
+  const void* ptr[6] = {p->q, p->k, p->q_out, p->k_out, p->dq_out, p->dk_out};
+  const int ld[6] = {p->ldq, p->ldk, p->ldqo, p->ldko, p->lddq, p->lddk};
+  const int64_t st[6] = {p->sq, p->sk, p->sqo, p->sko, p->sdq, p->sdk};
+  LBMK_REQUIRE(p->eps >= 0.f, "norm_rope: eps %g", (double)p->eps);
+  const int we = p->w_f32 ? 4 : 2;
+  LBMK_REQUIRE((!p->wq || lbmk_aligned(p->wq, we)) && (!p->wk || lbmk_aligned(p->wk, we)), "norm_rope: misaligned weight");
+  if ((int64_t)p->B * p->N == 0) return LBMK_OK;      // nothing is read: the pointers may be null
+  if (p->rot > 0) {
+    LBMK_REQUIRE(p->table && p->pos && p->positions > 0, "norm_rope: rotation without a table or positions");
+    LBMK_REQUIRE(lbmk_aligned(p->table, 8) && lbmk_aligned(p->pos, 4), "norm_rope: misaligned table or positions");
+  }
+  for (int i = 0; i < (bwd ? 6 : 4); ++i) {
+    const int H = i % 2 ? p->Hk : p->Hq;
+    if (H == 0) continue;
+    LBMK_REQUIRE(ptr[i], "norm_rope: null pointer");
+    LBMK_REQUIRE(lbmk_aligned(ptr[i], 16) && ld[i] % row == 0 && st[i] % row == 0, "norm_rope: rows must start on 16 bytes");
+    LBMK_REQUIRE(p->N <= 1 || ld[i] >= H * p->D, "norm_rope: token stride %d below %d heads of %d", ld[i], H, p->D);
+    LBMK_REQUIRE(p->B <= 1 || st[i] >= 0, "norm_rope: negative batch stride");
+  }
+  return LBMK_OK;
+}
+
+NormRope nr_desc(const lbmk_norm_rope_desc* p) {
+  NormRope d = {};
+  d.x[0] = p->q; d.x[1] = p->k;
+  d.w[0] = p->wq; d.w[1] = p->wk;
+  d.y[0] = p->q_out; d.y[1] = p->k_out;
+  d.dy[0] = p->dq_out; d.dy[1] = p->dk_out;
+  d.table = (const float2*)p->table;
+  d.pos = p->pos;
+  d.sx[0] = p->sq; d.sx[1] = p->sk; d.sy[0] = p->sqo; d.sy[1] = p->sko; d.sdy[0] = p->sdq; d.sdy[1] = p->sdk;
+  d.ldx[0] = p->ldq; d.ldx[1] = p->ldk; d.ldy[0] = p->ldqo; d.ldy[1] = p->ldko; d.lddy[0] = p->lddq; d.lddy[1] = p->lddk;
+  d.H[0] = p->Hq; d.H[1] = p->Hk;
+  d.D = p->D; d.rot = p->rot; d.axes = p->rot ? p->axes : 1; d.F = p->rot ? p->rot / 2 / p->axes : 1;
+  d.P = p->positions; d.tokens = p->B * p->N; d.N = p->N > 0 ? p->N : 1; d.w_f32 = p->w_f32; d.eps = p->eps;
+  d.w_wide = (!p->wq || lbmk_aligned(p->wq, 16)) && (!p->wk || lbmk_aligned(p->wk, 16));
+  return d;
+}
+
+}  // namespace
+
+extern "C" int64_t lbmk_norm_rope_bwd_scratch_floats(int D) { return D > 0 ? (int64_t)NR_BWD_BLOCKS * 2 * D : 0; }
+
+extern "C" int lbmk_norm_rope(const lbmk_norm_rope_desc* p, void* stream) {
+  const int rc = nr_check(p, false);
+  if (rc != LBMK_OK) return rc;
+  if ((int64_t)p->B * p->N == 0 || p->Hq + p->Hk == 0) return LBMK_OK;
+  NormRope d = nr_desc(p);
+  nr_run(d, p->f32, p->interleaved, false, (hipStream_t)stream);
+  return lbmk_check_launch("norm_rope");
+}
+
+extern "C" int lbmk_norm_rope_bwd(const lbmk_norm_rope_desc* p, float* scratch, void* dwq, void* dwk, void* stream) {
+  const int rc = nr_check(p, true);
+  if (rc != LBMK_OK) return rc;
+  LBMK_REQUIRE(scratch && lbmk_aligned(scratch, 4), "norm_rope_bwd: no scratch");
+  hipStream_t s = (hipStream_t)stream;
+  int blocks = 0;
+  if ((int64_t)p->B * p->N > 0 && p->Hq + p->Hk > 0) {
+    NormRope d = nr_desc(p);
+    d.partial = scratch;
+    blocks = nr_run(d, p->f32, p->interleaved, true, s);
+  }
+  if (dwq || dwk)
+    hipLaunchKernelGGL(norm_rope_dw_kernel, dim3((2 * p->D + 15) / 16), dim3(256), 0, s, scratch, blocks, p->D, dwq, dwk, p->w_f32);
+  return lbmk_check_launch("norm_rope_bwd");
+}

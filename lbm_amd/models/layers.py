@@ -179,6 +179,15 @@ def training(*tensors_or_params) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors_or_params)
 
 
+def qk_norm_rope(q, k, head_dim: int, q_weight, k_weight, table=None, positions=None, *, eps: float = 1e-6, interleaved: bool = False):
+    """RMS norm of every q / k head and the position rotation -> (q', k'); differentiable in q, k and the weights.
+    Arguments: ops.qk_norm_rope."""
+    if training(q, k, q_weight, k_weight):
+        from ..autograd import QKNormRopeFn
+        return QKNormRopeFn.apply(q, k, q_weight, k_weight, head_dim, table, positions, eps, interleaved)
+    return ops.qk_norm_rope(q, k, head_dim, q_weight, k_weight, table, positions, eps=eps, interleaved=interleaved)
+
+
 def fused_rows(module: _Cached, name: str, layers, bias: bool):
     """Packs several Linear layers that share an input into one [sum N, K] weight."""
     params = []

@@ -5,6 +5,7 @@ operands, allocates the output with ``torch.empty`` and hands raw pointers plus 
 current HIP stream to liblbmk.  Activations are bf16 channels-last: a ``[B, H, W, C]``
 tensor (contiguous) which is at the same time the ``[B*H*W, C]`` token matrix.
 """
+import contextlib
 import ctypes as C
 import os
 import math
@@ -14,7 +15,7 @@ from typing import Optional
 import torch
 
 from . import _C
-from ._C import ACT_GEGLU, ACT_NONE, ACT_RELU, ACT_SILU, DT_BF16, DT_F32, IgemmDesc, check, lib
+from ._C import ACT_GEGLU, ACT_NONE, ACT_RELU, ACT_SILU, DT_BF16, DT_F32, IgemmDesc, NormRopeDesc, check, lib
 
 bf16 = torch.bfloat16
 
@@ -1410,3 +1411,147 @@ def lpips_head_bwd(f0, f1, w, keep, gout: torch.Tensor) -> torch.Tensor:
     check(lib.lbmk_lpips_head_bwd(f0.data_ptr(), f1.data_ptr(), w.data_ptr(), _ptr(keep), g.data_ptr(), df0.data_ptr(),
                                   B, HW, Cc, _stream()), "lbmk_lpips_head_bwd")
     return df0
+
+
+# --------------------------------------------------------------------------------------
+# token operators: head norms with the position rotation
+# --------------------------------------------------------------------------------------
+def _want(cond, msg: str):
+    if not cond:
+        raise ValueError(msg)
+
+
+def _same_device(first: torch.Tensor, *ts):
+    for t in ts:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"operands on {first.device} and {t.device}")
+
+
+def _on(t: torch.Tensor):
+    """the context in which ``t``'s device is the current one (launches and streams follow the current device)"""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _token_rows(name: str, t: torch.Tensor, heads: Optional[int], head_dim: int) -> torch.Tensor:
+    """``t`` as [B, N, heads * head_dim] with unit channel stride and rows on 16 bytes; column windows of wider rows pass"""
+    _want(t.dim() in (2, 3), f"{name}: [B, N, C] or [N, C] expected, got {tuple(t.shape)}")
+    t = t if t.dim() == 3 else t[None]
+    c = t.shape[2]
+    _want(c % head_dim == 0 and c > 0 and (heads is None or c == heads * head_dim),
+          f"{name}: {c} channels are not {'' if heads is None else heads} heads of {head_dim}")
+    unit = 16 // t.element_size()
+    ok = (t.stride(2) == 1 and t.data_ptr() % 16 == 0 and (t.shape[1] <= 1 or (t.stride(1) % unit == 0 and c <= t.stride(1) < 1 << 31))
+          and (t.shape[0] <= 1 or (t.stride(0) % unit == 0 and t.stride(0) >= 0)))
+    _want(ok or t.numel() == 0, f"{name}: strides {t.stride()} at address {t.data_ptr():#x}: channels must be adjacent and every "
+                                "token's row must start on 16 bytes")
+    return t
+
+
+def token_rows_ready(t: torch.Tensor) -> torch.Tensor:
+    """``t``, or a contiguous copy where the kernels cannot read it in place (an output gradient that autograd expanded
+    from a scalar or cut out of another tensor)"""
+    unit = 16 // t.element_size()
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % unit == 0 for s in t.stride()[:-1]) and \
+        (t.dim() < 2 or t.shape[-2] <= 1 or t.stride(-2) >= t.shape[-1])
+    return t if ok else t.contiguous()
+
+
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(1) if t.shape[1] > 1 else t.shape[2]
+
+
+def _sb(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else 0
+
+
+def rope_table(positions: int, pairs: int, theta: float = 10000.0, device=None) -> torch.Tensor:
+    """cosine and sine of position * theta^(-j / pairs): f32 [positions, pairs, 2], computed in 64 bits (an angle of a
+    far position has no digits left for its fraction of a turn in f32)"""
+    _want(positions > 0 and pairs > 0 and theta > 0, f"rope_table: {positions} positions, {pairs} pairs, theta {theta}")
+    ang = torch.arange(positions, dtype=torch.float64)[:, None] * theta ** (-torch.arange(pairs, dtype=torch.float64) / pairs)
+    return torch.stack((ang.cos(), ang.sin()), -1).to(torch.float32).to(device if device is not None else "cuda").contiguous()
+
+
+def _norm_rope_desc(q, k, head_dim, q_weight, k_weight, table, positions, eps, interleaved):
+    _same_device(q, k, q_weight, k_weight, table, positions)
+    _want(q.dtype in (bf16, torch.float32) and k.dtype == q.dtype, f"qk_norm_rope: q {q.dtype}, k {k.dtype} (both bf16 or both f32)")
+    q3, k3 = _token_rows("q", q, None, head_dim), _token_rows("k", k, None, head_dim)
+    _want(q3.shape[:2] == k3.shape[:2] and q.dim() == k.dim(), f"qk_norm_rope: q {tuple(q.shape)}, k {tuple(k.shape)}")
+    B, N = q3.shape[:2]
+    d = NormRopeDesc()
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        _want(w is None or (w.shape == (head_dim,) and w.is_contiguous() and w.dtype in (bf16, torch.float32)),
+              f"{name}: a bf16 or f32 vector of {head_dim}")
+    _want(q_weight is None or k_weight is None or q_weight.dtype == k_weight.dtype, "qk_norm_rope: the two weights have one dtype")
+    w = q_weight if q_weight is not None else k_weight
+    d.wq, d.wk, d.w_f32 = _ptr(q_weight), _ptr(k_weight), 1 if w is not None and w.dtype == torch.float32 else 0
+    _want((table is None) == (positions is None), "qk_norm_rope: table and positions go together")
+    if table is not None:
+        _want(table.dtype == torch.float32 and table.dim() == 3 and table.shape[2] == 2 and table.is_contiguous() and table.numel() > 0,
+              "table: contiguous f32 [positions, pairs, 2] (rope_table)")
+        _want(positions.dtype == torch.int32 and positions.is_contiguous(), "positions: contiguous int32")
+        lead = tuple(q.shape[:-1])
+        axes = 1 if tuple(positions.shape) == lead else positions.shape[-1] if tuple(positions.shape[:-1]) == lead else 0
+        _want(axes >= 1, f"positions {tuple(positions.shape)}: {lead} or {lead} x axes")
+        d.table, d.pos, d.axes, d.positions = table.data_ptr(), positions.data_ptr(), axes, table.shape[0]
+        d.rot = 2 * axes * table.shape[1]
+        _want(d.rot <= head_dim and d.rot % 8 == 0,
+              f"qk_norm_rope: {axes} axes of {table.shape[1]} pairs rotate {d.rot} of {head_dim} channels (a multiple of 8)")
+    _want(head_dim % 8 == 0 and 8 <= head_dim <= 256, f"qk_norm_rope: head_dim {head_dim} (8 ... 256, a multiple of 8)")
+    _want(eps >= 0, f"qk_norm_rope: eps {eps}")
+    _need_gpu(q)
+    d.q, d.k = q3.data_ptr(), k3.data_ptr()
+    d.B, d.N, d.Hq, d.Hk, d.D = B, N, q3.shape[2] // head_dim, k3.shape[2] // head_dim, head_dim
+    d.ldq, d.ldk, d.sq, d.sk = _ld(q3), _ld(k3), _sb(q3), _sb(k3)
+    d.f32, d.interleaved, d.eps = 1 if q.dtype == torch.float32 else 0, 1 if interleaved else 0, eps
+    return d
+
+
+def _norm_rope_out(d, q, k, out, head_dim):
+    """fills in the outputs: ``out`` or new contiguous tensors"""
+    qo, ko = out if out is not None else (torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device))
+    _same_device(q, qo, ko)
+    _want(qo.dtype == q.dtype and ko.dtype == q.dtype and qo.shape == q.shape and ko.shape == k.shape, "out: shapes and dtype of q and k")
+    q3, k3 = _token_rows("out[0]", qo, None, head_dim), _token_rows("out[1]", ko, None, head_dim)
+    _want((q3.shape[0] <= 1 or q3.stride(0) > 0) and (k3.shape[0] <= 1 or k3.stride(0) > 0), "out: a broadcast batch cannot be written")
+    d.q_out, d.k_out = q3.data_ptr(), k3.data_ptr()
+    d.ldqo, d.ldko, d.sqo, d.sko = _ld(q3), _ld(k3), _sb(q3), _sb(k3)
+    return qo, ko
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, head_dim: int, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                 table: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None, *, eps: float = 1e-6,
+                 interleaved: bool = False, out=None):
+    """RMS norm of every head of q and k and the rotation by the token's position, in one pass -> (q', k').
+
+    q: [B, N, Hq * D] or [N, Hq * D], k likewise with its own head count; bf16 or f32; column windows of a packed
+    projection are taken as they are.  q_weight / k_weight: [D] gains, bf16 or f32, or None.  ``table`` (``rope_table``)
+    [P, F, 2] and int32 ``positions`` [B, N] or [B, N, axes] rotate the first 2 * axes * F channels of a head: pair j
+    takes axis j // F and column j % F, and is channels (j, j + axes * F), or (2j, 2j + 1) when ``interleaved``.  A
+    position outside the table gives NaN.  No table: the norm alone.  ``out``: (q', k') destinations, also q and k
+    themselves.  Not differentiable: models.layers.qk_norm_rope is."""
+    d = _norm_rope_desc(q, k, head_dim, q_weight, k_weight, table, positions, eps, interleaved)
+    qo, ko = _norm_rope_out(d, q, k, out, head_dim)
+    with _on(q):
+        check(lib.lbmk_norm_rope(C.byref(d), _stream()), "lbmk_norm_rope")
+    return qo, ko
+
+
+def qk_norm_rope_bwd(q, k, dq_out, dk_out, head_dim: int, q_weight, k_weight, table=None, positions=None, *, eps: float = 1e-6,
+                     interleaved: bool = False, out=None):
+    """Gradients of ``qk_norm_rope`` for its inputs q, k and the gradients of its outputs -> (dq, dk, dq_weight, dk_weight);
+    the weights' gradients (None for a weight that is None) have the weights' dtype and are summed in a fixed order.
+    ``out``: (dq, dk) destinations."""
+    d = _norm_rope_desc(q, k, head_dim, q_weight, k_weight, table, positions, eps, interleaved)
+    _same_device(q, dq_out, dk_out)
+    _want(dq_out.dtype == q.dtype and dk_out.dtype == q.dtype and dq_out.shape == q.shape and dk_out.shape == k.shape,
+          "qk_norm_rope_bwd: gradients have the shapes and dtype of q and k")
+    g3, h3 = _token_rows("dq_out", dq_out, None, head_dim), _token_rows("dk_out", dk_out, None, head_dim)
+    d.dq_out, d.dk_out = g3.data_ptr(), h3.data_ptr()
+    d.lddq, d.lddk, d.sdq, d.sdk = _ld(g3), _ld(h3), _sb(g3), _sb(h3)
+    dq, dk = _norm_rope_out(d, q, k, out, head_dim)
+    scratch = torch.empty(lib.lbmk_norm_rope_bwd_scratch_floats(head_dim), dtype=torch.float32, device=q.device)
+    dwq, dwk = (None if w is None else torch.empty_like(w) for w in (q_weight, k_weight))
+    with _on(q):
+        check(lib.lbmk_norm_rope_bwd(C.byref(d), scratch.data_ptr(), _ptr(dwq), _ptr(dwk), _stream()), "lbmk_norm_rope_bwd")
+    return dq, dk, dwq, dwk
