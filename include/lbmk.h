@@ -235,6 +235,63 @@ int lbmk_flash_attn_bwd(const void* q, const void* qt, const void* k, const void
                         int64_t sq, int64_t sk, int64_t so, int64_t sqt, int64_t sdot, int64_t skt,
                         float scale, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Attention in which every query sees one interval of keys, with its backward pass.  No counterpart in the reference (its
+ * attention is unmasked); stands next to lbmk_flash_attn_fwd / _bwd.
+ *   s_ij = cap * tanh(scale * q_i.k_j / cap) - slopes[h] * |i + Nk - Nq - j|     (cap = 0: no cap; slopes = NULL: no bias)
+ *   o_i  = softmax over j in [ranges[b][i][0], ranges[b][i][1]) of s_ij, times V; an empty interval gives zeros
+ *   q, o, dout : bf16 [B][Nq][ldq / ldo / ldg], head h at columns h*D ..;  k, v : bf16 [B][Nk][ldk / ldv] with Hk heads, key
+ *                head h / (H / Hk) serves head h;  dq, dk, dv : contiguous
+ *   ranges     : int32 [B][Nq][2] (8-byte aligned; lbmk_key_ranges or the caller's own, clipped to [0, Nk)); NULL: every key
+ *   lse        : f32 [B][H][Nq] log2-sum-exp (of the base-2 scores; +inf for an empty row): written forward (NULL: not
+ *                wanted), read backward
+ *   scratch    : backward only, lbmk_ranged_attn_bwd_scratch_floats(...) floats, 16-byte aligned
+ * What an operand holds at places that a query does not see has no influence on its row, inf and NaN included; a value that is not
+ * finite at a place it does see makes the sums it enters not finite (NaN).
+ * D: 8 ... 160, a multiple of 8.  Any Nq, Nk.  Batch strides (elements): sq, sk, sv, so, sg.  scale > 0.
+ * ---------------------------------------------------------------------- */
+typedef struct lbmk_ranged_attn_desc {
+  const void *q, *k, *v, *dout;
+  void *o, *dq, *dk, *dv;
+  float* lse;
+  const int32_t* ranges;
+  const float* slopes;
+  float* scratch;
+  int32_t B, H, Hk, Nq, Nk, D;
+  int32_t ldq, ldk, ldv, ldo, ldg;
+  int64_t sq, sk, sv, so, sg;
+  float scale, cap;
+} lbmk_ranged_attn_desc;
+int lbmk_ranged_attn(const lbmk_ranged_attn_desc* d, void* stream);
+int64_t lbmk_ranged_attn_bwd_scratch_floats(int B, int H, int Hk, int Nq, int Nk, int D);
+int lbmk_ranged_attn_bwd(const lbmk_ranged_attn_desc* d, void* stream);
+
+/* The intervals of a batch: query i of row b stands at position p = i + Nk - Nq and sees
+ *   the keys of its document (doc_offsets: ascending token counts, docs + 1 per row of stride doc_stride, 0: one list for all;
+ *   a position outside all documents sees none) below lens[b], when causal = 1 only those up to p and those among the first
+ *   prefix[b] of its document, when window > 0 only the last `window` up to p.  NULL doc_offsets: one document of all keys. */
+int lbmk_key_ranges(int32_t* ranges, const int32_t* doc_offsets, int docs, int64_t doc_stride, const int32_t* prefix,
+                    const int32_t* lens, int B, int Nq, int Nk, int causal, int window, void* stream);
+
+/* The same attention for n new tokens per request over caches that already hold them:
+ *   q, o : bf16 [B][n][ldq] (o contiguous);  k, v : bf16 [B][cap_rows][ldk / ldv];  lens : int32 [B] tokens in the cache, the
+ *   new ones included (values outside [0, cap_rows] are clipped).  New token i stands at p = lens[b] - n + i and sees the keys up
+ *   to p (window > 0: the last `window` of them); p < 0: a row of zeros.  Rows of the cache from lens[b] on are not read.
+ *   scratch : lbmk_cached_attn_scratch_floats(...) floats, 8-byte aligned (NULL when 0). */
+typedef struct lbmk_cached_attn_desc {
+  const void *q, *k, *v;
+  void* o;
+  const int32_t* lens;
+  const float* slopes;
+  float* scratch;
+  int32_t B, H, Hk, n, cap_rows, D, window;
+  int32_t ldq, ldk, ldv;
+  int64_t sq, sk, sv;
+  float scale, cap;
+} lbmk_cached_attn_desc;
+int64_t lbmk_cached_attn_scratch_floats(int B, int H, int Hk, int n, int cap_rows, int D);
+int lbmk_cached_attn(const lbmk_cached_attn_desc* d, void* stream);
+
 /* Row softmax: f32 scores [rows][ld_in] -> bf16 probabilities [rows][ld_out]
  * (unfused attention for the VAE mid-block: 1 head, head_dim 512). */
 int lbmk_softmax_rows(const float* s, void* p, int64_t rows, int cols,

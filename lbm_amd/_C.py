@@ -62,6 +62,18 @@ class NormRopeDesc(C.Structure):
                [("f32", i32), ("w_f32", i32), ("interleaved", i32), ("eps", f32)]
 
 
+class RangedAttnDesc(C.Structure):
+    _fields_ = [(n, vp) for n in ("q", "k", "v", "dout", "o", "dq", "dk", "dv", "lse", "ranges", "slopes", "scratch")] + \
+               [(n, i32) for n in ("B", "H", "Hk", "Nq", "Nk", "D", "ldq", "ldk", "ldv", "ldo", "ldg")] + \
+               [(n, i64) for n in ("sq", "sk", "sv", "so", "sg")] + [("scale", f32), ("cap", f32)]
+
+
+class CachedAttnDesc(C.Structure):
+    _fields_ = [(n, vp) for n in ("q", "k", "v", "o", "lens", "slopes", "scratch")] + \
+               [(n, i32) for n in ("B", "H", "Hk", "n", "cap_rows", "D", "window", "ldq", "ldk", "ldv")] + \
+               [(n, i64) for n in ("sq", "sk", "sv")] + [("scale", f32), ("cap", f32)]
+
+
 # name -> (restype, argtypes); mirrors include/lbmk.h one to one
 SIGNATURES = {
     "lbmk_version": (i32, []),
@@ -81,6 +93,12 @@ SIGNATURES = {
     "lbmk_norm_rope": (i32, [C.POINTER(NormRopeDesc), vp]),
     "lbmk_norm_rope_bwd_scratch_floats": (i64, [i32]),
     "lbmk_norm_rope_bwd": (i32, [C.POINTER(NormRopeDesc), vp, vp, vp, vp]),
+    "lbmk_ranged_attn": (i32, [C.POINTER(RangedAttnDesc), vp]),
+    "lbmk_ranged_attn_bwd_scratch_floats": (i64, [i32] * 6),
+    "lbmk_ranged_attn_bwd": (i32, [C.POINTER(RangedAttnDesc), vp]),
+    "lbmk_key_ranges": (i32, [vp, vp, i32, i64, vp, vp, i32, i32, i32, i32, i32, vp]),
+    "lbmk_cached_attn_scratch_floats": (i64, [i32] * 6),
+    "lbmk_cached_attn": (i32, [C.POINTER(CachedAttnDesc), vp]),
     "lbmk_flash_attn_fwd": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, i32,
                                   i64, i64, i64, i64, f32, vp, vp]),
     "lbmk_flash_attn_bwd": (i32, [vp] * 13 + [i32] * 9 + [i64] * 6 + [f32, vp]),

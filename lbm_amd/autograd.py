@@ -385,6 +385,25 @@ class AttentionFn(torch.autograd.Function):
         return dq[:, :ctx.nq], dk[:, :ctx.nk], dv[:, :ctx.nk], None, None, None
 
 
+class RangedAttentionFn(torch.autograd.Function):
+    """Attention over key ranges (ops.ranged_attn): keeps q, k, v, the output and the rows' log-sum-exp; the scores are
+    recomputed in the backward kernels."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, heads, kv_heads, head_dim, ranges, scale, cap, slopes):
+        o, lse = ops.ranged_attn(q, k, v, heads, kv_heads, head_dim, ranges, scale=scale, cap=cap, slopes=slopes, return_lse=True)
+        ctx.save_for_backward(q, k, v, o, lse, ranges, slopes)
+        ctx.cfg = (heads, kv_heads, head_dim, scale, cap)
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        q, k, v, o, lse, ranges, slopes = ctx.saved_tensors
+        heads, kv_heads, head_dim, scale, cap = ctx.cfg
+        return (*ops.ranged_attn_bwd(q, k, v, o, ops.token_rows_ready(do), lse, heads, kv_heads, head_dim, ranges, scale=scale, cap=cap,
+                                     slopes=slopes), None, None, None, None, None, None, None)
+
+
 class SelfAttnQKVFn(torch.autograd.Function):
     """Self-attention whose three bias-free input projections run as ONE GEMM over the stacked weights:
     qkv = x @ [W_a; W_b; W_c]^T, o = softmax(q k^T * scale) v.  ``mod`` (the attention module) supplies the

@@ -1,0 +1,784 @@
+// Attention in which every query sees one interval [lo, hi) of keys: documents packed into a row, prefixes, causal and
+// windowed masks, padded batches; scores optionally capped by a tanh and biased by the distance; grouped key heads.
+//
+//   s_ij = cap tanh(scale q_i.k_j / cap) - slope_h |i + Nk - Nq - j|      p_i = softmax over j in [lo_i, hi_i)      o_i = p_i V
+// An empty interval gives a row of zeros.  Backward, with p recomputed from the rows' log-sum-exp and delta_i = dO_i.O_i:
+//   dV = P^T dO    dP = dO V^T    dS = P (dP - delta) (1 - tanh^2) scale    dQ = dS K    dK = dS^T Q
+//
+// Same formulation as the unmasked kernels: scores are produced transposed to the operand that they feed next
+// (S^T = K Q^T, the query on the lane), so the exponentiated tile goes from registers into the next product, and a
+// row's statistics live in one lane pair.  Unlike those, every operand is read as it lies in memory (attn_tile.h).
+// A workgroup of 4 waves owns 128 rows, 32 per wave, and walks only the keys between the first and the last that one of its
+// rows sees; a wave skips a 64-key tile none of its rows sees and leaves out the comparisons where all of them see all of it.
+// No atomics: results do not change from run to run.
+#include "attn_tile.h"
+
+namespace {
+
+constexpr int RB = 128;   // rows (queries or keys) of a workgroup
+constexpr int TB = 64;    // tokens per tile of the walked operand
+
+struct Ranged {
+  const bf16_t *q, *k, *v, *dout;
+  bf16_t *o, *dq, *dk, *dv;
+  float *lse, *delta, *part;          // part: f32 [2][splits][B][Nk][Hk * D] when splits > 1
+  const int32_t* ranges;              // [B][Nq][2] or null: every key
+  const float* slopes;                // [H]
+  int4* tiles;                        // [B][ceil(Nq / 32)] smallest lo, largest hi, largest lo, smallest hi of 32 queries
+  int64_t sq, sk, sv, so, sg;         // batch strides
+  int ldq, ldk, ldv, ldo, ldg;
+  int B, H, Hk, Nq, Nk, D, blocks, splits;
+  float scale;
+  ScoreMap map;
+};
+
+// lowest start of a running maximum: below every score that matters, and finite, so that a row that has seen nothing yet
+// needs no special case (its exponents are -inf, its sums 0)
+constexpr float M_NONE = -3.0e38f;
+
+__device__ __forceinline__ int2 row_range(const Ranged& a, int b, int q) {
+  if (!a.ranges) return make_int2(0, a.Nk);
+  const int2 r = *(const int2*)(a.ranges + ((int64_t)b * a.Nq + q) * 2);
+  return make_int2(max(r.x, 0), min(r.y, a.Nk));
+}
+
+// the walked interval of a workgroup and what its waves need to know about theirs
+struct Walk {
+  int begin, end;            // keys that some row of the workgroup sees
+  int lo_min, hi_max;        // of this wave's rows (an empty row: none)
+  int lo_max, hi_min;        // keys that all of them see
+};
+
+__device__ __forceinline__ Walk walk_of(int2 r, int wave, int (*sm)[2]) {
+  const bool empty = r.x >= r.y;
+  Walk w;
+  w.lo_min = wave_min_i(empty ? 0x7fffffff : r.x);
+  w.hi_max = wave_max_i(empty ? 0 : r.y);
+  w.lo_max = wave_max_i(empty ? 0x7fffffff : r.x);
+  w.hi_min = wave_min_i(empty ? 0 : r.y);
+  if ((threadIdx.x & 63) == 0) {
+    sm[wave][0] = w.lo_min;
+    sm[wave][1] = w.hi_max;
+  }
+  __syncthreads();
+  w.begin = min(min(sm[0][0], sm[1][0]), min(sm[2][0], sm[3][0]));
+  w.end = max(max(sm[0][1], sm[1][1]), max(sm[2][1], sm[3][1]));
+  w.begin = __builtin_amdgcn_readfirstlane(w.begin);
+  w.end = __builtin_amdgcn_readfirstlane(w.end);
+  return w;
+}
+
+template <int DH>
+__global__ __launch_bounds__(256, DH <= 64 ? 3 : 2) void ranged_fwd_kernel(const Ranged a) {
+  using T = Tile<DH>;
+  constexpr int KS = T::KS, DT = T::DT, NI = T::CPR / 4, STAGE = 2 * TB * T::ROW;
+  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];      // two stages of (K tile, V tile)
+  __shared__ int span[4][2];
+
+  const int t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int r = lane & 31, h = lane >> 5;
+  const int heads = a.H * a.B;
+  // the workgroups of the last rows first: with a causal mask they have the most keys
+  const int hb = blockIdx.x % heads, qb = a.blocks - 1 - blockIdx.x / heads;
+  const int b = hb / a.H, head = hb - b * a.H, khead = head / (a.H / a.Hk);
+  const int q0 = qb * RB + wave * 32, q = q0 + r, qr = min(q, a.Nq - 1);
+
+  const int2 range = row_range(a, b, qr);
+  const Walk w = walk_of(range, wave, span);
+  const bf16_t* K = a.k + b * a.sk + (int64_t)khead * a.D;
+  const bf16_t* V = a.v + b * a.sv + (int64_t)khead * a.D;
+
+  bf16x8 qf[KS];
+  load_frags<KS>(a.q + b * a.sq + (int64_t)qr * a.ldq + (int64_t)head * a.D, h, a.D, qf);
+  const float slope = a.map.biased ? a.slopes[head] * 1.4426950408889634f : 0.f;
+  const int pos = qr + a.Nk - a.Nq;
+  const unsigned len = (unsigned)max(range.y - range.x, 0);
+
+  f32x16 o[DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
+  float m_run = M_NONE, l_run = 0.f;
+  // the maximum may lag behind a row's by 2^LAG: p <= 256, and the accumulators are rescaled a few times per row, not per tile
+  constexpr float LAG = 8.f;
+
+  unsigned koffs[NI], voffs[NI];
+  T::template offsets<NI>(t, 256, a.ldk, a.D, koffs);
+  T::template offsets<NI>(t, 256, a.ldv, a.D, voffs);
+  int kr[KS], clo[DT], chi[DT];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) kr[ks] = T::row_off(r, ks, h);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) T::col_off(lane, dt, clo[dt], chi[dt]);
+
+  auto stage = [&](int kv0, char* buf) __attribute__((always_inline)) {
+    T::template stage<NI, TB>(K, kv0, w.end, a.ldk, a.D, koffs, wave, 4, buf);
+    T::template stage<NI, TB>(V, kv0, w.end, a.ldv, a.D, voffs, wave, 4, buf + TB * T::ROW);
+  };
+  if (w.begin < w.end) stage(w.begin, smem);
+  int cur = 0;
+  for (int kv0 = w.begin; kv0 < w.end; kv0 += TB) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();                 // the tile is in place, and every wave is done with the other buffer
+    const char* sK = smem + cur * STAGE;
+    const char* sV = sK + TB * T::ROW;
+    cur ^= 1;
+    if (kv0 + TB < w.end) stage(kv0 + TB, smem + cur * STAGE);
+    if (w.lo_min >= kv0 + TB || w.hi_max <= kv0) continue;       // no row of this wave sees the tile
+    const bool masked = w.lo_max > kv0 || w.hi_min < kv0 + TB;
+
+    f32x16 s[2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sK + kt * 32 * T::ROW, kr[ks]), qf[ks], ks == 0 ? zero : s[kt], 0, 0, 0);
+    }
+    if (a.map.cap_out != 0.f) {
+      asm volatile("" ::: "memory");           // (keeps these uniform conditions branches)
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float x = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[kt][e] * a.map.cap_in) + 1.f);
+          s[kt][e] = fmaf(-2.f * a.map.cap_out, x, a.map.cap_out);
+        }
+    }
+    if (a.map.biased) {
+      asm volatile("" ::: "memory");
+      const float f = a.map.cap_out != 0.f ? 1.f : a.map.scale;
+      const float d0 = (float)(pos - kv0 - 4 * h);
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[kt][e] = fmaf(-slope, fabsf(d0 - (float)(32 * kt + acc_row(e, 0))), s[kt][e] * f);
+    }
+    if (masked) {
+      asm volatile("" ::: "memory");
+      const unsigned k0 = (unsigned)(kv0 + 4 * h - range.x);
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (k0 + (unsigned)(32 * kt + acc_row(e, 0)) >= len) s[kt][e] = -INFINITY;
+    }
+    // ---- online softmax: a row is the lane pair (l, l + 32) ----
+    float mx = fmaxf(fmaxf(s[0][0], s[0][1]), s[1][0]);
+#pragma unroll
+    for (int e = 2; e < 16; e += 2) mx = fmaxf(fmaxf(mx, s[0][e]), s[0][e + 1]);
+#pragma unroll
+    for (int e = 1; e < 15; e += 2) mx = fmaxf(fmaxf(mx, s[1][e]), s[1][e + 1]);
+    mx = fmaxf(mx, s[1][15]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * a.map.mul;
+    if (__builtin_amdgcn_ballot_w64(mx > m_run + LAG) != 0) {
+      const float m_new = fmaxf(m_run, mx);
+      const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+      l_run *= alpha;
+#pragma unroll
+      for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
+      m_run = m_new;
+    }
+    const float nm = -m_run;
+    float ps0 = 0.f, ps1 = 0.f;
+    bf16x8 pf[2][2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      float p[16];
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        p[e] = __builtin_amdgcn_exp2f(fmaf(s[kt][e], a.map.mul, nm));
+        p[e + 1] = __builtin_amdgcn_exp2f(fmaf(s[kt][e + 1], a.map.mul, nm));
+        ps0 += p[e];
+        ps1 += p[e + 1];
+      }
+      pack_column(p, pf[kt]);       // bf16 operand of P V: half a step per probability, of random sign over the keys
+    }
+    l_run += ps0 + ps1;
+
+    if (masked) {
+      uint32_t bad = 0;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) bad |= not_finite(T::col_frag(sV + 16 * m * T::ROW, clo[dt], chi[dt]));
+      if (__builtin_amdgcn_ballot_w64(bad != 0) != 0) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          f32x16 hit = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int m = 0; m < 4; ++m) mfma_guarded(T::col_frag(sV + 16 * m * T::ROW, clo[dt], chi[dt]), pf[m >> 1][m & 1], o[dt], hit);
+          poison(o[dt], hit);
+        }
+        continue;
+      }
+    }
+    // ---- O^T += V^T P^T ----
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::col_frag(sV + 16 * m * T::ROW, clo[dt], chi[dt]), pf[m >> 1][m & 1], o[dt], 0, 0, 0);
+  }
+
+  const float l = l_run + __shfl_xor(l_run, 32, 64);
+  const bool none = range.x >= range.y;
+  const float inv = none ? 0.f : 1.0f / l;
+  if (q < a.Nq) {
+    if (a.lse && h == 0) a.lse[((int64_t)b * a.H + head) * a.Nq + q] = none ? INFINITY : m_run + __builtin_amdgcn_logf(l);
+    bf16_t* op = a.o + b * a.so + (int64_t)q * a.ldo + (int64_t)head * a.D;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int c = 32 * dt + 8 * g + 4 * h;
+        if (c < a.D) {
+          u16x4 ov;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ov.v[e] = f2bf(none ? 0.f : o[dt][4 * g + e] * inv);
+          *(u16x4*)(op + c) = ov;
+        }
+      }
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void put_rows(bf16_t* op, const f32x16 (&acc)[DT], float mul, int h, int D) {
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = 32 * dt + 8 * g + 4 * h;
+      if (c < D) {
+        u16x4 ov;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ov.v[e] = f2bf(acc[dt][4 * g + e] * mul);
+        *(u16x4*)(op + c) = ov;
+      }
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ void put_rows_f32(float* op, const f32x16 (&acc)[DT], float mul, int h, int D) {
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = 32 * dt + 8 * g + 4 * h;
+      if (c < D) {
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[dt][4 * g + e] * mul;
+        *(f32x4*)(op + c) = v;
+      }
+    }
+}
+
+// dQ and delta; also writes, for the second kernel, what the ranges of each 32 queries have in common
+template <int DH>
+__global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dq_kernel(const Ranged a) {
+  using T = Tile<DH>;
+  constexpr int KS = T::KS, DT = T::DT, NI = T::CPR / 4, STAGE = 2 * TB * T::ROW;
+  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
+  __shared__ int span[4][2];
+
+  const int t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int r = lane & 31, h = lane >> 5;
+  const int heads = a.H * a.B;
+  const int hb = blockIdx.x % heads, qb = a.blocks - 1 - blockIdx.x / heads;
+  const int b = hb / a.H, head = hb - b * a.H, khead = head / (a.H / a.Hk);
+  const int q0 = qb * RB + wave * 32, q = q0 + r, qr = min(q, a.Nq - 1);
+
+  const int2 range = row_range(a, b, qr);
+  const Walk w = walk_of(range, wave, span);
+  if (a.tiles && head == 0 && lane == 0 && q0 < a.Nq)
+    a.tiles[(int64_t)b * ((a.Nq + 31) / 32) + q0 / 32] = make_int4(w.lo_min, w.hi_max, w.lo_max, w.hi_min);
+  const bf16_t* K = a.k + b * a.sk + (int64_t)khead * a.D;
+  const bf16_t* V = a.v + b * a.sv + (int64_t)khead * a.D;
+
+  bf16x8 qf[KS], gf[KS];
+  load_frags<KS>(a.q + b * a.sq + (int64_t)qr * a.ldq + (int64_t)head * a.D, h, a.D, qf);
+  load_frags<KS>(a.dout + b * a.sg + (int64_t)qr * a.ldg + (int64_t)head * a.D, h, a.D, gf);
+  const int64_t stat = ((int64_t)b * a.H + head) * a.Nq + qr;
+  float delta = 0.f;
+  {
+    bf16x8 of[KS];
+    load_frags<KS>(a.o + b * a.so + (int64_t)qr * a.ldo + (int64_t)head * a.D, h, a.D, of);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) delta = fmaf((float)gf[ks][e], (float)of[ks][e], delta);
+    delta += __shfl_xor(delta, 32, 64);
+    if (q < a.Nq && h == 0) a.delta[stat] = delta;
+  }
+  const float nl = -a.lse[stat];
+  const float slope = a.map.biased ? a.slopes[head] * 1.4426950408889634f : 0.f;
+  const int pos = qr + a.Nk - a.Nq;
+  const unsigned len = (unsigned)max(range.y - range.x, 0);
+
+  f32x16 acc[DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
+  unsigned koffs[NI], voffs[NI];
+  T::template offsets<NI>(t, 256, a.ldk, a.D, koffs);
+  T::template offsets<NI>(t, 256, a.ldv, a.D, voffs);
+  int kr[KS], clo[DT], chi[DT];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) kr[ks] = T::row_off(r, ks, h);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) T::col_off(lane, dt, clo[dt], chi[dt]);
+
+  auto stage = [&](int kv0, char* buf) __attribute__((always_inline)) {
+    T::template stage<NI, TB>(K, kv0, w.end, a.ldk, a.D, koffs, wave, 4, buf);
+    T::template stage<NI, TB>(V, kv0, w.end, a.ldv, a.D, voffs, wave, 4, buf + TB * T::ROW);
+  };
+  if (w.begin < w.end) stage(w.begin, smem);
+  int cur = 0;
+  for (int kv0 = w.begin; kv0 < w.end; kv0 += TB) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    const char* sK = smem + cur * STAGE;
+    const char* sV = sK + TB * T::ROW;
+    cur ^= 1;
+    if (kv0 + TB < w.end) stage(kv0 + TB, smem + cur * STAGE);
+    if (w.lo_min >= kv0 + TB || w.hi_max <= kv0) continue;
+    const bool masked = w.lo_max > kv0 || w.hi_min < kv0 + TB;
+
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      f32x16 s, dp;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sK + kt * 32 * T::ROW, kr[ks]), qf[ks], ks == 0 ? zero : s, 0, 0, 0);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sV + kt * 32 * T::ROW, kr[ks]), gf[ks], ks == 0 ? zero : dp, 0, 0, 0);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dp[e] -= delta;
+      if (a.map.cap_out != 0.f) {
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float x = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[e] * a.map.cap_in) + 1.f);
+          s[e] = fmaf(-2.f * a.map.cap_out, x, a.map.cap_out);
+          dp[e] *= 4.f * x * (1.f - x);                       // 1 - tanh^2
+        }
+      }
+      if (a.map.biased) {
+        asm volatile("" ::: "memory");
+        const float f = a.map.cap_out != 0.f ? 1.f : a.map.scale;
+        const float d0 = (float)(pos - kv0 - 32 * kt - 4 * h);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = fmaf(-slope, fabsf(d0 - (float)acc_row(e, 0)), s[e] * f);
+      }
+      float ds[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) ds[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.map.mul, nl)) * dp[e];
+      if (masked) {
+        asm volatile("" ::: "memory");
+        const unsigned k0 = (unsigned)(kv0 + 32 * kt + 4 * h - range.x);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (k0 + (unsigned)acc_row(e, 0) >= len) ds[e] = 0.f;
+      }
+      bf16x8 df[2];
+      pack_column(ds, df);          // bf16 operand of dS K: half a step per element, of random sign over the keys
+      const char* sk = sK + 32 * kt * T::ROW;
+      if (masked) {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int ss = 0; ss < 2; ++ss) bad |= not_finite(T::col_frag(sk + 16 * ss * T::ROW, clo[dt], chi[dt]));
+        if (__builtin_amdgcn_ballot_w64(bad != 0) != 0) {
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) {
+            f32x16 hit = zero;
+#pragma unroll
+            for (int ss = 0; ss < 2; ++ss) mfma_guarded(T::col_frag(sk + 16 * ss * T::ROW, clo[dt], chi[dt]), df[ss], acc[dt], hit);
+            poison(acc[dt], hit);
+          }
+          continue;
+        }
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int ss = 0; ss < 2; ++ss)
+          acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::col_frag(sk + 16 * ss * T::ROW, clo[dt], chi[dt]), df[ss], acc[dt], 0, 0, 0);
+    }
+  }
+  if (q < a.Nq) put_rows<DT>(a.dq + ((int64_t)b * a.Nq + q) * a.H * a.D + (int64_t)head * a.D, acc, a.scale, h, a.D);
+}
+
+// dK and dV of 128 keys: walks the query tiles of every head that shares the key head.  With few workgroups the walk is cut
+// into `splits` parts whose sums are added afterwards in their order.
+template <int DH>
+__global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dkv_kernel(const Ranged a) {
+  using T = Tile<DH>;
+  constexpr int KS = T::KS, DT = T::DT, NI = T::CPR / 4, STAGE = 2 * TB * T::ROW + 4 * TB * 4;
+  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];      // two stages of (Q, dO, and lse, delta, lo, hi of the rows)
+
+  const int t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int r = lane & 31, h = lane >> 5;
+  const int heads = a.Hk * a.B, group = a.H / a.Hk;
+  const int hb = blockIdx.x % heads, kb = blockIdx.x / heads;       // the first keys first: with a causal mask most rows see them
+  const int b = hb / a.Hk, khead = hb - b * a.Hk;
+  const int k0 = kb * RB, kw = k0 + wave * 32, key = kw + r, kc = min(key, a.Nk - 1);
+  const int kend = min(k0 + RB, a.Nk);
+
+  bf16x8 kf[KS], vf[KS];
+  load_frags<KS>(a.k + b * a.sk + (int64_t)kc * a.ldk + (int64_t)khead * a.D, h, a.D, kf);
+  load_frags<KS>(a.v + b * a.sv + (int64_t)kc * a.ldv + (int64_t)khead * a.D, h, a.D, vf);
+  f32x16 dk[DT], dv[DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dk[i][e] = dv[i][e] = 0.f;
+
+  unsigned qoffs[NI], goffs[NI];
+  T::template offsets<NI>(t, 256, a.ldq, a.D, qoffs);
+  T::template offsets<NI>(t, 256, a.ldg, a.D, goffs);
+  int rr[KS], clo[DT], chi[DT];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) rr[ks] = T::row_off(r, ks, h);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) T::col_off(lane, dt, clo[dt], chi[dt]);
+
+  const int nqt = (a.Nq + TB - 1) / TB, nsub = (a.Nq + 31) / 32;
+  const int64_t work = (int64_t)group * nqt;
+  const int first = (int)(work * blockIdx.y / a.splits), last = (int)(work * (blockIdx.y + 1) / a.splits);
+  const int4* tiles = a.ranges ? a.tiles + (int64_t)b * nsub : nullptr;
+
+  // next unit of work from i on whose 64 queries see one of this workgroup's keys
+  auto next = [&](int i) __attribute__((always_inline)) {
+    for (; i < last && tiles; ++i) {
+      const int qt = i % nqt;
+      const int4 x = tiles[2 * qt];
+      int lo = x.x, hi = x.y;
+      if (2 * qt + 1 < nsub) {
+        const int4 y = tiles[2 * qt + 1];
+        lo = min(lo, y.x);
+        hi = max(hi, y.y);
+      }
+      if (lo < kend && hi > k0) break;
+    }
+    return __builtin_amdgcn_readfirstlane(i);
+  };
+  auto stage = [&](int i, char* buf) __attribute__((always_inline)) {
+    const int gi = i / nqt, qt = i - gi * nqt, head = khead * group + gi, q0 = qt * TB;
+    T::template stage<NI, TB>(a.q + b * a.sq + (int64_t)head * a.D, q0, a.Nq, a.ldq, a.D, qoffs, wave, 4, buf);
+    T::template stage<NI, TB>(a.dout + b * a.sg + (int64_t)head * a.D, q0, a.Nq, a.ldg, a.D, goffs, wave, 4, buf + TB * T::ROW);
+    // one wave per row statistic; rows past the end read zeros (their q and dO are zeros too: they add nothing)
+    const int rows = min(TB, a.Nq - q0);
+    const int64_t st = ((int64_t)b * a.H + head) * a.Nq + q0;
+    if (wave < 2 || a.ranges) {
+      const void* base = wave == 0 ? (const void*)(a.lse + st) : wave == 1 ? (const void*)(a.delta + st)
+                                                                           : (const void*)(a.ranges + ((int64_t)b * a.Nq + q0) * 2);
+      const unsigned off = wave < 2 ? lane * 4u : lane * 8u + (wave == 3 ? 4u : 0u);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)base, 0, rows * (wave < 2 ? 4 : 8), 0x00020000),
+                                               (__attribute__((address_space(3))) void*)(buf + 2 * TB * T::ROW + wave * TB * 4), 4, off, 0, 0, 0);
+    }
+  };
+
+  int cur = 0, i = next(first);
+  if (i < last) stage(i, smem);
+  while (i < last) {
+    const int j = next(i + 1);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    const char* sQ = smem + cur * STAGE;
+    const char* sG = sQ + TB * T::ROW;
+    const float* sL = (const float*)(sG + TB * T::ROW);
+    cur ^= 1;
+    if (j < last) stage(j, smem + cur * STAGE);
+    const int gi = i / nqt, qt = i - gi * nqt, head = khead * group + gi;
+    const float slope = a.map.biased ? a.slopes[head] * 1.4426950408889634f : 0.f;
+    i = j;
+
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      bool masked = false;
+      if (tiles) {
+        if (2 * qt + u >= nsub) continue;
+        const int4 x = tiles[2 * qt + u];
+        if (x.x >= kw + 32 || x.y <= kw) continue;          // none of these queries sees a key of this wave
+        masked = x.z > kw || x.w < kw + 32;
+      }
+      const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      f32x16 s, dp;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sQ + u * 32 * T::ROW, rr[ks]), kf[ks], ks == 0 ? zero : s, 0, 0, 0);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sG + u * 32 * T::ROW, rr[ks]), vf[ks], ks == 0 ? zero : dp, 0, 0, 0);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 d4 = *(const f32x4*)(sL + TB + 32 * u + 8 * g + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dp[4 * g + e] -= d4[e];
+      }
+      if (a.map.cap_out != 0.f) {
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float x = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[e] * a.map.cap_in) + 1.f);
+          s[e] = fmaf(-2.f * a.map.cap_out, x, a.map.cap_out);
+          dp[e] *= 4.f * x * (1.f - x);
+        }
+      }
+      if (a.map.biased) {
+        asm volatile("" ::: "memory");
+        const float f = a.map.cap_out != 0.f ? 1.f : a.map.scale;
+        const float d0 = (float)(qt * TB + 32 * u + 4 * h + a.Nk - a.Nq - kc);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = fmaf(-slope, fabsf(d0 + (float)acc_row(e, 0)), s[e] * f);
+      }
+      float p[16], ds[16];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 l4 = *(const f32x4*)(sL + 32 * u + 8 * g + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], a.map.mul, -l4[e]));
+          ds[4 * g + e] = p[4 * g + e] * dp[4 * g + e];
+        }
+      }
+      if (masked) {
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int4 lo = *(const int4*)(sL + 2 * TB + 32 * u + 8 * g + 4 * h);
+          const int4 hi = *(const int4*)(sL + 3 * TB + 32 * u + 8 * g + 4 * h);
+          const int l[4] = {lo.x, lo.y, lo.z, lo.w}, g4[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (kc < l[e] || kc >= g4[e]) p[4 * g + e] = ds[4 * g + e] = 0.f;
+        }
+      }
+      bf16x8 pf[2], df[2];
+      pack_column(p, pf);
+      pack_column(ds, df);
+      const char* sq = sQ + 32 * u * T::ROW;
+      const char* sg = sG + 32 * u * T::ROW;
+      if (masked) {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int ss = 0; ss < 2; ++ss) {
+            bad |= not_finite(T::col_frag(sq + 16 * ss * T::ROW, clo[dt], chi[dt]));
+            bad |= not_finite(T::col_frag(sg + 16 * ss * T::ROW, clo[dt], chi[dt]));
+          }
+        if (__builtin_amdgcn_ballot_w64(bad != 0) != 0) {
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) {
+            f32x16 hq = zero, hg = zero;
+#pragma unroll
+            for (int ss = 0; ss < 2; ++ss) {
+              mfma_guarded(T::col_frag(sg + 16 * ss * T::ROW, clo[dt], chi[dt]), pf[ss], dv[dt], hg);
+              mfma_guarded(T::col_frag(sq + 16 * ss * T::ROW, clo[dt], chi[dt]), df[ss], dk[dt], hq);
+            }
+            poison(dv[dt], hg);
+            poison(dk[dt], hq);
+          }
+          continue;
+        }
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int ss = 0; ss < 2; ++ss) {
+          dv[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::col_frag(sg + 16 * ss * T::ROW, clo[dt], chi[dt]), pf[ss], dv[dt], 0, 0, 0);
+          dk[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::col_frag(sq + 16 * ss * T::ROW, clo[dt], chi[dt]), df[ss], dk[dt], 0, 0, 0);
+        }
+    }
+  }
+  if (key < a.Nk) {
+    const int64_t at = ((int64_t)b * a.Nk + key) * a.Hk * a.D + (int64_t)khead * a.D;
+    if (a.splits > 1) {
+      const int64_t all = (int64_t)a.B * a.Nk * a.Hk * a.D;
+      put_rows_f32<DT>(a.part + (int64_t)blockIdx.y * all + at, dk, a.scale, h, a.D);
+      put_rows_f32<DT>(a.part + (int64_t)(a.splits + blockIdx.y) * all + at, dv, 1.f, h, a.D);
+    } else {
+      put_rows<DT>(a.dk + at, dk, a.scale, h, a.D);
+      put_rows<DT>(a.dv + at, dv, 1.f, h, a.D);
+    }
+  }
+}
+
+// The interval of keys that each query of a packed, padded or generated batch sees (see lbmk_key_ranges)
+__global__ __launch_bounds__(256) void key_ranges_kernel(int32_t* out, const int32_t* offsets, const int32_t* prefix, const int32_t* lens,
+                                                         int B, int Nq, int Nk, int docs, int64_t so, int causal, int window) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (int64_t)B * Nq) return;
+  const int b = (int)(i / Nq), pos = (int)(i - (int64_t)b * Nq) + Nk - Nq;
+  int lo = 0, hi = lens ? min(max(lens[b], 0), Nk) : Nk;
+  if (offsets) {
+    // the document: the last offset at or below the position (offsets ascend; a search over anything else still ends)
+    const int32_t* o = offsets + b * so;
+    int l = 0, r = docs;                    // o[l] <= pos < o[r] once found
+    if (pos < o[0] || pos >= o[docs]) {
+      lo = hi = 0;                          // padding in front of the first or behind the last document
+    } else {
+      while (r - l > 1) {
+        const int m = (l + r) >> 1;
+        if (o[m] <= pos) l = m;
+        else r = m;
+      }
+      lo = max(o[l], 0);
+      hi = min(hi, o[r]);
+    }
+  }
+  int last = causal ? pos + 1 : hi;
+  if (prefix) last = max(last, min(lo, Nk) + min(max(prefix[b], 0), Nk));      // the first tokens (of each document) are seen by all
+  hi = min(hi, last);
+  if (window > 0) lo = max(lo, pos + 1 - window);
+  if (pos < 0 || lo >= hi) lo = hi = 0;
+  *(int2*)(out + 2 * i) = make_int2(lo, hi);
+}
+
+int pad_head(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 160; }
+
+// splits of the key kernel's walk: enough workgroups for two per CU, at least four tiles each, at most eight parts
+int dkv_splits(int B, int H, int Hk, int Nq, int Nk) {
+  const int64_t blocks = (int64_t)((Nk + RB - 1) / RB) * Hk * B, work = (int64_t)(H / Hk) * ((Nq + TB - 1) / TB);
+  int64_t s = (2ll * lbmk_num_cus() + blocks - 1) / (blocks > 0 ? blocks : 1);
+  if (s > work / 4) s = work / 4;
+  return (int)(s < 1 ? 1 : s > 8 ? 8 : s);
+}
+
+int ranged_check(const lbmk_ranged_attn_desc* p, bool bwd) {
+  LBMK_REQUIRE(p, "ranged_attn: null descriptor");
+  LBMK_REQUIRE(p->D >= 8 && p->D <= 160 && p->D % 8 == 0, "ranged_attn: head_dim %d (8 ... 160, a multiple of 8)", p->D);
+  LBMK_REQUIRE(p->H > 0 && p->Hk > 0 && p->H % p->Hk == 0, "ranged_attn: %d heads over %d key heads", p->H, p->Hk);
+  LBMK_REQUIRE(p->B >= 0 && p->Nq >= 0 && p->Nk >= 0, "ranged_attn: negative sizes");
+  LBMK_REQUIRE((int64_t)p->B * p->H * ((p->Nq + RB - 1) / RB) < (1ll << 31) && (int64_t)p->B * p->Hk * ((p->Nk + RB - 1) / RB) < (1ll << 31) &&
+                   p->Nq < (1 << 30) && p->Nk < (1 << 30) && (int64_t)(p->H / p->Hk) * ((p->Nq + TB - 1) / TB) < (1ll << 31),
+               "ranged_attn: sizes");
+  LBMK_REQUIRE(p->scale > 0.f && p->cap >= 0.f, "ranged_attn: scale %g, cap %g", (double)p->scale, (double)p->cap);
+  if (p->B == 0 || p->Nq == 0) return LBMK_OK;
+  const void* ptr[8] = {p->q, p->o, p->dout, p->dq, p->k, p->v, p->dk, p->dv};
+  const int ld[8] = {p->ldq, p->ldo, p->ldg, 0, p->ldk, p->ldv, 0, 0};
+  const int64_t st[8] = {p->sq, p->so, p->sg, 0, p->sk, p->sv, 0, 0};
+  for (int i = 0; i < 8; ++i) {
+    if (!bwd && (i == 2 || i == 3 || i >= 6)) continue;
+    if (i >= 4 && p->Nk == 0) continue;
+    LBMK_REQUIRE(ptr[i] && lbmk_aligned(ptr[i], 16), "ranged_attn: null or misaligned pointer (rows start on 16 bytes)");
+    if (i == 3 || i >= 6) continue;
+    const int64_t wide = (int64_t)(i < 4 ? p->H : p->Hk) * p->D;
+    LBMK_REQUIRE(ld[i] % 8 == 0 && ld[i] >= wide && ld[i] <= (1 << 23) && st[i] % 8 == 0 && st[i] >= 0, "ranged_attn: row stride %d, batch stride %lld",
+                 ld[i], (long long)st[i]);
+  }
+  LBMK_REQUIRE(!p->ranges || lbmk_aligned(p->ranges, 8), "ranged_attn: misaligned ranges");
+  LBMK_REQUIRE(!p->slopes || lbmk_aligned(p->slopes, 4), "ranged_attn: misaligned slopes");
+  if (bwd) LBMK_REQUIRE(p->lse && p->scratch && lbmk_aligned(p->scratch, 16), "ranged_attn_bwd: no log-sum-exp or scratch");
+  return LBMK_OK;
+}
+
+Ranged ranged_args(const lbmk_ranged_attn_desc* p) {
+  Ranged a = {};
+  a.q = (const bf16_t*)p->q; a.k = (const bf16_t*)p->k; a.v = (const bf16_t*)p->v; a.dout = (const bf16_t*)p->dout;
+  a.o = (bf16_t*)p->o; a.dq = (bf16_t*)p->dq; a.dk = (bf16_t*)p->dk; a.dv = (bf16_t*)p->dv;
+  a.lse = p->lse;
+  a.ranges = p->ranges;
+  a.slopes = p->slopes;
+  a.sq = p->sq; a.sk = p->sk; a.sv = p->sv; a.so = p->so; a.sg = p->sg;
+  a.ldq = p->ldq; a.ldk = p->ldk; a.ldv = p->ldv; a.ldo = p->ldo; a.ldg = p->ldg;
+  a.B = p->B; a.H = p->H; a.Hk = p->Hk; a.Nq = p->Nq; a.Nk = p->Nk; a.D = p->D;
+  a.splits = 1;
+  a.scale = p->scale;
+  const float log2e = 1.4426950408889634f;
+  a.map.scale = p->scale * log2e;
+  a.map.cap_in = p->cap > 0.f ? 2.f * p->scale * log2e / p->cap : 0.f;
+  a.map.cap_out = p->cap * log2e;
+  a.map.biased = p->slopes != nullptr;
+  a.map.mul = p->cap > 0.f || p->slopes ? 1.f : a.map.scale;
+  return a;
+}
+
+#define BY_HEAD(DHP, KERNEL, GRID)                                                               \
+  switch (DHP) {                                                                                 \
+    case 32: hipLaunchKernelGGL((KERNEL<32>), GRID, dim3(256), 0, s, a); break;                  \
+    case 64: hipLaunchKernelGGL((KERNEL<64>), GRID, dim3(256), 0, s, a); break;                  \
+    case 96: hipLaunchKernelGGL((KERNEL<96>), GRID, dim3(256), 0, s, a); break;                  \
+    case 128: hipLaunchKernelGGL((KERNEL<128>), GRID, dim3(256), 0, s, a); break;                \
+    default: hipLaunchKernelGGL((KERNEL<160>), GRID, dim3(256), 0, s, a); break;                 \
+  }
+
+__global__ __launch_bounds__(256) void sum_splits_kernel(const float* __restrict__ part, bf16_t* dk, bf16_t* dv, int64_t n, int splits) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;       // n is a multiple of 8
+  if (i >= 2 * n) return;
+  const bool second = i >= n;
+  const float* p = part + (second ? (int64_t)splits * n + (i - n) : i);
+  f32x4 v = *(const f32x4*)p;
+  for (int s = 1; s < splits; ++s) v += *(const f32x4*)(p + (int64_t)s * n);
+  u16x4 o;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o.v[e] = f2bf(v[e]);
+  *(u16x4*)((second ? dv : dk) + (second ? i - n : i)) = o;
+}
+
+}  // namespace
+
+extern "C" int lbmk_key_ranges(int32_t* ranges, const int32_t* doc_offsets, int docs, int64_t doc_stride, const int32_t* prefix,
+                               const int32_t* lens, int B, int Nq, int Nk, int causal, int window, void* stream) {
+  LBMK_REQUIRE(B >= 0 && Nq >= 0 && Nk >= 0 && Nq < (1 << 30) && Nk < (1 << 30) && window >= 0 && (int64_t)B * Nq < (1ll << 38), "key_ranges: sizes");
+  if (B == 0 || Nq == 0) return LBMK_OK;
+  LBMK_REQUIRE(ranges && lbmk_aligned(ranges, 8), "key_ranges: null or misaligned output");
+  LBMK_REQUIRE(!doc_offsets || docs >= 1, "key_ranges: %d documents", docs);
+  hipLaunchKernelGGL(key_ranges_kernel, dim3((unsigned)(((int64_t)B * Nq + 255) / 256)), dim3(256), 0, (hipStream_t)stream, ranges, doc_offsets, prefix,
+                     lens, B, Nq, Nk, docs, doc_stride, causal, window);
+  return lbmk_check_launch("key_ranges");
+}
+
+extern "C" int lbmk_ranged_attn(const lbmk_ranged_attn_desc* p, void* stream) {
+  const int rc = ranged_check(p, false);
+  if (rc != LBMK_OK) return rc;
+  if (p->B == 0 || p->Nq == 0) return LBMK_OK;
+  Ranged a = ranged_args(p);
+  a.blocks = (a.Nq + RB - 1) / RB;
+  hipStream_t s = (hipStream_t)stream;
+  BY_HEAD(pad_head(a.D), ranged_fwd_kernel, dim3(a.blocks * a.H * a.B));
+  return lbmk_check_launch("ranged_attn");
+}
+
+// delta [B][H][Nq], the summaries of the queries' ranges, and the parts of the key kernel
+extern "C" int64_t lbmk_ranged_attn_bwd_scratch_floats(int B, int H, int Hk, int Nq, int Nk, int D) {
+  if (B <= 0 || H <= 0 || Hk <= 0 || Nq <= 0 || H % Hk) return 0;
+  const int64_t delta = ((int64_t)B * H * Nq + 3) / 4 * 4, tiles = (int64_t)B * ((Nq + 31) / 32) * 4;
+  const int splits = dkv_splits(B, H, Hk, Nq, Nk);
+  return delta + tiles + (splits > 1 ? 2ll * splits * B * Nk * Hk * D : 0);
+}
+
+extern "C" int lbmk_ranged_attn_bwd(const lbmk_ranged_attn_desc* p, void* stream) {
+  const int rc = ranged_check(p, true);
+  if (rc != LBMK_OK) return rc;
+  if (p->B == 0 || p->Nq == 0) return LBMK_OK;
+  Ranged a = ranged_args(p);
+  a.delta = p->scratch;
+  a.tiles = (int4*)(p->scratch + ((int64_t)a.B * a.H * a.Nq + 3) / 4 * 4);
+  hipStream_t s = (hipStream_t)stream;
+  a.blocks = (a.Nq + RB - 1) / RB;
+  BY_HEAD(pad_head(a.D), ranged_bwd_dq_kernel, dim3(a.blocks * a.H * a.B));
+  if (a.Nk > 0) {
+    a.splits = dkv_splits(a.B, a.H, a.Hk, a.Nq, a.Nk);
+    a.part = (float*)(a.tiles + (int64_t)a.B * ((a.Nq + 31) / 32));
+    BY_HEAD(pad_head(a.D), ranged_bwd_dkv_kernel, dim3((a.Nk + RB - 1) / RB * a.Hk * a.B, a.splits));
+    if (a.splits > 1) {
+      const int64_t n = (int64_t)a.B * a.Nk * a.Hk * a.D;
+      hipLaunchKernelGGL(sum_splits_kernel, dim3((unsigned)((2 * n / 4 + 255) / 256)), dim3(256), 0, s, a.part, a.dk, a.dv, n, a.splits);
+    }
+  }
+  return lbmk_check_launch("ranged_attn_bwd");
+}

@@ -1,0 +1,151 @@
+// Tiles of bf16 rows in LDS and the MFMA operands read from them, shared by the attention kernels over key ranges.
+//
+// A tile is R rows (tokens) x DH channels as they lie in memory; it is written by LDS-DMA, lane-linear, and read in two
+// ways: as rows (16 bytes = 8 channels of one token: operand with the channel along k) and transposed with
+// ds_read_b64_tr_b16 (8 tokens of one channel: operand with the token along k).  So neither K / V nor Q / dO need a
+// channel-major copy in memory.  The 16-byte slots of a row are XOR-swizzled so that both kinds of reads touch every bank
+// once: 16 rows x one slot, and 4 rows x 4 neighbouring slots.
+#pragma once
+#include "common.h"
+
+namespace {
+
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(8))) short s16x8;
+
+constexpr unsigned TILE_OOB = 0x80000000u;     // a byte offset that every descriptor refuses: the chunk reads as zeros
+
+template <int DH>
+struct Tile {
+  static constexpr int CPR = DH / 8;           // 16-byte chunks per row
+  static constexpr int ROW = DH * 2;           // bytes per row
+  static constexpr int KS = DH / 16;           // 16-deep MFMA steps over the channels
+  static constexpr int DT = DH / 32;           // 32-channel tiles
+
+  // 256 bytes of banks hold 256 / ROW rows: the swizzle supplies the bits that the row offset does not
+  static __device__ __forceinline__ int swz(int row) {
+    if constexpr (DH % 128 == 0) return ((row & 3) << 2) | ((row >> 2) & 3);
+    else if constexpr (DH % 64 == 0) return ((row & 2) << 1) | ((row >> 2) & 3);
+    else return (row >> 2) & 3;
+  }
+  // byte offsets of this thread's chunks within a tile of the source (D real channels, row stride ld)
+  template <int NI>
+  static __device__ __forceinline__ void offsets(int t, int threads, int ld, int D, unsigned (&off)[NI]) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int idx = i * threads + t, row = idx / CPR, c = (idx % CPR) ^ swz(row);
+      off[i] = c * 8 < D ? (unsigned)row * (unsigned)ld * 2u + (unsigned)c * 16u : TILE_OOB;
+    }
+  }
+  // stages rows [row0, min(row0 + R, end)) of src; rows from `end` on read as zeros.  `wave` is wave-uniform
+  template <int NI, int R>
+  static __device__ __forceinline__ void stage(const bf16_t* src, int64_t row0, int end, int ld, int D, const unsigned (&off)[NI],
+                                               int wave, int waves, char* dst) {
+    const int rows = min(R, end - (int)row0);
+    const int bytes = ((rows - 1) * ld + D) * 2;
+    const bf16_t* base = src + row0 * ld;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) buffer_lds16(base, bytes, off[i], 0, dst + (i * waves + wave) * 1024);
+  }
+  // operand with the channel along k: row `row`, channels 16 ks + 8 h .. + 7
+  static __device__ __forceinline__ int row_off(int row, int ks, int h) { return row * ROW + (((2 * ks + h) ^ swz(row)) << 4); }
+  static __device__ __forceinline__ bf16x8 row_frag(const char* tile, int off) { return *(const bf16x8*)(tile + off); }
+  // operand with the token along k: channels 32 dt + (lane & 31), tokens 8 h .. 8 h + 7 (+ 16 m: add 16 m ROW): offsets of the
+  // two transposing reads
+  static __device__ __forceinline__ void col_off(int lane, int dt, int& lo, int& hi) {
+    const int l = lane & 15, h = lane >> 5, b = (lane >> 4) & 1;
+    const int ra = 8 * h + (l >> 2), rb = ra + 4, ch = 4 * dt + 2 * b + ((l & 3) >> 1);
+    lo = ra * ROW + 16 * (ch ^ swz(ra)) + 8 * (l & 1);
+    hi = rb * ROW + 16 * (ch ^ swz(rb)) + 8 * (l & 1);
+  }
+  static __device__ __forceinline__ bf16x8 col_frag(const char* tile, int lo, int hi) {
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(tile + lo));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(tile + hi));
+    const s16x8 v = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    return __builtin_bit_cast(bf16x8, v);
+  }
+};
+
+// lane (r, h) <- X[row][16 ks + 8 h .. + 7], zero from channel D on
+template <int KS>
+__device__ __forceinline__ void load_frags(const bf16_t* row, int h, int D, bf16x8 (&f)[KS]) {
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    if (16 * ks + 8 * h < D) f[ks] = *(const bf16x8*)(row + 16 * ks + 8 * h);
+    else
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[ks][e] = (__bf16)0.f;
+  }
+}
+
+// An accumulator column (32 rows of k over the lane pair l, l + 32, in fours) as two 8-deep operand slices per lane: after the
+// bf16 pack the pair swaps halves, so a lane holds rows 16 ss + 8 h .. + 7
+__device__ __forceinline__ void pack_column(const float (&p)[16], bf16x8 (&f)[2]) {
+#pragma unroll
+  for (int ss = 0; ss < 2; ++ss) {
+    bf16x8 v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (__bf16)p[8 * ss + e];
+    const u32x4 w = __builtin_bit_cast(u32x4, v);
+    const auto s0 = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+    const auto s1 = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+    const u32x4 x = {s0[0], s1[0], s0[1], s1[1]};
+    f[ss] = __builtin_bit_cast(bf16x8, x);
+  }
+}
+
+// Masked places hold 0 in one operand, and 0 * inf or 0 * NaN in the other would poison a sum that must not see them.  A tile
+// with masked places is therefore scanned; in the rare case that it holds a value that is not finite, its products take
+// the finite values alone, and a second product of indicators (not finite x not masked) says which sums become NaN.
+__device__ __forceinline__ uint32_t not_finite(bf16x8 v) {      // != 0: some element is inf or NaN
+  const u32x4 w = __builtin_bit_cast(u32x4, v);
+  uint32_t a = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a |= (w[i] & 0x7f807f80u) + 0x00800080u;
+  return a & 0x80008000u;
+}
+__device__ __forceinline__ void mfma_guarded(bf16x8 a, bf16x8 b, f32x16& acc, f32x16& hit) {
+  bf16x8 fin, ind, pat;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint16_t bits = __builtin_bit_cast(uint16_t, (__bf16)a[e]);
+    const bool ok = (bits & 0x7f80) != 0x7f80;
+    fin[e] = ok ? (__bf16)a[e] : (__bf16)0.f;
+    ind[e] = ok ? (__bf16)0.f : (__bf16)1.f;
+    pat[e] = (__builtin_bit_cast(uint16_t, (__bf16)b[e]) & 0x7fff) ? (__bf16)1.f : (__bf16)0.f;
+  }
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fin, b, acc, 0, 0, 0);
+  hit = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ind, pat, hit, 0, 0, 0);
+}
+__device__ __forceinline__ void poison(f32x16& acc, const f32x16& hit) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    if (hit[e] > 0.f) acc[e] = __builtin_nanf("");
+}
+
+// row of accumulator element e in lane half h
+__device__ __forceinline__ constexpr int acc_row(int e, int h) { return (e & 3) + 8 * (e >> 2) + 4 * h; }
+
+__device__ __forceinline__ int wave_min_i(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int wave_max_i(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
+// What turns a product q.k into the exponent (base 2) of the softmax:
+//   cap:  C tanh(scale q.k / cap), C = cap log2(e), tanh(x) = 1 - 2 / (exp(2 x) + 1)        bias: - slope |distance|
+// Without either the scaling is left to the fused multiply-add that subtracts the maximum.
+struct ScoreMap {
+  float mul;        // factor still to be applied to a mapped score (scale * log2(e), or 1 when cap or bias already did)
+  float scale;      // scale * log2(e)
+  float cap_in;     // 2 scale log2(e) / cap
+  float cap_out;    // cap log2(e); 0: no cap
+  int biased;
+};
+
+}  // namespace

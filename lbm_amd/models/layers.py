@@ -188,6 +188,17 @@ def qk_norm_rope(q, k, head_dim: int, q_weight, k_weight, table=None, positions=
     return ops.qk_norm_rope(q, k, head_dim, q_weight, k_weight, table, positions, eps=eps, interleaved=interleaved)
 
 
+def ranged_attention(q, k, v, heads: int, kv_heads: int, head_dim: int, ranges=None, *, scale=None, cap: float = 0.0, slopes=None):
+    """Attention in which every query sees one interval of keys (ops.key_ranges), with capped or distance-biased scores and
+    grouped key heads; differentiable in q, k and v (the slopes are constants).  Arguments: ops.ranged_attn."""
+    if training(q, k, v, slopes):
+        if slopes is not None and slopes.requires_grad:
+            raise NotImplementedError("ranged_attention has no gradient for the slopes: pass slopes.detach()")
+        from ..autograd import RangedAttentionFn
+        return RangedAttentionFn.apply(q, k, v, heads, kv_heads, head_dim, ranges, scale, cap, slopes)
+    return ops.ranged_attn(q, k, v, heads, kv_heads, head_dim, ranges, scale=scale, cap=cap, slopes=slopes)
+
+
 def fused_rows(module: _Cached, name: str, layers, bias: bool):
     """Packs several Linear layers that share an input into one [sum N, K] weight."""
     params = []

@@ -15,7 +15,7 @@ from typing import Optional
 import torch
 
 from . import _C
-from ._C import ACT_GEGLU, ACT_NONE, ACT_RELU, ACT_SILU, DT_BF16, DT_F32, IgemmDesc, NormRopeDesc, check, lib
+from ._C import ACT_GEGLU, ACT_NONE, ACT_RELU, ACT_SILU, DT_BF16, DT_F32, CachedAttnDesc, IgemmDesc, NormRopeDesc, RangedAttnDesc, check, lib
 
 bf16 = torch.bfloat16
 
@@ -1555,3 +1555,151 @@ def qk_norm_rope_bwd(q, k, dq_out, dk_out, head_dim: int, q_weight, k_weight, ta
     with _on(q):
         check(lib.lbmk_norm_rope_bwd(C.byref(d), scratch.data_ptr(), _ptr(dwq), _ptr(dwk), _stream()), "lbmk_norm_rope_bwd")
     return dq, dk, dwq, dwk
+
+
+# --------------------------------------------------------------------------------------
+# token operators: attention over key ranges, and over a cache
+# --------------------------------------------------------------------------------------
+def key_ranges(B: int, Nq: int, Nk: Optional[int] = None, *, causal: bool = False, window: int = 0,
+               prefix: Optional[torch.Tensor] = None, documents: Optional[torch.Tensor] = None,
+               lens: Optional[torch.Tensor] = None, device=None) -> torch.Tensor:
+    """The interval of keys that each query sees, int32 [B, Nq, 2] (first, one behind the last; equal: none): the mask that
+    ``ranged_attn`` takes, made once per batch and used by every layer.  Query i stands at position p = i + Nk - Nq.
+
+    documents: int32 [n + 1] or [B, n + 1] ascending token counts; a query sees its own document, a position outside all of
+    them nothing.  causal: keys up to p.  window (with causal): only the last ``window`` of those.  prefix (with causal,
+    int32 [B]): the first tokens of each document are seen by all its queries.  lens: int32 [B], keys from there on are
+    padding."""
+    Nk = Nq if Nk is None else Nk
+    _want(B >= 0 and Nq >= 0 and Nk >= 0 and window >= 0, f"key_ranges: B {B}, Nq {Nq}, Nk {Nk}, window {window}")
+    _want(causal or (window == 0 and prefix is None), "key_ranges: window and prefix go with causal")
+    _want(window == 0 or prefix is None, "key_ranges: a window with a prefix is no interval")
+    given = [t for t in (prefix, documents, lens) if t is not None]
+    for name, t in (("prefix", prefix), ("lens", lens)):
+        _want(t is None or (t.dtype == torch.int32 and t.shape == (B,) and t.is_contiguous()), f"{name}: contiguous int32 [{B}]")
+    if documents is not None:
+        _want(documents.dtype == torch.int32 and documents.is_contiguous() and documents.shape[-1] >= 2 and
+              (documents.dim() == 1 or (documents.dim() == 2 and documents.shape[0] == B)),
+              f"documents: contiguous int32 [n + 1] or [{B}, n + 1] token counts")
+    if given:
+        _same_device(given[0], *given[1:])
+        _want(device is None or torch.device(device).type == given[0].device.type, f"key_ranges: operands on {given[0].device}, device {device}")
+    dev = given[0].device if given else torch.device(device if device is not None else "cuda")
+    if dev.type != "cuda":
+        raise RuntimeError("lbm_amd kernels run on the GPU only; there is no CPU fallback")
+    out = torch.empty(B, Nq, 2, dtype=torch.int32, device=dev)
+    docs = documents.shape[-1] - 1 if documents is not None else 0
+    with _on(out):
+        check(lib.lbmk_key_ranges(out.data_ptr(), _ptr(documents), docs, docs + 1 if documents is not None and documents.dim() == 2 else 0,
+                                  _ptr(prefix), _ptr(lens), B, Nq, Nk, 1 if causal else 0, window, _stream()), "lbmk_key_ranges")
+    return out
+
+
+def _score_args(name, d, head_dim, scale, cap, slopes, heads, like):
+    scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
+    _want(0 < scale < math.inf, f"{name}: scale {scale} (positive)")
+    _want(0 <= cap < math.inf, f"{name}: cap {cap} (0: none)")
+    if slopes is not None:
+        _want(slopes.dtype == torch.float32 and slopes.shape == (heads,) and slopes.is_contiguous(), f"slopes: contiguous f32 [{heads}]")
+        _same_device(like, slopes)
+    d.scale, d.cap, d.slopes = scale, float(cap), _ptr(slopes)
+
+
+def _attn_rows(name, t, heads, head_dim, B, dtype=bf16):
+    _want(t.dtype == dtype, f"{name}: {t.dtype} (the kernels over key ranges take bf16)")
+    _want(t.dim() == 3 and (B is None or t.shape[0] == B), f"{name}: [{'B' if B is None else B}, N, {heads * head_dim}] expected, got {tuple(t.shape)}")
+    t = _token_rows(name, t, heads, head_dim)
+    _want(_ld(t) <= 1 << 23, f"{name}: row stride {_ld(t)}")
+    return t
+
+
+def _ranged_desc(q, k, v, heads, kv_heads, head_dim, ranges, scale, cap, slopes) -> RangedAttnDesc:
+    _want(head_dim % 8 == 0 and 8 <= head_dim <= 160, f"ranged_attn: head_dim {head_dim} (8 ... 160, a multiple of 8)")
+    _want(heads > 0 and kv_heads > 0 and heads % kv_heads == 0, f"ranged_attn: {heads} heads over {kv_heads} key heads")
+    q = _attn_rows("q", q, heads, head_dim, None)
+    B = q.shape[0]
+    k, v = _attn_rows("k", k, kv_heads, head_dim, B), _attn_rows("v", v, kv_heads, head_dim, B)
+    _want(k.shape == v.shape, f"ranged_attn: k {tuple(k.shape)}, v {tuple(v.shape)}")
+    _same_device(q, k, v, ranges)
+    d = RangedAttnDesc()
+    if ranges is not None:
+        _want(ranges.dtype == torch.int32 and tuple(ranges.shape) == (B, q.shape[1], 2) and ranges.is_contiguous() and ranges.data_ptr() % 8 == 0,
+              f"ranges: contiguous int32 [{B}, {q.shape[1]}, 2] (key_ranges)")
+        d.ranges = ranges.data_ptr()
+    _score_args("ranged_attn", d, head_dim, scale, cap, slopes, heads, q)
+    _need_gpu(q)
+    d.q, d.k, d.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    d.B, d.H, d.Hk, d.Nq, d.Nk, d.D = B, heads, kv_heads, q.shape[1], k.shape[1], head_dim
+    d.ldq, d.ldk, d.ldv, d.sq, d.sk, d.sv = _ld(q), _ld(k), _ld(v), _sb(q), _sb(k), _sb(v)
+    return d
+
+
+def ranged_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, kv_heads: int, head_dim: int,
+                ranges: Optional[torch.Tensor] = None, *, scale: Optional[float] = None, cap: float = 0.0,
+                slopes: Optional[torch.Tensor] = None, return_lse: bool = False):
+    """Attention in which query i of row b sees the keys ranges[b, i, 0] .. ranges[b, i, 1] - 1 (``key_ranges``, or any int32
+    [B, Nq, 2], clipped to the keys; None: all): o = softmax(s) v, s = cap * tanh(scale q.k / cap) - slopes[h] * distance, with
+    cap 0 for no cap and slopes (f32 [heads]) None for no bias; the distance is |i + Nk - Nq - j|.  A query that sees no key
+    gets zeros, and what q, k, v hold at places that are not seen has no influence.
+
+    q: bf16 [B, Nq, heads * D], k / v: bf16 [B, Nk, kv_heads * D] (column windows of packed projections pass), key head
+    h // (heads // kv_heads) serves head h; D a multiple of 8 up to 160.  ``return_lse``: also the f32 [B, heads, Nq]
+    log2-sum-exp rows that ``ranged_attn_bwd`` takes.  Not differentiable: models.layers.ranged_attention is."""
+    d = _ranged_desc(q, k, v, heads, kv_heads, head_dim, ranges, scale, cap, slopes)
+    o = torch.empty(d.B, d.Nq, heads * head_dim, dtype=bf16, device=q.device)
+    lse = torch.empty(d.B, heads, d.Nq, dtype=torch.float32, device=q.device) if return_lse else None
+    d.o, d.lse, d.ldo, d.so = o.data_ptr(), _ptr(lse), heads * head_dim, o.stride(0)
+    with _on(q):
+        check(lib.lbmk_ranged_attn(C.byref(d), _stream()), "lbmk_ranged_attn")
+    return (o, lse) if return_lse else o
+
+
+def ranged_attn_bwd(q, k, v, o, do, lse, heads: int, kv_heads: int, head_dim: int, ranges=None, *, scale: Optional[float] = None,
+                    cap: float = 0.0, slopes=None):
+    """Gradients (dq, dk, dv) of ``ranged_attn`` for its output ``o``, the output's gradient ``do`` and the rows ``lse``; the
+    gradients of shared key heads are summed in a fixed order."""
+    d = _ranged_desc(q, k, v, heads, kv_heads, head_dim, ranges, scale, cap, slopes)
+    o, do = _attn_rows("o", o, heads, head_dim, d.B), _attn_rows("do", do, heads, head_dim, d.B)
+    _want(o.shape == q.shape and do.shape == q.shape, "ranged_attn_bwd: o and do have q's shape")
+    _want(lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (d.B, heads, d.Nq), f"lse: contiguous f32 [{d.B}, {heads}, {d.Nq}]")
+    _same_device(q, o, do, lse)
+    new = torch.empty if d.Nq and d.B else torch.zeros      # without queries the keys' gradients are zeros that no kernel writes
+    dq, dk, dv = (new(t.shape, dtype=bf16, device=q.device) for t in (q, k, v))
+    scratch = torch.empty(lib.lbmk_ranged_attn_bwd_scratch_floats(d.B, heads, kv_heads, d.Nq, d.Nk, head_dim), dtype=torch.float32, device=q.device)
+    d.o, d.dout, d.lse, d.scratch = o.data_ptr(), do.data_ptr(), lse.data_ptr(), scratch.data_ptr()
+    d.dq, d.dk, d.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    d.ldo, d.ldg, d.so, d.sg = _ld(o), _ld(do), _sb(o), _sb(do)
+    with _on(q):
+        check(lib.lbmk_ranged_attn_bwd(C.byref(d), _stream()), "lbmk_ranged_attn_bwd")
+    return dq, dk, dv
+
+
+def cached_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lens: torch.Tensor, heads: int, kv_heads: int,
+                head_dim: int, *, scale: Optional[float] = None, cap: float = 0.0, slopes: Optional[torch.Tensor] = None,
+                window: int = 0) -> torch.Tensor:
+    """``ranged_attn`` for the n newest tokens of each request over caches that already hold their keys and values.
+    q: bf16 [B, n, heads * D]; caches: bf16 [B, rows, kv_heads * D] (any row and batch stride); lens: int32 [B] on the device,
+    tokens in each cache with the new ones (clipped to [0, rows]).  New token i stands at lens - n + i and sees the keys up to
+    itself (``window`` > 0: the last ``window`` of them); a token in front of the cache's start gets zeros.  Cache rows from
+    lens on are not read.  The keys are split over workgroups by the device's own lengths, so a captured call follows them."""
+    _want(head_dim % 8 == 0 and 8 <= head_dim <= 160, f"cached_attn: head_dim {head_dim} (8 ... 160, a multiple of 8)")
+    _want(heads > 0 and kv_heads > 0 and heads % kv_heads == 0, f"cached_attn: {heads} heads over {kv_heads} key heads")
+    _want(window >= 0, f"cached_attn: window {window}")
+    q = _attn_rows("q", q, heads, head_dim, None)
+    B, n = q.shape[:2]
+    k, v = _attn_rows("k_cache", k_cache, kv_heads, head_dim, B), _attn_rows("v_cache", v_cache, kv_heads, head_dim, B)
+    _want(k.shape == v.shape, f"cached_attn: k_cache {tuple(k.shape)}, v_cache {tuple(v.shape)}")
+    _want(lens.dtype == torch.int32 and tuple(lens.shape) == (B,) and lens.is_contiguous(), f"lens: contiguous int32 [{B}]")
+    _same_device(q, k, v, lens)
+    d = CachedAttnDesc()
+    _score_args("cached_attn", d, head_dim, scale, cap, slopes, heads, q)
+    _need_gpu(q)
+    o = torch.empty(B, n, heads * head_dim, dtype=bf16, device=q.device)
+    nfl = lib.lbmk_cached_attn_scratch_floats(B, heads, kv_heads, n, k.shape[1], head_dim)
+    scratch = torch.empty(nfl, dtype=torch.float32, device=q.device) if nfl else None
+    d.q, d.k, d.v, d.o, d.lens, d.scratch = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lens.data_ptr(), _ptr(scratch)
+    d.B, d.H, d.Hk, d.n, d.cap_rows, d.D, d.window = B, heads, kv_heads, n, k.shape[1], head_dim, window
+    d.ldq, d.ldk, d.ldv, d.sq, d.sk, d.sv = _ld(q), _ld(k), _ld(v), _sb(q), _sb(k), _sb(v)
+    with _on(q):
+        check(lib.lbmk_cached_attn(C.byref(d), _stream()), "lbmk_cached_attn")
+    return o
