@@ -113,6 +113,12 @@ typedef struct lbmk_igemm_desc {
                            returns the same bits either way (the choice may depend on the batch size, the result
                            does not).  For the few-row, deep-K layers of a small batch (256 ... 1024 tokens against
                            K up to 23,040: 20 ... 80 tiles on 256 CUs)                                            */
+  const void* lr_t;     /* lr_up != NULL: low-rank adapters of many requests beside a linear layer (bf16, 1x1, batch 1, */
+  const void* lr_up;    /* alpha 1): acc[m][n] += sum_k lr_t[m][k] * lr_up[a][n][k] before the epilogue, a = lr_index[m / lr_rows]; */
+  const int32_t* lr_index; /* a outside [0, lr_count): no adapter, the row of lr_t is not read.  lr_t: bf16 [M][lr_k], columns from */
+  int32_t lr_rank;      /* lr_rank on zeros (lbmk_adapter_down); lr_up: bf16 [lr_count][N][lr_rank]; lr_k = lr_rank rounded  */
+  int32_t lr_k;         /* up to 32.  Tiles 12, 13, 14, 17, 18 (Cin % 64 == 0), 3 (otherwise)                            */
+  int32_t lr_rows, lr_count;
 } lbmk_igemm_desc;
 
 int lbmk_igemm(const lbmk_igemm_desc* d, void* stream);
@@ -168,6 +174,22 @@ int lbmk_groupnorm_from_partials(const void* x, void* y, const float* gamma, con
 /* LayerNorm over the last dim of [rows][C] bf16 (BasicTransformerBlock norm1/2/3, eps 1e-5). */
 int lbmk_layernorm(const void* x, void* y, const float* gamma, const float* beta,
                    int rows, int C, float eps, void* stream);
+
+/* ------------------------------------------------------------------------
+ * A linear layer shared by many requests, each with a low-rank adapter of its own or none:
+ *   y[m] = x[m] W^T + bias + scaling[a] (x[m] down[a]^T) up[a]^T,   a = index[m / rows]  (outside [0, count): no adapter)
+ * No counterpart in the reference; stands next to lbmk_igemm.  lbmk_adapter_down writes t[m] = scaling[a] x[m] down[a]^T (bf16
+ * [requests * rows][tk], tk = rank rounded up to 32, columns from rank on zeros; rows without an adapter are left as they are);
+ * lbmk_igemm with lr_* fields, or for up to lbmk_adapter_few_rows() rows lbmk_adapter_linear_few, adds t up[a]^T to the shared
+ * product in f32, before y is rounded.
+ *   x : bf16 [requests * rows][ldx], K channels (a multiple of 8);  down : bf16 [count][rank][K];  up : bf16 [count][N][rank];
+ *   w : bf16 [N][ldw];  bias : f32 [N] or NULL;  scaling : f32 [count] or NULL (ones);  index : int32 [requests];  rank 1 ... 256
+ * ---------------------------------------------------------------------- */
+int lbmk_adapter_down(const void* x, const void* down, const int32_t* index, const float* scaling, void* t, int requests, int rows,
+                      int K, int64_t ldx, int rank, int tk, int count, void* stream);
+int lbmk_adapter_few_rows(void);
+int lbmk_adapter_linear_few(const void* x, const void* w, const float* bias, const void* t, const void* up, const int32_t* index, void* y,
+                            int requests, int rows, int N, int K, int64_t ldx, int ldw, int64_t ldy, int rank, int tk, int count, void* stream);
 
 /* ------------------------------------------------------------------------
  * RMS norm of every query / key head and the rotation by the token's position, in one pass:

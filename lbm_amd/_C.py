@@ -51,6 +51,7 @@ class IgemmDesc(C.Structure):
         ("out_up2", i32), ("gn_nslab", i32), ("gn_strip_off", i32),
         ("smx_mode", i32), ("smx_max", vp), ("smx_part", vp),
         ("f32_chunks", i32), ("f32_part", vp),
+        ("lr_t", vp), ("lr_up", vp), ("lr_index", vp), ("lr_rank", i32), ("lr_k", i32), ("lr_rows", i32), ("lr_count", i32),
     ]
 
 
@@ -90,6 +91,9 @@ SIGNATURES = {
     "lbmk_groupnorm_static_max_floats": (i64, []),
     "lbmk_groupnorm_static": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, f32, i32, vp]),
     "lbmk_layernorm": (i32, [vp, vp, vp, vp, i32, i32, f32, vp]),
+    "lbmk_adapter_down": (i32, [vp] * 5 + [i32, i32, i32, i64, i32, i32, i32, vp]),
+    "lbmk_adapter_few_rows": (i32, []),
+    "lbmk_adapter_linear_few": (i32, [vp] * 7 + [i32, i32, i32, i32, i64, i32, i64, i32, i32, i32, vp]),
     "lbmk_norm_rope": (i32, [C.POINTER(NormRopeDesc), vp]),
     "lbmk_norm_rope_bwd_scratch_floats": (i64, [i32]),
     "lbmk_norm_rope_bwd": (i32, [C.POINTER(NormRopeDesc), vp, vp, vp, vp]),

@@ -1,0 +1,184 @@
+// A projection shared by many requests, each with a low-rank adapter of its own (or none):
+//
+//   y[m] = x[m] W^T + bias + t[m] B_a^T          t[m] = s_a x[m] A_a^T          a = index[request of row m]
+//
+// The factor products are a few per cent of the shared one, so what costs is reading x again and every launch.  Two steps:
+//   * adapter_down: t, bf16 (its half step is relative to the adapter's own share of y).  16 rows x 16 ranks per wave on
+//     v_mfma_f32_16x16x32_bf16, both operands K-contiguous and read straight into registers; the four waves of a workgroup
+//     split K and are joined in LDS in a fixed order, because there are too few row groups to fill the chip otherwise.
+//   * the shared product with t B_a^T added to its accumulators before the one rounding of y: many rows in lbmk_igemm
+//     (lr_* fields), few rows here: with up to 64 rows the weight is read once and its bytes are the floor, so a workgroup
+//     of 8 waves takes 16 output columns, its waves split K, and W goes from memory into MFMA operands without LDS.
+#include "common.h"
+
+namespace {
+
+__device__ __forceinline__ bf16x8 zero8() {
+  const u32x4 z = {0u, 0u, 0u, 0u};
+  return __builtin_bit_cast(bf16x8, z);
+}
+
+constexpr int DOWN_WAVES = 4;
+
+// grid: (ceil(rank / 16), ceil(rows / 16) * requests)
+__global__ __launch_bounds__(64 * DOWN_WAVES) void adapter_down_kernel(const bf16_t* __restrict__ x, const bf16_t* __restrict__ down,
+                                                                      const int32_t* __restrict__ index, const float* __restrict__ scaling,
+                                                                      bf16_t* __restrict__ t, int rows, int K, int64_t ldx, int rank, int tk,
+                                                                      int count) {
+  __shared__ f32x4 part[DOWN_WAVES][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 15, lq = lane >> 4;
+  const int groups = (rows + 15) / 16, request = blockIdx.y / groups, m0 = (blockIdx.y - request * groups) * 16, r0 = blockIdx.x * 16;
+  const int a = index[request];
+  if ((unsigned)a >= (unsigned)count) return;                  // no adapter: nobody reads these rows of t
+  const int m = min(m0 + lr, rows - 1), n = min(r0 + lr, rank - 1);
+  const bf16_t* xr = x + ((int64_t)request * rows + m) * ldx + 8 * lq;
+  const bf16_t* dr = down + ((int64_t)a * rank + n) * K + 8 * lq;
+  // K in chunks of 32: an equal, contiguous share per wave
+  const int chunks = (K + 31) / 32, per = (chunks + DOWN_WAVES - 1) / DOWN_WAVES;
+  const int c0 = wave * per, c1 = min(c0 + per, chunks);
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 5
+  for (int c = c0; c < c1; ++c) {
+    const bool in = 32 * c + 8 * lq < K;                       // K % 8 == 0
+    const bf16x8 fd = in ? *(const bf16x8*)(dr + 32 * c) : zero8(), fx = in ? *(const bf16x8*)(xr + 32 * c) : zero8();
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fd, fx, acc, 0, 0, 0);
+  }
+  part[wave][lane] = acc;
+  __syncthreads();
+  if (wave != 0) return;
+#pragma unroll
+  for (int w = 1; w < DOWN_WAVES; ++w) acc += part[w][lane];
+  if (m0 + lr >= rows) return;
+  const float s = scaling ? scaling[a] : 1.f;
+  // lane: row m0 + lr, ranks r0 + 4 lq .. + 3; ranks from `rank` on are zeros
+  u16x4 o;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o.v[e] = f2bf(r0 + 4 * lq + e < rank ? acc[e] * s : 0.f);
+  *(u16x4*)(t + ((int64_t)request * rows + m0 + lr) * tk + r0 + 4 * lq) = o;
+}
+
+constexpr int FEW_WAVES = 8, FEW_ROWS = 64;
+
+// MT: row groups of 16
+template <int MT>
+__global__ __launch_bounds__(64 * FEW_WAVES) void adapter_few_kernel(const bf16_t* __restrict__ x, const bf16_t* __restrict__ w,
+                                                                   const float* __restrict__ bias, const bf16_t* __restrict__ t,
+                                                                   const bf16_t* __restrict__ up, const int32_t* __restrict__ index,
+                                                                   bf16_t* __restrict__ y, int M, int rows, int N, int K, int64_t ldx, int ldw,
+                                                                   int64_t ldy, int rank, int tk, int count) {
+  __shared__ f32x4 part[FEW_WAVES][MT][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 15, lq = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const bf16_t* wr = w + (int64_t)min(n0 + lr, N - 1) * ldw + 8 * lq;
+  const bf16_t* xr[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) xr[i] = x + (int64_t)min(16 * i + lr, M - 1) * ldx + 8 * lq;
+  f32x4 acc[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int chunks = (K + 31) / 32;
+  // the waves take chunks in turn: eight of them read 512 consecutive bytes of each row of W
+#pragma unroll 4
+  for (int c = wave; c < chunks; c += FEW_WAVES) {
+    const bool in = 32 * c + 8 * lq < K;
+    const bf16x8 fw = in ? *(const bf16x8*)(wr + 32 * c) : zero8();
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const bf16x8 fx = in ? *(const bf16x8*)(xr[i] + 32 * c) : zero8();
+      acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw, fx, acc[i], 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) part[wave][i][lane] = acc[i];
+  __syncthreads();
+  // output (m, n): four neighbouring columns per thread, as they lie in the accumulators
+  for (int o = threadIdx.x; o < MT * 64; o += 64 * FEW_WAVES) {
+    const int i = o >> 6, l = o & 63, m = 16 * i + (l & 15), n = n0 + 4 * (l >> 4);
+    if (m >= M || n >= N) continue;                            // N % 4 == 0
+    f32x4 v = part[0][i][l];
+#pragma unroll
+    for (int k = 1; k < FEW_WAVES; ++k) v += part[k][i][l];
+    if (bias)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += bias[n + e];
+    const int a = index[m / rows];
+    if ((unsigned)a < (unsigned)count) {
+      const bf16_t* tr = t + (int64_t)m * tk;
+      const bf16_t* ur = up + ((int64_t)a * N + n) * rank;
+      f32x4 d = {0.f, 0.f, 0.f, 0.f};
+      if ((rank & 7) == 0) {
+        for (int k = 0; k < rank; k += 8) {
+          const u16x8 tv = *(const u16x8*)(tr + k);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const u16x8 uv = *(const u16x8*)(ur + (int64_t)e * rank + k);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) d[e] = fmaf(bf2f(tv.v[q]), bf2f(uv.v[q]), d[e]);
+          }
+        }
+      } else {
+        for (int k = 0; k < rank; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) d[e] = fmaf(bf2f(tr[k]), bf2f(ur[(int64_t)e * rank + k]), d[e]);
+      }
+      v += d;
+    }
+    u16x4 ov;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ov.v[e] = f2bf(v[e]);
+    *(u16x4*)(y + (int64_t)m * ldy + n) = ov;
+  }
+}
+
+}  // namespace
+
+extern "C" int lbmk_adapter_down(const void* x, const void* down, const int32_t* index, const float* scaling, void* t, int requests,
+                                 int rows, int K, int64_t ldx, int rank, int tk, int count, void* stream) {
+  LBMK_REQUIRE(requests >= 0 && rows >= 0 && K > 0 && K % 8 == 0 && rank > 0 && rank <= 256 && count > 0, "adapter_down: sizes");
+  LBMK_REQUIRE(tk % 32 == 0 && tk >= rank && tk - rank < 32, "adapter_down: t has %d columns for rank %d (rounded up to 32)", tk, rank);
+  if (requests == 0 || rows == 0) return LBMK_OK;
+  LBMK_REQUIRE(x && down && index && t && lbmk_aligned(x, 16) && lbmk_aligned(down, 16) && lbmk_aligned(t, 16) && lbmk_aligned(index, 4) &&
+                   (!scaling || lbmk_aligned(scaling, 4)), "adapter_down: null or misaligned pointer");
+  LBMK_REQUIRE(ldx % 8 == 0 && ldx >= K, "adapter_down: row stride %lld", (long long)ldx);
+  const int64_t groups = (int64_t)requests * ((rows + 15) / 16);
+  LBMK_REQUIRE(groups < (1ll << 31) && (int64_t)requests * rows < (1ll << 31), "adapter_down: too many rows");
+  // (grid.y carries the row groups and is limited to 65535: larger batches go in slices of whole requests)
+  const int per = (rows + 15) / 16, most = 65535 / per;
+  LBMK_REQUIRE(most > 0, "adapter_down: %d rows per request (at most %d)", rows, 65535 * 16);
+  for (int r = 0; r < requests; r += most) {
+    const int n = requests - r < most ? requests - r : most;
+    hipLaunchKernelGGL(adapter_down_kernel, dim3(tk / 16, n * per), dim3(64 * DOWN_WAVES), 0, (hipStream_t)stream,
+                       (const bf16_t*)x + (int64_t)r * rows * ldx, (const bf16_t*)down, index + r, scaling, (bf16_t*)t + (int64_t)r * rows * tk, rows, K,
+                       ldx, rank, tk, count);
+  }
+  return lbmk_check_launch("adapter_down");
+}
+
+extern "C" int lbmk_adapter_few_rows(void) { return FEW_ROWS; }
+
+extern "C" int lbmk_adapter_linear_few(const void* x, const void* w, const float* bias, const void* t, const void* up, const int32_t* index,
+                                       void* y, int requests, int rows, int N, int K, int64_t ldx, int ldw, int64_t ldy, int rank, int tk, int count,
+                                       void* stream) {
+  LBMK_REQUIRE(requests >= 0 && rows >= 0 && (int64_t)requests * rows <= FEW_ROWS, "adapter_linear_few: %d requests of %d rows (at most %d rows)",
+               requests, rows, FEW_ROWS);
+  LBMK_REQUIRE(N > 0 && N % 4 == 0 && K > 0 && K % 8 == 0 && rank > 0 && rank <= 256 && count > 0 && tk % 32 == 0 && tk >= rank, "adapter_linear_few: sizes");
+  if (requests == 0 || rows == 0) return LBMK_OK;
+  LBMK_REQUIRE(x && w && t && up && index && y && lbmk_aligned(x, 16) && lbmk_aligned(w, 16) && lbmk_aligned(t, 16) &&
+                   lbmk_aligned(up, rank % 8 == 0 ? 16 : 2) && lbmk_aligned(index, 4) && lbmk_aligned(y, 8) && (!bias || lbmk_aligned(bias, 4)),
+               "adapter_linear_few: null or misaligned pointer");
+  LBMK_REQUIRE(ldx % 8 == 0 && ldx >= K && ldw % 8 == 0 && ldw >= K && ldy % 4 == 0 && ldy >= N, "adapter_linear_few: row strides");
+  const int M = requests * rows;
+#define FEW(MT)                                                                                                                    \
+  hipLaunchKernelGGL((adapter_few_kernel<MT>), dim3((N + 15) / 16), dim3(64 * FEW_WAVES), 0, (hipStream_t)stream, (const bf16_t*)x, \
+                     (const bf16_t*)w, bias, (const bf16_t*)t, (const bf16_t*)up, index, (bf16_t*)y, M, rows, N, K, ldx, ldw, ldy, rank, tk, count)
+  switch ((M + 15) / 16) {
+    case 1: FEW(1); break;
+    case 2: FEW(2); break;
+    case 3: FEW(3); break;
+    default: FEW(4); break;
+  }
+#undef FEW
+  return lbmk_check_launch("adapter_linear_few");
+}

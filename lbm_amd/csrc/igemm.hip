@@ -430,6 +430,62 @@ __device__ __forceinline__ void igemm_epilogue_smx(const lbmk_igemm_desc& p, f32
   }
 }
 
+// Low-rank adapters of many requests (lr_* fields): acc[m][n] += sum_k t[m][k] up[a][n][k], a the adapter of the request that
+// row m belongs to, in the accumulators before the epilogue's one rounding.  The rank is a few MFMA steps deep, so the operands
+// come straight from memory (L2): no staging, and nothing in the K loop.  A 16-row group that holds rows of two requests keeps a
+// product only in the lanes of its own rows (a lane holds one row): a request never sees another one's adapter, NaN included.
+template <int MI, int NI>
+__device__ __forceinline__ void igemm_low_rank(const lbmk_igemm_desc& p, f32x4 (&acc)[MI][NI], int mbase, int nbase, int lane) {
+  const int lr = lane & 15, lq = lane >> 4;
+  const int last = min(mbase + MI * 16, p.M) - 1;
+  if (mbase > last) return;
+  const bf16_t* __restrict__ t = (const bf16_t*)p.lr_t;
+  const bf16_t* __restrict__ up = (const bf16_t*)p.lr_up;
+  const int b1 = last / p.lr_rows;
+  for (int b = mbase / p.lr_rows; b <= b1; ++b) {
+    const int a = __builtin_amdgcn_readfirstlane(p.lr_index[b]);
+    if ((unsigned)a >= (unsigned)p.lr_count) continue;
+    const int r0 = b * p.lr_rows, r1 = min(r0 + p.lr_rows, p.M);
+    const bf16_t* ua = up + (int64_t)a * p.N * p.lr_rank;
+    for (int k0 = 0; k0 < p.lr_k; k0 += 32) {
+      const int k = k0 + 8 * lq;
+      bf16x8 fu[NI];
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        const int n = nbase + 16 * j + lr;
+        u16x8 v = {{0, 0, 0, 0, 0, 0, 0, 0}};
+        if (n < p.N) {
+          const bf16_t* u = ua + (int64_t)n * p.lr_rank + k;
+          if ((p.lr_rank & 7) == 0) {
+            if (k < p.lr_rank) v = *(const u16x8*)u;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (k + e < p.lr_rank) v.v[e] = u[e];
+          }
+        }
+        fu[j] = __builtin_bit_cast(bf16x8, v);
+      }
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const int g0 = mbase + 16 * i, m = g0 + lr;
+        if (g0 >= r1 || g0 + 16 <= r0) continue;
+        const bool mine = m >= r0 && m < r1;
+        const bf16x8 ft = *(const bf16x8*)(t + (int64_t)(mine ? m : max(r0, g0)) * p.lr_k + k);
+        const bool whole = g0 >= r0 && g0 + 16 <= r1;
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+          const f32x4 v = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fu[j], ft, acc[i][j], 0, 0, 0);
+          if (whole) acc[i][j] = v;
+          else
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][e] = mine ? v[e] : acc[i][j][e];
+        }
+      }
+    }
+  }
+}
+
 // FAST: Cin % 64 == 0 -- every lane of a K-tile is on the same filter tap, so the
 // tap / channel walk is scalar and a load costs three vector ALU instructions.
 // OCC: workgroups meant to share a CU (caps the register budget at 512 / (OCC * waves per SIMD)).
@@ -445,6 +501,7 @@ __device__ __forceinline__ void igemm_epilogue_smx(const lbmk_igemm_desc& p, f32
 // hundred cycles, so every wave issues its loads in its READ phase only, behind its fragment reads.  For that to meet the
 // landing deadlines the activation tile has two stage buffers whose halves are staged by the group that does not read
 // them, and the weight tile (read by both groups) has three.
+// SMX: 1 / 2 the two passes of a row softmax, 3 a product with low-rank adapters (igemm_low_rank)
 template <int BM, int BN, int WAVES_M, int WAVES_N, bool DBUF, bool FAST, bool STAMP = false, int OCC = 1, bool GNS = false, bool ROWA = false, bool PP = false, int SMX = 0>
 __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, (WAVES_M * WAVES_N * OCC + 3) / 4) void igemm_kernel(const lbmk_igemm_desc p) {
   constexpr int NW = WAVES_M * WAVES_N;         // waves per workgroup (4 or 8)
@@ -973,7 +1030,8 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, (WAVES_M * WAVES_N * OCC + 
 
   DBG_C(7);
   DBG_T(3);
-  if constexpr (SMX != 0) {
+  if constexpr (SMX == 3) igemm_low_rank<MI, NI>(p, acc, m0 + wm * WM, n0 + wn * WN, lane);
+  if constexpr (SMX == 1 || SMX == 2) {
     igemm_epilogue_smx<MI, NI, SMX>(p, acc, m0 + wm * WM, n0 + wn * WN, lane, zo, (int)blockIdx.z, (n0 / BN) * WAVES_N + wn,
                                     tiles_n * WAVES_N);
     return;
@@ -1031,6 +1089,14 @@ inline bool pp_ok(const lbmk_igemm_desc& d) {
   return d.stride == 1 && !d.up2 && d.pad_t == 1 && d.pad_l == 1 && d.OH == d.IH && d.OW == d.IW;
 }
 
+// tiles that are built with the low-rank adapter product: one per size class of the linear layers
+inline bool low_rank_tile(int tile) { return tile == 3 || tile == 12 || tile == 13 || tile == 14 || tile == 17 || tile == 18; }
+template <int BM, int BN, int WMs, int WNs, bool DBUF, bool FAST, int OCC = 1, bool PP = false>
+void launch_low_rank(const lbmk_igemm_desc& d, hipStream_t s) {
+  const int tm = (d.M + BM - 1) / BM, tn = (d.N + BN - 1) / BN;
+  hipLaunchKernelGGL((igemm_kernel<BM, BN, WMs, WNs, DBUF, FAST, false, OCC, false, false, PP, 3>), dim3((unsigned)(tm * tn)), dim3(64 * WMs * WNs), 0, s, d);
+}
+
 template <int BM, int BN, int WMs, int WNs, bool DBUF, bool STAMP = false, int OCC = 1, bool ROWA = false, bool PP = false>
 void launch(const lbmk_igemm_desc& d, hipStream_t s) {
   const int tm = (d.M + BM - 1) / BM, tn = (d.N + BN - 1) / BN;
@@ -1072,6 +1138,7 @@ int lbmk_igemm_f32_launch(const lbmk_igemm_desc* d, void* stream);     // fp32.h
 
 extern "C" int lbmk_igemm(const lbmk_igemm_desc* dp, void* stream) {
   LBMK_REQUIRE(dp != nullptr, "igemm: null descriptor");
+  LBMK_REQUIRE(!dp->lr_up || (!dp->in_f32 && !dp->smx_mode), "igemm: adapters go with a bf16 linear layer");
   if (dp->in_f32) return lbmk_igemm_f32_launch(dp, stream);      // fp32 mode: f32 operands on the f32-input MFMA
   lbmk_igemm_desc d = *dp;
   LBMK_REQUIRE(d.a && d.w && d.out, "igemm: null operand");
@@ -1138,9 +1205,19 @@ extern "C" int lbmk_igemm(const lbmk_igemm_desc* dp, void* stream) {
       hipLaunchKernelGGL((igemm_kernel<256, 256, 4, 4, true, true, false, 1, false, false, false, 2>), grid, dim3(1024), 0, (hipStream_t)stream, d);
     return lbmk_check_launch("igemm");
   }
+  const bool low_rank = d.lr_up != nullptr;
+  if (low_rank) {
+    LBMK_REQUIRE(d.KH == 1 && d.batch == 1 && d.alpha == 1.f && !gn && !d.out_up2 && d.act != LBMK_ACT_GEGLU && !d.rowvec && d.IH == 1 && d.IW == 1,
+                 "igemm: adapters go with a plain linear layer");
+    LBMK_REQUIRE(d.lr_t && d.lr_index && d.lr_count > 0 && d.lr_rows > 0 && d.M % d.lr_rows == 0, "igemm: adapters of %d rows per request over %d rows",
+                 d.lr_rows, d.M);
+    LBMK_REQUIRE(d.lr_rank > 0 && d.lr_rank <= 256 && d.lr_k % 32 == 0 && d.lr_k >= d.lr_rank, "igemm: adapter rank %d (t has %d columns)", d.lr_rank, d.lr_k);
+    LBMK_REQUIRE(lbmk_aligned(d.lr_t, 16) && lbmk_aligned(d.lr_up, d.lr_rank % 8 == 0 ? 16 : 2) && lbmk_aligned(d.lr_index, 4), "igemm: misaligned adapter");
+  }
   int tile = d.tile;
+  if (low_rank && !fast_path(d)) tile = 3;
   if (tile < 0) {
-    if (d.act != LBMK_ACT_GEGLU && d.N <= 16) tile = 2;
+    if (d.act != LBMK_ACT_GEGLU && d.N <= 16 && !low_rank) tile = 2;
     else if (rowa_enabled() && rowa_ok(d) && d.N >= 96 && d.N <= 128 && d.M >= 65536) tile = 15;   // measured 6-20 % ahead of every other tile on these
     else {
       // Cost model over the production tiles: time of the busiest CU.  A CU holding w workgroups of a
@@ -1166,7 +1243,9 @@ extern "C" int lbmk_igemm(const lbmk_igemm_desc* dp, void* stream) {
       const int nkt = (d.K + 63) / 64;
       double best = 1e300;
       tile = 0;
+      if (low_rank) tile = 13;
       for (const Cand& c : cands) {
+        if (low_rank && (c.tile == 3 || !low_rank_tile(c.tile))) continue;
         if (gn && !(c.tile == 0 || c.tile == 7 || c.tile == 8 || c.tile == 10 || c.tile == 14 || c.tile == 15 || c.tile == 17)) continue;   // statistics strips are 64 rows per wave, column groups in pairs
         if (d.act == LBMK_ACT_GEGLU && (c.tile == 11 || c.tile == 18)) continue;   // odd number of column groups per wave
         if ((c.tile == 17 || c.tile == 18) && !(pp_enabled() && pp_ok(d))) continue;
@@ -1194,6 +1273,18 @@ extern "C" int lbmk_igemm(const lbmk_igemm_desc* dp, void* stream) {
   if (tile == 15) LBMK_REQUIRE(rowa_ok(d), "igemm: tile %d takes 3x3 stride-1 same-size convolutions with Cin %% 64 == 0 only", tile);
   if (tile >= 17 && tile <= 19) LBMK_REQUIRE(pp_ok(d), "igemm: tile %d (ping-pong schedule) takes 1x1 and 2x2 / 3x3 stride-1 same-size layers with Cin %% 64 == 0 only", tile);
   hipStream_t s = (hipStream_t)stream;
+  if (low_rank) {
+    LBMK_REQUIRE(low_rank_tile(tile) && (tile == 3) == !fast_path(d), "igemm: tile %d has no adapter product", tile);
+    switch (tile) {
+      case 3: launch_low_rank<64, 64, 2, 2, false, false>(d, s); break;
+      case 12: launch_low_rank<128, 64, 2, 2, true, true, 3>(d, s); break;
+      case 13: launch_low_rank<64, 64, 2, 2, true, true, 4>(d, s); break;
+      case 14: launch_low_rank<128, 128, 2, 2, true, true, 2>(d, s); break;
+      case 17: launch_low_rank<256, 256, 4, 2, true, true, 1, true>(d, s); break;
+      case 18: launch_low_rank<256, 160, 4, 2, true, true, 1, true>(d, s); break;
+    }
+    return lbmk_check_launch("igemm");
+  }
   switch (tile) {
     case 0: launch<128, 128, 2, 2, false, false, 4>(d, s); break;
     case 1: launch<128, 64, 2, 2, false, false, 4>(d, s); break;

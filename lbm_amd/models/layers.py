@@ -137,6 +137,13 @@ class HipLinear(nn.Linear, _Cached):
         return ops.linear(x, pw, residual=residual, rowvec=rowvec, rows_per_image=rows_per_image, act=act, out=out)
 
 
+    def forward_adapters(self, x, down, up, index, scaling=None):
+        """This layer for a batch of requests with low-rank adapters of their own (ops.linear_adapters); inference only."""
+        if torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad):
+            raise NotImplementedError("forward_adapters is inference-only: call it under torch.no_grad()")
+        return ops.linear_adapters(x, self.packed(), down, up, index, scaling)
+
+
 class HipGroupNorm(nn.GroupNorm, _Cached):
     def affine_f32(self):
         return self._cached("a", (self.weight, self.bias),

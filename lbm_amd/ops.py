@@ -1703,3 +1703,67 @@ def cached_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, l
     with _on(q):
         check(lib.lbmk_cached_attn(C.byref(d), _stream()), "lbmk_cached_attn")
     return o
+
+
+# --------------------------------------------------------------------------------------
+# token operators: a linear layer with the low-rank adapters of many requests
+# --------------------------------------------------------------------------------------
+def linear_adapters(x: torch.Tensor, pw: PackedWeight, down: torch.Tensor, up: torch.Tensor, index: torch.Tensor,
+                    scaling: Optional[torch.Tensor] = None, *, tile: int = -1) -> torch.Tensor:
+    """y = x W^T + b + scaling[a] (x down[a]^T) up[a]^T with a = index[request]: one shared layer, each request with its own
+    low-rank adapter, or without (an index outside [0, count)).
+
+    x: bf16 [requests, rows, K] or [requests, K] (one row each; any row stride); ``pw``: the shared layer
+    (``pack_linear_weight``); down: bf16 [count, rank, K], up: bf16 [count, N, rank] (rank 1 ... 256), scaling: f32 [count] or
+    None; index: int32 [requests] on the device.  The adapter's share is added in f32, before y's one rounding; a row's result does
+    not depend on the other requests' adapters.  Serving only: no gradients."""
+    _want(x.dim() in (2, 3), f"linear_adapters: x [requests, rows, K] or [requests, K] expected, got {tuple(x.shape)}")
+    x3 = x if x.dim() == 3 else x[:, None]
+    R, rows, K = x3.shape
+    _want(x.dtype == bf16 and pw.w.dtype == bf16 and down.dtype == bf16 and up.dtype == bf16,
+          f"linear_adapters: x {x.dtype}, weight {pw.w.dtype}, adapters {down.dtype} / {up.dtype} (all bf16)")
+    _want(not pw.geglu and pw.KH == 1 and pw.KW == 1, "linear_adapters: a plain linear layer")
+    _want(K == pw.K and K % 8 == 0 and pw.N % 8 == 0, f"linear_adapters: x has {K} channels, the layer is {pw.K} -> {pw.N} (multiples of 8)")
+    _want(down.dim() == 3 and up.dim() == 3 and down.shape[0] == up.shape[0] > 0 and down.shape[2] == K and up.shape[1] == pw.N and
+          down.shape[1] == up.shape[2] and 1 <= up.shape[2] <= 256 and down.is_contiguous() and up.is_contiguous() and
+          down.data_ptr() % 16 == 0 and up.data_ptr() % 16 == 0,
+          f"linear_adapters: down {tuple(down.shape)}, up {tuple(up.shape)} (contiguous [count, rank, {K}], [count, {pw.N}, rank], rank 1 ... 256)")
+    count, rank = down.shape[:2]
+    _want(index.dtype == torch.int32 and tuple(index.shape) == (R,) and index.is_contiguous(), f"index: contiguous int32 [{R}]")
+    _want(scaling is None or (scaling.dtype == torch.float32 and tuple(scaling.shape) == (count,) and scaling.is_contiguous()),
+          f"scaling: contiguous f32 [{count}]")
+    _same_device(x, pw.w, pw.bias, down, up, index, scaling)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, down, up, scaling)):
+        raise NotImplementedError("linear_adapters is inference-only: call it under torch.no_grad() or detach its operands")
+    # one row stride for all rows (a request's rows follow the previous one's)
+    ldx = x3.stride(1) if rows > 1 else x3.stride(0) if R > 1 else K
+    ok = x3.stride(2) == 1 and x.data_ptr() % 16 == 0 and ldx % 8 == 0 and ldx >= K and (rows <= 1 or R <= 1 or x3.stride(0) == rows * ldx)
+    _want(ok or x.numel() == 0, f"linear_adapters: strides {x.stride()}: channels adjacent, one stride of a multiple of 8 between all rows")
+    _need_gpu(x)
+    T, N = R * rows, pw.N
+    out = torch.empty(*x.shape[:-1], N, dtype=bf16, device=x.device)
+    if T == 0:
+        return out
+    tk = ceil_to(rank, 32)
+    t = torch.empty(T, tk, dtype=bf16, device=x.device)
+    with _on(x):
+        s = _stream()
+        check(lib.lbmk_adapter_down(x.data_ptr(), down.data_ptr(), index.data_ptr(), _ptr(scaling), t.data_ptr(), R, rows, K, ldx, rank, tk, count, s),
+              "lbmk_adapter_down")
+        if tile < 0 and T <= ADAPTER_FEW_ROWS:
+            check(lib.lbmk_adapter_linear_few(x.data_ptr(), pw.w.data_ptr(), _ptr(pw.bias), t.data_ptr(), up.data_ptr(), index.data_ptr(),
+                                              out.data_ptr(), R, rows, N, K, ldx, pw.Kp, N, rank, tk, count, s), "lbmk_adapter_linear_few")
+            return out
+        d = IgemmDesc()
+        d.a, d.w, d.out, d.bias = x.data_ptr(), pw.w.data_ptr(), out.data_ptr(), _ptr(pw.bias)
+        d.M, d.N, d.K, d.Kp, d.Cin, d.a_cs = T, N, K, pw.Kp, K, ldx
+        d.IH = d.IW = d.OH = d.OW = d.KH = d.KW = d.stride = 1
+        d.ldo, d.act, d.alpha, d.batch, d.tile = N, ACT_NONE, 1.0, 1, tile
+        d.lr_t, d.lr_up, d.lr_index = t.data_ptr(), up.data_ptr(), index.data_ptr()
+        d.lr_rank, d.lr_k, d.lr_rows, d.lr_count = rank, tk, rows, count
+        _igemm(d, 2.0 * T * (pw.alg_nk or N * K))
+    return out
+
+
+# rows up to which the shared weight is streamed through registers instead of a tiled product
+ADAPTER_FEW_ROWS = lib.lbmk_adapter_few_rows()
