@@ -267,6 +267,8 @@ int lbmk_flash_attn_bwd(const void* q, const void* qt, const void* k, const void
  *   ranges     : int32 [B][Nq][2] (8-byte aligned; lbmk_key_ranges or the caller's own, clipped to [0, Nk)); NULL: every key
  *   lse        : f32 [B][H][Nq] log2-sum-exp (of the base-2 scores; +inf for an empty row): written forward (NULL: not
  *                wanted), read backward
+ *   rest       : bf16 [B][Nq][H*D], what rounding took from o: written forward, read backward, where it halves the error of
+ *                rowsum(dout * o) and with it a third of dq's and dk's (NULL: not wanted)
  *   scratch    : backward only, lbmk_ranged_attn_bwd_scratch_floats(...) floats, 16-byte aligned
  * What an operand holds at places that a query does not see has no influence on its row, inf and NaN included; a value that is not
  * finite at a place it does see makes the sums it enters not finite (NaN).
@@ -274,7 +276,7 @@ int lbmk_flash_attn_bwd(const void* q, const void* qt, const void* k, const void
  * ---------------------------------------------------------------------- */
 typedef struct lbmk_ranged_attn_desc {
   const void *q, *k, *v, *dout;
-  void *o, *dq, *dk, *dv;
+  void *o, *rest, *dq, *dk, *dv;
   float* lse;
   const int32_t* ranges;
   const float* slopes;

@@ -64,7 +64,7 @@ class NormRopeDesc(C.Structure):
 
 
 class RangedAttnDesc(C.Structure):
-    _fields_ = [(n, vp) for n in ("q", "k", "v", "dout", "o", "dq", "dk", "dv", "lse", "ranges", "slopes", "scratch")] + \
+    _fields_ = [(n, vp) for n in ("q", "k", "v", "dout", "o", "rest", "dq", "dk", "dv", "lse", "ranges", "slopes", "scratch")] + \
                [(n, i32) for n in ("B", "H", "Hk", "Nq", "Nk", "D", "ldq", "ldk", "ldv", "ldo", "ldg")] + \
                [(n, i64) for n in ("sq", "sk", "sv", "so", "sg")] + [("scale", f32), ("cap", f32)]
 

@@ -391,17 +391,18 @@ class RangedAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, heads, kv_heads, head_dim, ranges, scale, cap, slopes):
-        o, lse = ops.ranged_attn(q, k, v, heads, kv_heads, head_dim, ranges, scale=scale, cap=cap, slopes=slopes, return_lse=True)
-        ctx.save_for_backward(q, k, v, o, lse, ranges, slopes)
+        o, lse, rest = ops.ranged_attn(q, k, v, heads, kv_heads, head_dim, ranges, scale=scale, cap=cap, slopes=slopes, return_lse=True,
+                                       return_rest=True)
+        ctx.save_for_backward(q, k, v, o, lse, rest, ranges, slopes)
         ctx.cfg = (heads, kv_heads, head_dim, scale, cap)
         return o
 
     @staticmethod
     def backward(ctx, do):
-        q, k, v, o, lse, ranges, slopes = ctx.saved_tensors
+        q, k, v, o, lse, rest, ranges, slopes = ctx.saved_tensors
         heads, kv_heads, head_dim, scale, cap = ctx.cfg
         return (*ops.ranged_attn_bwd(q, k, v, o, ops.token_rows_ready(do), lse, heads, kv_heads, head_dim, ranges, scale=scale, cap=cap,
-                                     slopes=slopes), None, None, None, None, None, None, None)
+                                     slopes=slopes, rest=rest), None, None, None, None, None, None, None)
 
 
 class SelfAttnQKVFn(torch.autograd.Function):

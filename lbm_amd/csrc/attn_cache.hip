@@ -91,6 +91,10 @@ __global__ __launch_bounds__(256) void cached_attn_kernel(const Cached a) {
     T::template stage<NI, CT>(V, kv0, c1, a.ldv, a.D, voffs, 0, 1, mine + buf * 2 * TILE + TILE);
   };
 
+  // a wave walks alone, so it alone repeats its walk where masked places held values that are not finite
+  auto walk = [&](auto form) __attribute__((always_inline)) {
+  constexpr bool GUARD = decltype(form)::guard;
+  bool bad = false;
   int kv0 = c0 + wave * CT, cur = 0;
   if (kv0 < c1) stage(kv0, 0);
   for (; kv0 < c1; kv0 += 4 * CT) {
@@ -157,14 +161,7 @@ __global__ __launch_bounds__(256) void cached_attn_kernel(const Cached a) {
     bf16x8 pf[2];
     pack_column(p, pf);
 
-    uint32_t bad = 0;
-    if (masked) {
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int m = 0; m < 2; ++m) bad |= not_finite(T::col_frag(sV + 16 * m * T::ROW, clo[dt], chi[dt]));
-    }
-    if (masked && __builtin_amdgcn_ballot_w64(bad != 0) != 0) {
+    if (GUARD && masked) {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         f32x16 hit = zero;
@@ -172,13 +169,25 @@ __global__ __launch_bounds__(256) void cached_attn_kernel(const Cached a) {
         for (int m = 0; m < 2; ++m) mfma_guarded(T::col_frag(sV + 16 * m * T::ROW, clo[dt], chi[dt]), pf[m], o[dt], hit);
         poison(o[dt], hit);
       }
-    } else {
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::col_frag(sV + 16 * m * T::ROW, clo[dt], chi[dt]), pf[m], o[dt], 0, 0, 0);
+      continue;
     }
+    if (!GUARD && masked) bad |= tile_not_finite<TILE>(sV, lane);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::col_frag(sV + 16 * m * T::ROW, clo[dt], chi[dt]), pf[m], o[dt], 0, 0, 0);
+  }
+  return bad;
+  };
+  if (walk(Plain())) {
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
+    m_run = M_NONE;
+    l_run = 0.f;
+    walk(Guarded());
   }
 
   // ---- join the four waves ----

@@ -20,7 +20,7 @@ constexpr int TB = 64;    // tokens per tile of the walked operand
 
 struct Ranged {
   const bf16_t *q, *k, *v, *dout;
-  bf16_t *o, *dq, *dk, *dv;
+  bf16_t *o, *rest, *dq, *dk, *dv;     // rest: [B][Nq][H * D], what rounding took from o
   float *lse, *delta, *part;          // part: f32 [2][splits][B][Nk][Hk * D] when splits > 1
   const int32_t* ranges;              // [B][Nq][2] or null: every key
   const float* slopes;                // [H]
@@ -117,6 +117,10 @@ __global__ __launch_bounds__(256, DH <= 64 ? 3 : 2) void ranged_fwd_kernel(const
     T::template stage<NI, TB>(K, kv0, w.end, a.ldk, a.D, koffs, wave, 4, buf);
     T::template stage<NI, TB>(V, kv0, w.end, a.ldv, a.D, voffs, wave, 4, buf + TB * T::ROW);
   };
+  // the walk over the keys; true: a masked tile holds values that are not finite, and the sums are worth nothing
+  auto walk = [&](auto form) __attribute__((always_inline)) {
+  constexpr bool GUARD = decltype(form)::guard;
+  bool bad = false;
   if (w.begin < w.end) stage(w.begin, smem);
   int cur = 0;
   for (int kv0 = w.begin; kv0 < w.end; kv0 += TB) {
@@ -200,29 +204,34 @@ __global__ __launch_bounds__(256, DH <= 64 ? 3 : 2) void ranged_fwd_kernel(const
     }
     l_run += ps0 + ps1;
 
-    if (masked) {
-      uint32_t bad = 0;
+    if (GUARD && masked) {
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
+      for (int dt = 0; dt < DT; ++dt) {
+        f32x16 hit = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int m = 0; m < 4; ++m) bad |= not_finite(T::col_frag(sV + 16 * m * T::ROW, clo[dt], chi[dt]));
-      if (__builtin_amdgcn_ballot_w64(bad != 0) != 0) {
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          f32x16 hit = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int m = 0; m < 4; ++m) mfma_guarded(T::col_frag(sV + 16 * m * T::ROW, clo[dt], chi[dt]), pf[m >> 1][m & 1], o[dt], hit);
-          poison(o[dt], hit);
-        }
-        continue;
+        for (int m = 0; m < 4; ++m) mfma_guarded(T::col_frag(sV + 16 * m * T::ROW, clo[dt], chi[dt]), pf[m >> 1][m & 1], o[dt], hit);
+        poison(o[dt], hit);
       }
+      continue;
     }
+    if (!GUARD && masked) bad |= tile_not_finite<TB * T::ROW>(sV, lane);
     // ---- O^T += V^T P^T ----
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int m = 0; m < 4; ++m)
         o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::col_frag(sV + 16 * m * T::ROW, clo[dt], chi[dt]), pf[m >> 1][m & 1], o[dt], 0, 0, 0);
+  }
+  return bad;
+  };
+  if (__syncthreads_or(walk(Plain()))) {
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
+    m_run = M_NONE;
+    l_run = 0.f;
+    walk(Guarded());
   }
 
   const float l = l_run + __shfl_xor(l_run, 32, 64);
@@ -237,10 +246,15 @@ __global__ __launch_bounds__(256, DH <= 64 ? 3 : 2) void ranged_fwd_kernel(const
       for (int g = 0; g < 4; ++g) {
         const int c = 32 * dt + 8 * g + 4 * h;
         if (c < a.D) {
-          u16x4 ov;
+          u16x4 ov, rv;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) ov.v[e] = f2bf(none ? 0.f : o[dt][4 * g + e] * inv);
+          for (int e = 0; e < 4; ++e) {
+            const float v = none ? 0.f : o[dt][4 * g + e] * inv;
+            ov.v[e] = f2bf(v);
+            rv.v[e] = f2bf(v - bf2f(ov.v[e]));
+          }
           *(u16x4*)(op + c) = ov;
+          if (a.rest) *(u16x4*)(a.rest + (((int64_t)b * a.Nq + q) * a.H + head) * a.D + c) = rv;
         }
       }
   }
@@ -313,6 +327,13 @@ __global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dq_kernel(co
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
       for (int e = 0; e < 8; ++e) delta = fmaf((float)gf[ks][e], (float)of[ks][e], delta);
+    if (a.rest) {      // dS = P (dP - delta) cancels: the half step of o would be the largest error of dQ and dK
+      load_frags<KS>(a.rest + (((int64_t)b * a.Nq + qr) * a.H + head) * a.D, h, a.D, of);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) delta = fmaf((float)gf[ks][e], (float)of[ks][e], delta);
+    }
     delta += __shfl_xor(delta, 32, 64);
     if (q < a.Nq && h == 0) a.delta[stat] = delta;
   }
@@ -339,6 +360,9 @@ __global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dq_kernel(co
     T::template stage<NI, TB>(K, kv0, w.end, a.ldk, a.D, koffs, wave, 4, buf);
     T::template stage<NI, TB>(V, kv0, w.end, a.ldv, a.D, voffs, wave, 4, buf + TB * T::ROW);
   };
+  auto walk = [&](auto form) __attribute__((always_inline)) {
+  constexpr bool GUARD = decltype(form)::guard;
+  bool bad = false;
   if (w.begin < w.end) stage(w.begin, smem);
   int cur = 0;
   for (int kv0 = w.begin; kv0 < w.end; kv0 += TB) {
@@ -350,6 +374,7 @@ __global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dq_kernel(co
     if (kv0 + TB < w.end) stage(kv0 + TB, smem + cur * STAGE);
     if (w.lo_min >= kv0 + TB || w.hi_max <= kv0) continue;
     const bool masked = w.lo_max > kv0 || w.hi_min < kv0 + TB;
+    if (!GUARD && masked) bad |= tile_not_finite<TB * T::ROW>(sK, lane);
 
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
@@ -392,22 +417,15 @@ __global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dq_kernel(co
       bf16x8 df[2];
       pack_column(ds, df);          // bf16 operand of dS K: half a step per element, of random sign over the keys
       const char* sk = sK + 32 * kt * T::ROW;
-      if (masked) {
-        uint32_t bad = 0;
+      if (GUARD && masked) {
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+        for (int dt = 0; dt < DT; ++dt) {
+          f32x16 hit = zero;
 #pragma unroll
-          for (int ss = 0; ss < 2; ++ss) bad |= not_finite(T::col_frag(sk + 16 * ss * T::ROW, clo[dt], chi[dt]));
-        if (__builtin_amdgcn_ballot_w64(bad != 0) != 0) {
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            f32x16 hit = zero;
-#pragma unroll
-            for (int ss = 0; ss < 2; ++ss) mfma_guarded(T::col_frag(sk + 16 * ss * T::ROW, clo[dt], chi[dt]), df[ss], acc[dt], hit);
-            poison(acc[dt], hit);
-          }
-          continue;
+          for (int ss = 0; ss < 2; ++ss) mfma_guarded(T::col_frag(sk + 16 * ss * T::ROW, clo[dt], chi[dt]), df[ss], acc[dt], hit);
+          poison(acc[dt], hit);
         }
+        continue;
       }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
@@ -415,6 +433,15 @@ __global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dq_kernel(co
         for (int ss = 0; ss < 2; ++ss)
           acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::col_frag(sk + 16 * ss * T::ROW, clo[dt], chi[dt]), df[ss], acc[dt], 0, 0, 0);
     }
+  }
+  return bad;
+  };
+  if (__syncthreads_or(walk(Plain()))) {
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
+    walk(Guarded());
   }
   if (q < a.Nq) put_rows<DT>(a.dq + ((int64_t)b * a.Nq + q) * a.H * a.D + (int64_t)head * a.D, acc, a.scale, h, a.D);
 }
@@ -490,6 +517,9 @@ __global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dkv_kernel(c
     }
   };
 
+  auto walk = [&](auto form) __attribute__((always_inline)) {
+  constexpr bool GUARD = decltype(form)::guard;
+  bool bad = false;
   int cur = 0, i = next(first);
   if (i < last) stage(i, smem);
   while (i < last) {
@@ -571,30 +601,21 @@ __global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dkv_kernel(c
       pack_column(ds, df);
       const char* sq = sQ + 32 * u * T::ROW;
       const char* sg = sG + 32 * u * T::ROW;
-      if (masked) {
-        uint32_t bad = 0;
+      if (GUARD && masked) {
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+        for (int dt = 0; dt < DT; ++dt) {
+          f32x16 hq = zero, hg = zero;
 #pragma unroll
           for (int ss = 0; ss < 2; ++ss) {
-            bad |= not_finite(T::col_frag(sq + 16 * ss * T::ROW, clo[dt], chi[dt]));
-            bad |= not_finite(T::col_frag(sg + 16 * ss * T::ROW, clo[dt], chi[dt]));
+            mfma_guarded(T::col_frag(sg + 16 * ss * T::ROW, clo[dt], chi[dt]), pf[ss], dv[dt], hg);
+            mfma_guarded(T::col_frag(sq + 16 * ss * T::ROW, clo[dt], chi[dt]), df[ss], dk[dt], hq);
           }
-        if (__builtin_amdgcn_ballot_w64(bad != 0) != 0) {
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            f32x16 hq = zero, hg = zero;
-#pragma unroll
-            for (int ss = 0; ss < 2; ++ss) {
-              mfma_guarded(T::col_frag(sg + 16 * ss * T::ROW, clo[dt], chi[dt]), pf[ss], dv[dt], hg);
-              mfma_guarded(T::col_frag(sq + 16 * ss * T::ROW, clo[dt], chi[dt]), df[ss], dk[dt], hq);
-            }
-            poison(dv[dt], hg);
-            poison(dk[dt], hq);
-          }
-          continue;
+          poison(dv[dt], hg);
+          poison(dk[dt], hq);
         }
+        continue;
       }
+      if (!GUARD && masked) bad |= tile_not_finite<32 * T::ROW>(sq, lane) | tile_not_finite<32 * T::ROW>(sg, lane);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -603,6 +624,15 @@ __global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dkv_kernel(c
           dk[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::col_frag(sq + 16 * ss * T::ROW, clo[dt], chi[dt]), df[ss], dk[dt], 0, 0, 0);
         }
     }
+  }
+  return bad;
+  };
+  if (__syncthreads_or(walk(Plain()))) {
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dk[i][e] = dv[i][e] = 0.f;
+    walk(Guarded());
   }
   if (key < a.Nk) {
     const int64_t at = ((int64_t)b * a.Nk + key) * a.Hk * a.D + (int64_t)khead * a.D;
@@ -682,6 +712,7 @@ int ranged_check(const lbmk_ranged_attn_desc* p, bool bwd) {
   }
   LBMK_REQUIRE(!p->ranges || lbmk_aligned(p->ranges, 8), "ranged_attn: misaligned ranges");
   LBMK_REQUIRE(!p->slopes || lbmk_aligned(p->slopes, 4), "ranged_attn: misaligned slopes");
+  LBMK_REQUIRE(!p->rest || lbmk_aligned(p->rest, 16), "ranged_attn: misaligned rest");
   if (bwd) LBMK_REQUIRE(p->lse && p->scratch && lbmk_aligned(p->scratch, 16), "ranged_attn_bwd: no log-sum-exp or scratch");
   return LBMK_OK;
 }
@@ -691,6 +722,7 @@ Ranged ranged_args(const lbmk_ranged_attn_desc* p) {
   a.q = (const bf16_t*)p->q; a.k = (const bf16_t*)p->k; a.v = (const bf16_t*)p->v; a.dout = (const bf16_t*)p->dout;
   a.o = (bf16_t*)p->o; a.dq = (bf16_t*)p->dq; a.dk = (bf16_t*)p->dk; a.dv = (bf16_t*)p->dv;
   a.lse = p->lse;
+  a.rest = (bf16_t*)p->rest;
   a.ranges = p->ranges;
   a.slopes = p->slopes;
   a.sq = p->sq; a.sk = p->sk; a.sv = p->sv; a.so = p->so; a.sg = p->sg;

@@ -94,22 +94,31 @@ __device__ __forceinline__ void pack_column(const float (&p)[16], bf16x8 (&f)[2]
   }
 }
 
-// Masked places hold 0 in one operand, and 0 * inf or 0 * NaN in the other would poison a sum that must not see them.  A tile
-// with masked places is therefore scanned; in the rare case that it holds a value that is not finite, its products take
-// the finite values alone, and a second product of indicators (not finite x not masked) says which sums become NaN.
-__device__ __forceinline__ uint32_t not_finite(bf16x8 v) {      // != 0: some element is inf or NaN
-  const u32x4 w = __builtin_bit_cast(u32x4, v);
+// Masked places hold 0 in one operand, and 0 * inf or 0 * NaN in the other would poison a sum that must not see them.  The walks
+// scan each tile that has masked places (a few instructions per 16 bytes, and such tiles are few); where one holds a value that
+// is not finite the whole walk is done again in a second form, whose masked tiles multiply the finite values alone and learn
+// from a product of indicators (not finite x not masked) which sums become NaN.  The first form carries none of that: with both
+// in one loop the registers spilled and the tile loads were waited for at once (2.5 x slower).  Finite sums are the same bits
+// whatever the masked places hold.
+struct Plain { static constexpr bool guard = false; };
+struct Guarded { static constexpr bool guard = true; };
+
+template <int BYTES>
+__device__ __forceinline__ bool tile_not_finite(const char* tile, int lane) {
   uint32_t a = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) a |= (w[i] & 0x7f807f80u) + 0x00800080u;
-  return a & 0x80008000u;
+  for (int i = 0; i < BYTES / 1024; ++i) {
+    const u32x4 w = *(const u32x4*)(tile + i * 1024 + lane * 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a |= (w[e] & 0x7f807f80u) + 0x00800080u;     // carries out of an exponent of all ones
+  }
+  return __builtin_amdgcn_ballot_w64((a & 0x80008000u) != 0) != 0;
 }
 __device__ __forceinline__ void mfma_guarded(bf16x8 a, bf16x8 b, f32x16& acc, f32x16& hit) {
   bf16x8 fin, ind, pat;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const uint16_t bits = __builtin_bit_cast(uint16_t, (__bf16)a[e]);
-    const bool ok = (bits & 0x7f80) != 0x7f80;
+    const bool ok = (__builtin_bit_cast(uint16_t, (__bf16)a[e]) & 0x7f80) != 0x7f80;
     fin[e] = ok ? (__bf16)a[e] : (__bf16)0.f;
     ind[e] = ok ? (__bf16)0.f : (__bf16)1.f;
     pat[e] = (__builtin_bit_cast(uint16_t, (__bf16)b[e]) & 0x7fff) ? (__bf16)1.f : (__bf16)0.f;

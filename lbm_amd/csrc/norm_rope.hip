@@ -10,14 +10,14 @@
 // Bound by memory: 4 bytes per element forward, 6 backward (bf16) and some 10 / 25 operations.  A head is held by
 // L = 2^k lanes, each with the TWO chunks of VEC channels that the rotation pairs up, so the rotation needs no exchange
 // between lanes and the norm a log2(L)-step butterfly.  The lanes of a group walk heads of ONE token, so its cosines and
-// sines are read once and stay in registers; four heads are loaded before the first is used, to have enough bytes in
-// flight.  All statistics and gradient sums are f32; each output is rounded once.
+// sines are read once and stay in registers; four heads are loaded before the first is used, and kept as they lie in
+// memory until then, to have enough bytes in flight.  All statistics and gradient sums are f32; each output is rounded once.
 #include "common.h"
 
 namespace {
 
 constexpr int NR_THREADS = 256;
-constexpr int NR_BATCH = 4;        // heads in flight per lane group
+constexpr int NR_BATCH = 4, NR_BATCH_BWD = 2;        // heads in flight per lane group
 
 struct NormRope {
   const void *x[2], *w[2], *dy[2];
@@ -28,29 +28,40 @@ struct NormRope {
   int64_t sx[2], sdy[2], sy[2];    // batch strides (elements)
   int ldx[2], lddy[2], ldy[2];     // token strides
   int H[2];
-  int D, rot, axes, F, P, tokens, N, w_f32, w_wide, gpt;
+  int D, rot, axes, F, P, tokens, N, w_f32, w_wide, wide, gpt;
   float eps;
 };
 
+// one chunk as it lies in memory: kept packed until it is used, so that many fit in flight
 template <typename T, int VEC>
-__device__ __forceinline__ void nr_load(const T* p, float (&v)[VEC]) {
-  if constexpr (sizeof(T) == 4) {
+struct Chunk {
+  static constexpr int WORDS = VEC * sizeof(T) / 4;
+  uint32_t w[WORDS];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (WORDS % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i < VEC; i += 4) {
-      const f32x4 a = *(const f32x4*)(p + i);
+      for (int i = 0; i < WORDS; i += 4) {
+        const u32x4 a = *(const u32x4*)((const uint32_t*)p + i);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[i + e] = a[e];
+        for (int e = 0; e < 4; ++e) w[i + e] = a[e];
+      }
+    } else {
+      const uint2 a = *(const uint2*)p;
+      w[0] = a.x;
+      w[1] = a.y;
     }
-  } else if constexpr (VEC == 8) {
-    const u16x8 a = *(const u16x8*)p;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = bf2f(a.v[e]);
-  } else {
-    const u16x4 a = *(const u16x4*)p;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = bf2f(a.v[e]);
   }
-}
+  __device__ __forceinline__ void get(float (&v)[VEC]) {
+    // opaque to the compiler: it would unpack at the load, and hold every head in flight at twice the registers
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) asm volatile("" : "+v"(w[i]));
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      if constexpr (sizeof(T) == 4) v[e] = __builtin_bit_cast(float, w[e]);
+      else v[e] = __builtin_bit_cast(float, (e & 1) ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    }
+  }
+};
 
 template <typename T, int VEC>
 __device__ __forceinline__ void nr_store(T* p, const float (&v)[VEC]) {
@@ -89,26 +100,44 @@ __device__ __forceinline__ void nr_chunks(int u, int D, int rot, int& a, int& b,
   turns_b = INTER && b >= 0 && b < rot;
 }
 
-// cosine / sine of the lane's pairs: VEC of them for two paired chunks, VEC / 2 per chunk when interleaved
+// cosine / sine of `n` = N pairs from pair j0 on.  A position outside the table: NaN, never a silent wrong angle.
+// Pairs of one axis lie next to each other in the table (wide: 16-byte loads); a chunk may also cross axes.
+template <int N>
+__device__ __forceinline__ void nr_pairs(const NormRope& d, int64_t token, int j0, float* c, float* s) {
+  const int32_t* pos = d.pos + token * d.axes;
+  if (d.wide) {
+    const int ax = j0 / d.F, p = pos[ax], pc = min(max(p, 0), d.P - 1);
+    const f32x4* row = (const f32x4*)(d.table + (int64_t)pc * d.F + (j0 - ax * d.F));
+    const float bad = pc == p ? 0.f : __builtin_nanf("");
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      const f32x4 v = row[e / 2];
+      c[e] = v[0] + bad;
+      s[e] = v[1] + bad;
+      c[e + 1] = v[2] + bad;
+      s[e + 1] = v[3] + bad;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int j = j0 + e, ax = j / d.F, p = pos[ax], pc = min(max(p, 0), d.P - 1);
+      const float2 v = d.table[(int64_t)pc * d.F + (j - ax * d.F)];
+      const float bad = pc == p ? 0.f : __builtin_nanf("");
+      c[e] = v.x + bad;
+      s[e] = v.y + bad;
+    }
+  }
+}
+
+// of the lane's chunks: VEC pairs for two chunks that the rotation combines, VEC / 2 per chunk when interleaved
 template <int VEC, bool INTER>
 __device__ __forceinline__ void nr_angles(const NormRope& d, int64_t token, int a, int b, bool ta, bool tb, float (&c)[VEC],
                                           float (&s)[VEC]) {
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    c[e] = 1.f;
-    s[e] = 0.f;
-    const bool turns = INTER ? (e < VEC / 2 ? ta : tb) : ta;
-    if (!turns) continue;
-    const int j = INTER ? (e < VEC / 2 ? a / 2 + e : b / 2 + e - VEC / 2) : a + e;
-    const int ax = j / d.F;
-    const int p = d.pos[token * d.axes + ax];
-    if ((unsigned)p < (unsigned)d.P) {
-      const float2 cs = d.table[(int64_t)p * d.F + (j - ax * d.F)];
-      c[e] = cs.x;
-      s[e] = cs.y;
-    } else {
-      c[e] = s[e] = __builtin_nanf("");     // a position outside the table: never a silent wrong angle
-    }
+  if constexpr (INTER) {
+    if (ta) nr_pairs<VEC / 2>(d, token, a / 2, c, s);
+    if (tb) nr_pairs<VEC / 2>(d, token, b / 2, c + VEC / 2, s + VEC / 2);
+  } else {
+    if (ta) nr_pairs<VEC>(d, token, a, c, s);
   }
 }
 
@@ -147,165 +176,172 @@ __device__ __forceinline__ float nr_sum(float v) {
   return v;
 }
 
+// blockIdx.y: 0 the queries, 1 the keys
 template <typename T, int VEC, bool INTER, int L, bool BWD>
 __global__ __launch_bounds__(NR_THREADS) void norm_rope_kernel(NormRope d) {
-  constexpr int GROUPS = NR_THREADS / L;
-  const int t = threadIdx.x, u = t % L, group = t / L;
+  constexpr int GROUPS = NR_THREADS / L, NB = BWD ? NR_BATCH_BWD : NR_BATCH;
+  const int t = threadIdx.x, u = t % L, group = t / L, z = blockIdx.y;
   const int tpb = GROUPS / d.gpt;                       // tokens per block and step
   const int sub = group % d.gpt;                        // this group's first head
+  const int H = d.H[z];
   int ca, cb;
   bool ta, tb;
   nr_chunks<VEC, INTER>(u, d.D, d.rot, ca, cb, ta, tb);
   const int pa = ca < 0 ? 0 : ca, pb = cb < 0 ? 0 : cb; // idle chunks read channel 0 and count as zeros
 
-  float w[2][2][VEC], dw[BWD ? 2 : 1][2][VEC];
+  const void* weight = d.w[z];
+  float wa[VEC], wb[VEC], dwa[VEC], dwb[VEC];
 #pragma unroll
-  for (int z = 0; z < 2; ++z)
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      w[z][0][e] = w[z][1][e] = 1.f;
-      if (BWD) dw[z][0][e] = dw[z][1][e] = 0.f;
-    }
-#pragma unroll
-  for (int z = 0; z < 2; ++z) {
-    if (!d.w[z]) continue;
+  for (int e = 0; e < VEC; ++e) {
+    wa[e] = wb[e] = 1.f;
+    dwa[e] = dwb[e] = 0.f;
+  }
+  if (weight) {
     if (d.w_wide && d.w_f32) {
-      nr_load<float, VEC>((const float*)d.w[z] + pa, w[z][0]);
-      nr_load<float, VEC>((const float*)d.w[z] + pb, w[z][1]);
+      Chunk<float, VEC> c;
+      c.load((const float*)weight + pa);
+      c.get(wa);
+      c.load((const float*)weight + pb);
+      c.get(wb);
     } else if (d.w_wide) {
-      nr_load<bf16_t, VEC>((const bf16_t*)d.w[z] + pa, w[z][0]);
-      nr_load<bf16_t, VEC>((const bf16_t*)d.w[z] + pb, w[z][1]);
+      Chunk<bf16_t, VEC> c;
+      c.load((const bf16_t*)weight + pa);
+      c.get(wa);
+      c.load((const bf16_t*)weight + pb);
+      c.get(wb);
     } else {                       // a parameter's slot in a flat buffer need not start on 16 bytes
+#pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        w[z][0][e] = d.w_f32 ? ((const float*)d.w[z])[pa + e] : bf2f(((const bf16_t*)d.w[z])[pa + e]);
-        w[z][1][e] = d.w_f32 ? ((const float*)d.w[z])[pb + e] : bf2f(((const bf16_t*)d.w[z])[pb + e]);
+        wa[e] = d.w_f32 ? ((const float*)weight)[pa + e] : bf2f(((const bf16_t*)weight)[pa + e]);
+        wb[e] = d.w_f32 ? ((const float*)weight)[pb + e] : bf2f(((const bf16_t*)weight)[pb + e]);
       }
     }
   }
   const float inv_d = 1.f / (float)d.D;
 
-  for (int64_t t0 = (int64_t)blockIdx.x * tpb; t0 < d.tokens; t0 += (int64_t)gridDim.x * tpb) {
+  for (int64_t t0 = (int64_t)blockIdx.x * tpb; H > 0 && t0 < d.tokens; t0 += (int64_t)gridDim.x * tpb) {
     const int64_t token = t0 + group / d.gpt;
     const bool live = token < d.tokens;                 // groups past the end keep step with the butterflies, reading token 0
     const int64_t tk = live ? token : 0;
     const int64_t bb = tk / d.N, nn = tk - bb * d.N;
-    float c[VEC], s[VEC];
-    nr_angles<VEC, INTER>(d, tk, ca, cb, ta, tb, c, s);
+    const T* xr = (const T*)d.x[z] + bb * d.sx[z] + nn * d.ldx[z];
+    const T* gr = BWD ? (const T*)d.dy[z] + bb * d.sdy[z] + nn * d.lddy[z] : nullptr;
+    T* yr = (T*)d.y[z] + bb * d.sy[z] + nn * d.ldy[z];
+    Chunk<T, VEC> xa[NB], xb[NB], ga[BWD ? NB : 1], gb[BWD ? NB : 1];
+    auto load = [&](int h0) __attribute__((always_inline)) {
 #pragma unroll
-    for (int z = 0; z < 2; ++z) {
-      const T* xr = (const T*)d.x[z] + bb * d.sx[z] + nn * d.ldx[z];
-      const T* gr = BWD ? (const T*)d.dy[z] + bb * d.sdy[z] + nn * d.lddy[z] : nullptr;
-      T* yr = (T*)d.y[z] + bb * d.sy[z] + nn * d.ldy[z];
-      constexpr int NB = BWD ? NR_BATCH / 2 : NR_BATCH;
-      for (int h0 = sub; h0 < d.H[z]; h0 += NB * d.gpt) {
-        float xa[NB][VEC], xb[NB][VEC], ga[BWD ? NB : 1][VEC], gb[BWD ? NB : 1][VEC];
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          const int h = h0 + i * d.gpt;
-          const int hc = h < d.H[z] ? h : sub;          // a head of this group's own: in bounds
-          nr_load<T, VEC>(xr + hc * d.D + pa, xa[i]);
-          nr_load<T, VEC>(xr + hc * d.D + pb, xb[i]);
-          if constexpr (BWD) {
-            nr_load<T, VEC>(gr + hc * d.D + pa, ga[i]);
-            nr_load<T, VEC>(gr + hc * d.D + pb, gb[i]);
-          }
+      for (int i = 0; i < NB; ++i) {
+        const int h = h0 + i * d.gpt;
+        const int hc = h < H ? h : min(sub, H - 1);     // a row in bounds, not used
+        xa[i].load(xr + hc * d.D + pa);
+        xb[i].load(xr + hc * d.D + pb);
+        if constexpr (BWD) {
+          ga[i].load(gr + hc * d.D + pa);
+          gb[i].load(gr + hc * d.D + pb);
         }
+      }
+    };
+    float c[VEC], s[VEC];
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          const int h = h0 + i * d.gpt;
-          const bool put = live && h < d.H[z];
-          float qa = 0.f, qb = 0.f;
+    for (int e = 0; e < VEC; ++e) c[e] = s[e] = 0.f;
+    for (int h0 = sub; h0 < H; h0 += NB * d.gpt) {
+      load(h0);
+      if (h0 == sub) nr_angles<VEC, INTER>(d, tk, ca, cb, ta, tb, c, s);      // under the first loads
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int h = h0 + i * d.gpt;
+        const bool put = live && h < H;
+        float va[VEC], vb[VEC], qa = 0.f, qb = 0.f;
+        xa[i].get(va);
+        xb[i].get(vb);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          qa = fmaf(va[e], va[e], qa);
+          qb = fmaf(vb[e], vb[e], qb);
+        }
+        // (a select, not a product: what an idle lane reads twice may be infinite)
+        const float ms = nr_sum<L>((ca < 0 ? 0.f : qa) + (cb < 0 ? 0.f : qb)) * inv_d;
+        const float rstd = __builtin_amdgcn_rsqf(ms + d.eps);
+        if constexpr (!BWD) {
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
-            qa = fmaf(xa[i][e], xa[i][e], qa);
-            qb = fmaf(xb[i][e], xb[i][e], qb);
+            va[e] = va[e] * rstd * wa[e];
+            vb[e] = vb[e] * rstd * wb[e];
           }
-          // (a select, not a product: what an idle lane reads twice may be infinite)
-          const float ms = nr_sum<L>((ca < 0 ? 0.f : qa) + (cb < 0 ? 0.f : qb)) * inv_d;
-          const float rstd = __builtin_amdgcn_rsqf(ms + d.eps);
-          if constexpr (!BWD) {
+          nr_rotate<VEC, INTER>(va, vb, c, s, ta, tb, 1.f);
+        } else {
+          float ua[VEC], ub[VEC], da = 0.f, db = 0.f;
+          ga[i].get(ua);
+          gb[i].get(ub);
+          nr_rotate<VEC, INTER>(ua, ub, c, s, ta, tb, -1.f);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              xa[i][e] = xa[i][e] * rstd * w[z][0][e];
-              xb[i][e] = xb[i][e] * rstd * w[z][1][e];
+          for (int e = 0; e < VEC; ++e) {
+            va[e] *= rstd;
+            vb[e] *= rstd;
+            if (put) {
+              dwa[e] = fmaf(ua[e], va[e], dwa[e]);
+              dwb[e] = fmaf(ub[e], vb[e], dwb[e]);
             }
-            nr_rotate<VEC, INTER>(xa[i], xb[i], c, s, ta, tb, 1.f);
-            if (put && ca >= 0) nr_store<T, VEC>(yr + h * d.D + ca, xa[i]);
-            if (put && cb >= 0) nr_store<T, VEC>(yr + h * d.D + cb, xb[i]);
-          } else {
-            nr_rotate<VEC, INTER>(ga[i], gb[i], c, s, ta, tb, -1.f);
-            float da = 0.f, db = 0.f;
+            ua[e] *= wa[e];
+            ub[e] *= wb[e];
+            da = fmaf(ua[e], va[e], da);
+            db = fmaf(ub[e], vb[e], db);
+          }
+          const float m = nr_sum<L>((ca < 0 ? 0.f : da) + (cb < 0 ? 0.f : db)) * inv_d;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              xa[i][e] *= rstd;
-              xb[i][e] *= rstd;
-              if (put) {
-                dw[z][0][e] = fmaf(ga[i][e], xa[i][e], dw[z][0][e]);
-                dw[z][1][e] = fmaf(gb[i][e], xb[i][e], dw[z][1][e]);
-              }
-              ga[i][e] *= w[z][0][e];
-              gb[i][e] *= w[z][1][e];
-              da = fmaf(ga[i][e], xa[i][e], da);
-              db = fmaf(gb[i][e], xb[i][e], db);
-            }
-            const float m = nr_sum<L>((ca < 0 ? 0.f : da) + (cb < 0 ? 0.f : db)) * inv_d;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              xa[i][e] = rstd * (ga[i][e] - xa[i][e] * m);
-              xb[i][e] = rstd * (gb[i][e] - xb[i][e] * m);
-            }
-            if (put && ca >= 0) nr_store<T, VEC>(yr + h * d.D + ca, xa[i]);
-            if (put && cb >= 0) nr_store<T, VEC>(yr + h * d.D + cb, xb[i]);
+          for (int e = 0; e < VEC; ++e) {
+            va[e] = rstd * (ua[e] - va[e] * m);
+            vb[e] = rstd * (ub[e] - vb[e] * m);
           }
         }
+        if (put && ca >= 0) nr_store<T, VEC>(yr + h * d.D + ca, va);
+        if (put && cb >= 0) nr_store<T, VEC>(yr + h * d.D + cb, vb);
       }
     }
   }
 
   if constexpr (BWD) {
     // the groups' sums of one block, in a fixed order: butterflies over the groups of a wave, then its four waves
-    __shared__ float part[NR_THREADS / 64][2][256];
+    __shared__ float part[NR_THREADS / 64][256];
     const int wave = t >> 6;
 #pragma unroll
-    for (int z = 0; z < 2; ++z)
+    for (int e = 0; e < VEC; ++e) {
+      float a = dwa[e], b = dwb[e];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        float a = dw[z][0][e], b = dw[z][1][e];
-#pragma unroll
-        for (int o = L; o < 64; o <<= 1) {
-          a += __shfl_xor(a, o, 64);
-          b += __shfl_xor(b, o, 64);
-        }
-        if ((t & 63) < L) {
-          if (ca >= 0) part[wave][z][ca + e] = a;
-          if (cb >= 0) part[wave][z][cb + e] = b;
-        }
+      for (int o = L; o < 64; o <<= 1) {
+        a += __shfl_xor(a, o, 64);
+        b += __shfl_xor(b, o, 64);
       }
+      if ((t & 63) < L) {
+        if (ca >= 0) part[wave][ca + e] = a;
+        if (cb >= 0) part[wave][cb + e] = b;
+      }
+    }
     __syncthreads();
-    for (int i = t; i < 2 * d.D; i += NR_THREADS) {
-      const int z = i / d.D, ch = i - z * d.D;
+    for (int i = t; i < d.D; i += NR_THREADS) {
       float v = 0.f;
 #pragma unroll
-      for (int k = 0; k < NR_THREADS / 64; ++k) v += part[k][z][ch];
-      d.partial[((int64_t)blockIdx.x * 2 + z) * d.D + ch] = v;
+      for (int k = 0; k < NR_THREADS / 64; ++k) v += part[k][i];
+      d.partial[((int64_t)blockIdx.x * 2 + z) * d.D + i] = v;
     }
   }
 }
 
-// dw[z][ch] = sum over blocks of partial[block][z][ch], 16 columns per workgroup, 16 strips of blocks added in order
-__global__ __launch_bounds__(256) void norm_rope_dw_kernel(const float* __restrict__ partial, int blocks, int D, void* dwq, void* dwk,
-                                                          int out_f32) {
-  __shared__ float sums[16][17];
+// dw[z][ch] = sum over blocks of partial[block][z][ch]: 16 columns per workgroup, 64 strips of blocks added in order
+__global__ __launch_bounds__(1024) void norm_rope_dw_kernel(const float* __restrict__ partial, int blocks, int D, void* dwq, void* dwk,
+                                                           int out_f32) {
+  __shared__ float sums[64][17];
   const int col = blockIdx.x * 16 + (threadIdx.x & 15), strip = threadIdx.x >> 4;
   float v = 0.f;
   if (col < 2 * D)
-    for (int b = strip; b < blocks; b += 16) v += partial[(int64_t)b * 2 * D + col];
+#pragma unroll 8
+    for (int b = strip; b < blocks; b += 64) v += partial[(int64_t)b * 2 * D + col];
   sums[strip][threadIdx.x & 15] = v;
   __syncthreads();
   if (strip == 0 && col < 2 * D) {
     float a = 0.f;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) a += sums[k][threadIdx.x];
+    for (int k = 0; k < 64; ++k) a += sums[k][threadIdx.x];
     void* dst = col < D ? dwq : dwk;
     if (!dst) return;
     const int ch = col < D ? col : col - D;
@@ -329,11 +365,11 @@ int nr_blocks(int tokens, int tpb, int limit) {
   return (int)(need < limit ? need : limit);
 }
 
-constexpr int NR_BLOCKS = 2048, NR_BWD_BLOCKS = 1024;
+constexpr int NR_BLOCKS = 2048, NR_BWD_BLOCKS = 1024;   // of the queries, and of the keys
 
 template <typename T, int VEC, bool INTER, bool BWD>
 void nr_launch(NormRope& d, int L, int blocks, hipStream_t s) {
-#define NR(l) hipLaunchKernelGGL((norm_rope_kernel<T, VEC, INTER, l, BWD>), dim3(blocks), dim3(NR_THREADS), 0, s, d)
+#define NR(l) hipLaunchKernelGGL((norm_rope_kernel<T, VEC, INTER, l, BWD>), dim3(blocks, 2), dim3(NR_THREADS), 0, s, d)
   switch (L) {
     case 1: NR(1); break;
     case 2: NR(2); break;
@@ -354,6 +390,7 @@ int nr_run(NormRope& d, int f32, int interleaved, bool bwd, hipStream_t s) {
   int gpt = 1;
   while (gpt < groups && gpt * per < heads) gpt <<= 1;
   d.gpt = gpt;
+  d.wide = d.rot > 0 && d.F % (interleaved ? vec / 2 : vec) == 0 && lbmk_aligned(d.table, 16);
   const int blocks = nr_blocks(d.tokens, groups / gpt, bwd ? NR_BWD_BLOCKS : NR_BLOCKS);
 #define NR_T(T)                                                        \
   do {                                                                 \
@@ -448,6 +485,6 @@ extern "C" int lbmk_norm_rope_bwd(const lbmk_norm_rope_desc* p, float* scratch, 
     blocks = nr_run(d, p->f32, p->interleaved, true, s);
   }
   if (dwq || dwk)
-    hipLaunchKernelGGL(norm_rope_dw_kernel, dim3((2 * p->D + 15) / 16), dim3(256), 0, s, scratch, blocks, p->D, dwq, dwk, p->w_f32);
+    hipLaunchKernelGGL(norm_rope_dw_kernel, dim3((2 * p->D + 15) / 16), dim3(1024), 0, s, scratch, blocks, p->D, dwq, dwk, p->w_f32);
   return lbmk_check_launch("norm_rope_bwd");
 }

@@ -1636,7 +1636,7 @@ def _ranged_desc(q, k, v, heads, kv_heads, head_dim, ranges, scale, cap, slopes)
 
 def ranged_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, kv_heads: int, head_dim: int,
                 ranges: Optional[torch.Tensor] = None, *, scale: Optional[float] = None, cap: float = 0.0,
-                slopes: Optional[torch.Tensor] = None, return_lse: bool = False):
+                slopes: Optional[torch.Tensor] = None, return_lse: bool = False, return_rest: bool = False):
     """Attention in which query i of row b sees the keys ranges[b, i, 0] .. ranges[b, i, 1] - 1 (``key_ranges``, or any int32
     [B, Nq, 2], clipped to the keys; None: all): o = softmax(s) v, s = cap * tanh(scale q.k / cap) - slopes[h] * distance, with
     cap 0 for no cap and slopes (f32 [heads]) None for no bias; the distance is |i + Nk - Nq - j|.  A query that sees no key
@@ -1644,29 +1644,32 @@ def ranged_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, k
 
     q: bf16 [B, Nq, heads * D], k / v: bf16 [B, Nk, kv_heads * D] (column windows of packed projections pass), key head
     h // (heads // kv_heads) serves head h; D a multiple of 8 up to 160.  ``return_lse``: also the f32 [B, heads, Nq]
-    log2-sum-exp rows that ``ranged_attn_bwd`` takes.  Not differentiable: models.layers.ranged_attention is."""
+    log2-sum-exp rows that ``ranged_attn_bwd`` takes; ``return_rest`` (with it): and what rounding took from o, bf16 like it,
+    which makes the gradients of q and k more exact.  Not differentiable: models.layers.ranged_attention is."""
     d = _ranged_desc(q, k, v, heads, kv_heads, head_dim, ranges, scale, cap, slopes)
     o = torch.empty(d.B, d.Nq, heads * head_dim, dtype=bf16, device=q.device)
     lse = torch.empty(d.B, heads, d.Nq, dtype=torch.float32, device=q.device) if return_lse else None
-    d.o, d.lse, d.ldo, d.so = o.data_ptr(), _ptr(lse), heads * head_dim, o.stride(0)
+    rest = torch.empty_like(o) if return_rest else None
+    d.o, d.rest, d.lse, d.ldo, d.so = o.data_ptr(), _ptr(rest), _ptr(lse), heads * head_dim, o.stride(0)
     with _on(q):
         check(lib.lbmk_ranged_attn(C.byref(d), _stream()), "lbmk_ranged_attn")
-    return (o, lse) if return_lse else o
+    return (o, lse, rest) if return_rest else (o, lse) if return_lse else o
 
 
 def ranged_attn_bwd(q, k, v, o, do, lse, heads: int, kv_heads: int, head_dim: int, ranges=None, *, scale: Optional[float] = None,
-                    cap: float = 0.0, slopes=None):
-    """Gradients (dq, dk, dv) of ``ranged_attn`` for its output ``o``, the output's gradient ``do`` and the rows ``lse``; the
-    gradients of shared key heads are summed in a fixed order."""
+                    cap: float = 0.0, slopes=None, rest=None):
+    """Gradients (dq, dk, dv) of ``ranged_attn`` for its output ``o`` (and ``rest``), the output's gradient ``do`` and the rows
+    ``lse``; the gradients of shared key heads are summed in a fixed order."""
     d = _ranged_desc(q, k, v, heads, kv_heads, head_dim, ranges, scale, cap, slopes)
     o, do = _attn_rows("o", o, heads, head_dim, d.B), _attn_rows("do", do, heads, head_dim, d.B)
     _want(o.shape == q.shape and do.shape == q.shape, "ranged_attn_bwd: o and do have q's shape")
     _want(lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (d.B, heads, d.Nq), f"lse: contiguous f32 [{d.B}, {heads}, {d.Nq}]")
-    _same_device(q, o, do, lse)
+    _want(rest is None or (rest.dtype == bf16 and rest.shape == q.shape and rest.is_contiguous()), "rest: contiguous bf16 of q's shape")
+    _same_device(q, o, do, lse, rest)
     new = torch.empty if d.Nq and d.B else torch.zeros      # without queries the keys' gradients are zeros that no kernel writes
     dq, dk, dv = (new(t.shape, dtype=bf16, device=q.device) for t in (q, k, v))
     scratch = torch.empty(lib.lbmk_ranged_attn_bwd_scratch_floats(d.B, heads, kv_heads, d.Nq, d.Nk, head_dim), dtype=torch.float32, device=q.device)
-    d.o, d.dout, d.lse, d.scratch = o.data_ptr(), do.data_ptr(), lse.data_ptr(), scratch.data_ptr()
+    d.o, d.rest, d.dout, d.lse, d.scratch = o.data_ptr(), _ptr(rest), do.data_ptr(), lse.data_ptr(), scratch.data_ptr()
     d.dq, d.dk, d.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
     d.ldo, d.ldg, d.so, d.sg = _ld(o), _ld(do), _sb(o), _sb(do)
     with _on(q):
