@@ -27,7 +27,7 @@ struct Ranged {
   int4* tiles;                        // [B][ceil(Nq / 32)] smallest lo, largest hi, largest lo, smallest hi of 32 queries
   int64_t sq, sk, sv, so, sg;         // batch strides
   int ldq, ldk, ldv, ldo, ldg;
-  int B, H, Hk, Nq, Nk, D, blocks, splits;
+  int B, H, Hk, Nq, Nk, D, blocks, parts, splits, cus, ordered, snake;
   float scale;
   ScoreMap map;
 };
@@ -42,50 +42,142 @@ __device__ __forceinline__ int2 row_range(const Ranged& a, int b, int q) {
   return make_int2(max(r.x, 0), min(r.y, a.Nk));
 }
 
+// Which (row of the batch, block of queries, part, head) a workgroup takes.
+//
+// Two parts per block of queries: part 1 takes the queries whose keys start behind those of the block's first query, part 0 the
+// others.  A block across two documents would walk the keys of both, one half of it idle in each, and it alone would set the
+// kernel's time; as two parts it does not.  Under a causal mask every query is of part 0, and part 1 ends at once.
+//
+// Documents and causal masks give the blocks very different numbers of keys, and a launch is often no more workgroups than the
+// chip holds at once: in any fixed order some CUs get three long ones and others three short ones.  So, with up to 512 items,
+// every workgroup ranks them by the span of keys that a few of their queries see (ties by index: a permutation, whatever the
+// ranges are) and takes the item of its own rank: the longest first.  Where the chip holds the whole launch at once (snake), every
+// other round of CUs backwards, so that a CU with a long one gets a short one beside it; otherwise the next longest goes to the
+// CU that is done first, as it should.
+// (All LDS of a kernel is one array: with a second object the compiler waits for the tile loads in flight before it reads it.)
+constexpr int ORDER_ITEMS = 512;
+__device__ __forceinline__ void block_of(const Ranged& a, int* key, int& b, int& qb, int& part, int& head) {
+  const int items = a.B * a.blocks * a.parts, total = items * a.H;
+  int id = blockIdx.x;
+  part = 0;
+  if (a.ordered) {
+    int& taken = key[ORDER_ITEMS];
+    const int round = id / a.cus, first = round * a.cus;
+    if (a.snake && (round & 1) && first + a.cus <= total) id = first + a.cus - 1 - (id - first);
+    const int half = a.B * a.blocks;                    // items from here on: part 1
+    for (int t = threadIdx.x; t < items; t += 256) {
+      const int it = t >= half ? t - half : t, tb = it / a.blocks, r0 = (it - tb * a.blocks) * RB, r1 = min(r0 + RB, a.Nq) - 1;
+      int lo = a.Nk, hi = 0;
+      const int at[3] = {r0, (r0 + r1) >> 1, r1};
+      int2 r[3];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) r[i] = row_range(a, tb, at[i]);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        const bool in = r[i].x < r[i].y && (a.parts == 1 || (r[i].x >= r[0].y) == (t >= half));
+        lo = in ? min(lo, r[i].x) : lo;
+        hi = in ? max(hi, r[i].y) : hi;
+      }
+      key[t] = (min(max(hi - lo, 0) >> 5, (1 << 21) - 1) << 9) + (ORDER_ITEMS - 1 - t);
+    }
+    const int padded = (items + 15) & ~15;
+    for (int t = items + (int)threadIdx.x; t < padded; t += 256) key[t] = -1;
+    __syncthreads();
+    for (int t = threadIdx.x; t < items; t += 256) {
+      const int mine = key[t];
+      int rank = 0;
+      for (int i = 0; i < padded; i += 16) {
+        int4 k[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) k[j] = *(const int4*)(key + i + 4 * j);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) rank += (k[j].x > mine) + (k[j].y > mine) + (k[j].z > mine) + (k[j].w > mine);
+      }
+      if (rank == id / a.H) taken = t;
+    }
+    __syncthreads();
+    const int item = __builtin_amdgcn_readfirstlane(taken);
+    part = item >= half;
+    const int it = part ? item - half : item;
+    b = it / a.blocks;
+    qb = it - b * a.blocks;
+    head = id % a.H;
+  } else {      // the last rows first: with a causal mask they have the most keys
+    const int hb = id % (a.H * a.B), at = id / (a.H * a.B);
+    part = at >= a.blocks;
+    qb = a.blocks - 1 - (part ? at - a.blocks : at);
+    b = hb / a.H;
+    head = hb - b * a.H;
+  }
+  // (uniform, and the compiler has to know: it would loop over the lanes' tile descriptors)
+  b = __builtin_amdgcn_readfirstlane(b);
+  qb = __builtin_amdgcn_readfirstlane(qb);
+  part = __builtin_amdgcn_readfirstlane(part);
+  head = __builtin_amdgcn_readfirstlane(head);
+}
+
+// whether query row `range` belongs to this part of the block that starts with query `first`
+__device__ __forceinline__ bool of_part(const Ranged& a, int b, int first, int part, int2 range) {
+  return a.parts == 1 || (range.x >= row_range(a, b, first).y) == (part != 0);
+}
+
 // the walked interval of a workgroup and what its waves need to know about theirs
 struct Walk {
   int begin, end;            // keys that some row of the workgroup sees
   int lo_min, hi_max;        // of this wave's rows (an empty row: none)
   int lo_max, hi_min;        // keys that all of them see
+  bool any;                  // some row is this workgroup's
 };
 
-__device__ __forceinline__ Walk walk_of(int2 r, int wave, int (*sm)[2]) {
+// `mine`: the row is this workgroup's (another part's counts as one that is not there)
+__device__ __forceinline__ Walk walk_of(int2 r, bool mine, int wave, int* sm) {
   const bool empty = r.x >= r.y;
   Walk w;
-  w.lo_min = wave_min_i(empty ? 0x7fffffff : r.x);
-  w.hi_max = wave_max_i(empty ? 0 : r.y);
-  w.lo_max = wave_max_i(empty ? 0x7fffffff : r.x);
-  w.hi_min = wave_min_i(empty ? 0 : r.y);
+  w.lo_min = wave_min_i(empty || !mine ? 0x7fffffff : r.x);
+  w.hi_max = wave_max_i(empty || !mine ? 0 : r.y);
+  w.lo_max = wave_max_i(!mine ? 0 : empty ? 0x7fffffff : r.x);
+  w.hi_min = wave_min_i(!mine ? 0x7fffffff : empty ? 0 : r.y);
+  const bool some = __builtin_amdgcn_ballot_w64(mine) != 0;
   if ((threadIdx.x & 63) == 0) {
-    sm[wave][0] = w.lo_min;
-    sm[wave][1] = w.hi_max;
+    sm[wave] = w.lo_min;
+    sm[4 + wave] = w.hi_max;
+    sm[8 + wave] = some;
   }
   __syncthreads();
-  w.begin = min(min(sm[0][0], sm[1][0]), min(sm[2][0], sm[3][0]));
-  w.end = max(max(sm[0][1], sm[1][1]), max(sm[2][1], sm[3][1]));
-  w.begin = __builtin_amdgcn_readfirstlane(w.begin);
-  w.end = __builtin_amdgcn_readfirstlane(w.end);
+  w.begin = __builtin_amdgcn_readfirstlane(min(min(sm[0], sm[1]), min(sm[2], sm[3])));
+  w.end = __builtin_amdgcn_readfirstlane(max(max(sm[4], sm[5]), max(sm[6], sm[7])));
+  w.any = __builtin_amdgcn_readfirstlane(sm[8] | sm[9] | sm[10] | sm[11]) != 0;
   return w;
+}
+
+// whether a wave of the workgroup says so (and every wave is done with what it did before)
+__device__ __forceinline__ bool any_wave(bool x, int wave, int* sm) {
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) sm[wave] = x;
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(sm[0] | sm[1] | sm[2] | sm[3]) != 0;
 }
 
 template <int DH>
 __global__ __launch_bounds__(256, DH <= 64 ? 3 : 2) void ranged_fwd_kernel(const Ranged a) {
   using T = Tile<DH>;
   constexpr int KS = T::KS, DT = T::DT, NI = T::CPR / 4, STAGE = 2 * TB * T::ROW;
-  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];      // two stages of (K tile, V tile)
-  __shared__ int span[4][2];
+  // two stages of (K tile, V tile), and a few words of the waves' own
+  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE + 64];
+  int* span = (int*)(smem + 2 * STAGE);
 
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int r = lane & 31, h = lane >> 5;
-  const int heads = a.H * a.B;
-  // the workgroups of the last rows first: with a causal mask they have the most keys
-  const int hb = blockIdx.x % heads, qb = a.blocks - 1 - blockIdx.x / heads;
-  const int b = hb / a.H, head = hb - b * a.H, khead = head / (a.H / a.Hk);
+  int b, qb, part, head;
+  block_of(a, (int*)smem, b, qb, part, head);
+  const int khead = head / (a.H / a.Hk);
   const int q0 = qb * RB + wave * 32, q = q0 + r, qr = min(q, a.Nq - 1);
 
   const int2 range = row_range(a, b, qr);
-  const Walk w = walk_of(range, wave, span);
+  const bool mine = of_part(a, b, qb * RB, part, range);
+  const Walk w = walk_of(range, mine, wave, span);
+  if (!w.any) return;
   const bf16_t* K = a.k + b * a.sk + (int64_t)khead * a.D;
   const bf16_t* V = a.v + b * a.sv + (int64_t)khead * a.D;
 
@@ -93,7 +185,7 @@ __global__ __launch_bounds__(256, DH <= 64 ? 3 : 2) void ranged_fwd_kernel(const
   load_frags<KS>(a.q + b * a.sq + (int64_t)qr * a.ldq + (int64_t)head * a.D, h, a.D, qf);
   const float slope = a.map.biased ? a.slopes[head] * 1.4426950408889634f : 0.f;
   const int pos = qr + a.Nk - a.Nq;
-  const unsigned len = (unsigned)max(range.y - range.x, 0);
+  const unsigned len = mine ? (unsigned)max(range.y - range.x, 0) : 0u;
 
   f32x16 o[DT];
 #pragma unroll
@@ -170,12 +262,12 @@ __global__ __launch_bounds__(256, DH <= 64 ? 3 : 2) void ranged_fwd_kernel(const
           if (k0 + (unsigned)(32 * kt + acc_row(e, 0)) >= len) s[kt][e] = -INFINITY;
     }
     // ---- online softmax: a row is the lane pair (l, l + 32) ----
-    float mx = fmaxf(fmaxf(s[0][0], s[0][1]), s[1][0]);
+    float mx = s[0][0];
 #pragma unroll
-    for (int e = 2; e < 16; e += 2) mx = fmaxf(fmaxf(mx, s[0][e]), s[0][e + 1]);
+    for (int kt = 0; kt < 2; ++kt)          // a tree of three-input maxima
 #pragma unroll
-    for (int e = 1; e < 15; e += 2) mx = fmaxf(fmaxf(mx, s[1][e]), s[1][e + 1]);
-    mx = fmaxf(mx, s[1][15]);
+      for (int e = kt == 0 ? 1 : 0; e + 1 < 16; e += 2) mx = fmaxf(fmaxf(mx, s[kt][e]), s[kt][e + 1]);
+    mx = fmaxf(mx, s[0][15]);
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * a.map.mul;
     if (__builtin_amdgcn_ballot_w64(mx > m_run + LAG) != 0) {
       const float m_new = fmaxf(m_run, mx);
@@ -224,7 +316,7 @@ __global__ __launch_bounds__(256, DH <= 64 ? 3 : 2) void ranged_fwd_kernel(const
   }
   return bad;
   };
-  if (__syncthreads_or(walk(Plain()))) {
+  if (any_wave(walk(Plain()), wave, span)) {
 #pragma unroll
     for (int i = 0; i < DT; ++i)
 #pragma unroll
@@ -237,7 +329,7 @@ __global__ __launch_bounds__(256, DH <= 64 ? 3 : 2) void ranged_fwd_kernel(const
   const float l = l_run + __shfl_xor(l_run, 32, 64);
   const bool none = range.x >= range.y;
   const float inv = none ? 0.f : 1.0f / l;
-  if (q < a.Nq) {
+  if (q < a.Nq && mine) {
     if (a.lse && h == 0) a.lse[((int64_t)b * a.H + head) * a.Nq + q] = none ? INFINITY : m_run + __builtin_amdgcn_logf(l);
     bf16_t* op = a.o + b * a.so + (int64_t)q * a.ldo + (int64_t)head * a.D;
 #pragma unroll
@@ -294,24 +386,30 @@ __device__ __forceinline__ void put_rows_f32(float* op, const f32x16 (&acc)[DT],
 
 // dQ and delta; also writes, for the second kernel, what the ranges of each 32 queries have in common
 template <int DH>
-__global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dq_kernel(const Ranged a) {
+__global__ __launch_bounds__(256, DH <= 64 ? 3 : DH <= 96 ? 2 : 1) void ranged_bwd_dq_kernel(const Ranged a) {
   using T = Tile<DH>;
   constexpr int KS = T::KS, DT = T::DT, NI = T::CPR / 4, STAGE = 2 * TB * T::ROW;
-  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
-  __shared__ int span[4][2];
+  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE + 64];
+  int* span = (int*)(smem + 2 * STAGE);
 
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int r = lane & 31, h = lane >> 5;
-  const int heads = a.H * a.B;
-  const int hb = blockIdx.x % heads, qb = a.blocks - 1 - blockIdx.x / heads;
-  const int b = hb / a.H, head = hb - b * a.H, khead = head / (a.H / a.Hk);
+  int b, qb, part, head;
+  block_of(a, (int*)smem, b, qb, part, head);
+  const int khead = head / (a.H / a.Hk);
   const int q0 = qb * RB + wave * 32, q = q0 + r, qr = min(q, a.Nq - 1);
 
   const int2 range = row_range(a, b, qr);
-  const Walk w = walk_of(range, wave, span);
-  if (a.tiles && head == 0 && lane == 0 && q0 < a.Nq)
-    a.tiles[(int64_t)b * ((a.Nq + 31) / 32) + q0 / 32] = make_int4(w.lo_min, w.hi_max, w.lo_max, w.hi_min);
+  if (head == 0 && part == 0 && q0 < a.Nq) {
+    const bool none = range.x >= range.y;
+    const int4 all = make_int4(wave_min_i(none ? 0x7fffffff : range.x), wave_max_i(none ? 0 : range.y), wave_max_i(none ? 0x7fffffff : range.x),
+                               wave_min_i(none ? 0 : range.y));
+    if (lane == 0) a.tiles[(int64_t)b * ((a.Nq + 31) / 32) + q0 / 32] = all;
+  }
+  const bool mine = of_part(a, b, qb * RB, part, range);
+  const Walk w = walk_of(range, mine, wave, span);
+  if (!w.any) return;
   const bf16_t* K = a.k + b * a.sk + (int64_t)khead * a.D;
   const bf16_t* V = a.v + b * a.sv + (int64_t)khead * a.D;
 
@@ -335,12 +433,12 @@ __global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dq_kernel(co
         for (int e = 0; e < 8; ++e) delta = fmaf((float)gf[ks][e], (float)of[ks][e], delta);
     }
     delta += __shfl_xor(delta, 32, 64);
-    if (q < a.Nq && h == 0) a.delta[stat] = delta;
+    if (q < a.Nq && mine && h == 0) a.delta[stat] = delta;
   }
   const float nl = -a.lse[stat];
   const float slope = a.map.biased ? a.slopes[head] * 1.4426950408889634f : 0.f;
   const int pos = qr + a.Nk - a.Nq;
-  const unsigned len = (unsigned)max(range.y - range.x, 0);
+  const unsigned len = mine ? (unsigned)max(range.y - range.x, 0) : 0u;
 
   f32x16 acc[DT];
 #pragma unroll
@@ -436,14 +534,14 @@ __global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dq_kernel(co
   }
   return bad;
   };
-  if (__syncthreads_or(walk(Plain()))) {
+  if (any_wave(walk(Plain()), wave, span)) {
 #pragma unroll
     for (int i = 0; i < DT; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
     walk(Guarded());
   }
-  if (q < a.Nq) put_rows<DT>(a.dq + ((int64_t)b * a.Nq + q) * a.H * a.D + (int64_t)head * a.D, acc, a.scale, h, a.D);
+  if (q < a.Nq && mine) put_rows<DT>(a.dq + ((int64_t)b * a.Nq + q) * a.H * a.D + (int64_t)head * a.D, acc, a.scale, h, a.D);
 }
 
 // dK and dV of 128 keys: walks the query tiles of every head that shares the key head.  With few workgroups the walk is cut
@@ -452,7 +550,9 @@ template <int DH>
 __global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dkv_kernel(const Ranged a) {
   using T = Tile<DH>;
   constexpr int KS = T::KS, DT = T::DT, NI = T::CPR / 4, STAGE = 2 * TB * T::ROW + 4 * TB * 4;
-  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];      // two stages of (Q, dO, and lse, delta, lo, hi of the rows)
+  // two stages of (Q, dO, and lse, delta, lo, hi of the rows)
+  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE + 64];
+  int* span = (int*)(smem + 2 * STAGE);
 
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -482,23 +582,51 @@ __global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dkv_kernel(c
   for (int dt = 0; dt < DT; ++dt) T::col_off(lane, dt, clo[dt], chi[dt]);
 
   const int nqt = (a.Nq + TB - 1) / TB, nsub = (a.Nq + 31) / 32;
-  const int64_t work = (int64_t)group * nqt;
-  const int first = (int)(work * blockIdx.y / a.splits), last = (int)(work * (blockIdx.y + 1) / a.splits);
   const int4* tiles = a.ranges ? a.tiles + (int64_t)b * nsub : nullptr;
 
-  // next unit of work from i on whose 64 queries see one of this workgroup's keys
-  auto next = [&](int i) __attribute__((always_inline)) {
-    for (; i < last && tiles; ++i) {
-      const int qt = i % nqt;
-      const int4 x = tiles[2 * qt];
-      int lo = x.x, hi = x.y;
-      if (2 * qt + 1 < nsub) {
-        const int4 y = tiles[2 * qt + 1];
-        lo = min(lo, y.x);
-        hi = max(hi, y.y);
-      }
-      if (lo < kend && hi > k0) break;
+  // whether some of the 64 queries of tile qt sees one of this workgroup's keys
+  auto sees = [&](int qt) __attribute__((always_inline)) {
+    if (!tiles) return true;
+    const int4 x = tiles[2 * qt];
+    int lo = x.x, hi = x.y;
+    if (2 * qt + 1 < nsub) {
+      const int4 y = tiles[2 * qt + 1];
+      lo = min(lo, y.x);
+      hi = max(hi, y.y);
     }
+    return lo < kend && hi > k0;
+  };
+  // a unit of work is a tile of one of the group's heads, i = head in the group * nqt + tile.  The parts get equal numbers of the
+  // tiles that see these keys: the first of this part, and how many
+  int first = 0, units;
+  {
+    int count = 0;
+    for (int t0 = 0; t0 < nqt; t0 += 64)
+      count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(t0 + lane < nqt && sees(min(t0 + lane, nqt - 1))));
+    const int64_t all = (int64_t)group * count;
+    const int u0 = (int)(all * blockIdx.y / a.splits);
+    units = (int)(all * (blockIdx.y + 1) / a.splits) - u0;
+    if (units > 0) {
+      int skip = u0 % count;
+      for (int t0 = 0;; t0 += 64) {
+        uint64_t m = __builtin_amdgcn_ballot_w64(t0 + lane < nqt && sees(min(t0 + lane, nqt - 1)));
+        const int c = __builtin_popcountll(m);
+        if (skip >= c) {
+          skip -= c;
+          continue;
+        }
+        for (; skip > 0; --skip) m &= m - 1;
+        first = u0 / count * nqt + t0 + __builtin_ctzll(m);
+        break;
+      }
+    }
+    first = __builtin_amdgcn_readfirstlane(first);
+    units = __builtin_amdgcn_readfirstlane(units);
+  }
+  // the next unit behind i (there is one)
+  auto next = [&](int i) __attribute__((always_inline)) {
+    do ++i;
+    while (!sees(i % nqt));
     return __builtin_amdgcn_readfirstlane(i);
   };
   auto stage = [&](int i, char* buf) __attribute__((always_inline)) {
@@ -520,17 +648,17 @@ __global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dkv_kernel(c
   auto walk = [&](auto form) __attribute__((always_inline)) {
   constexpr bool GUARD = decltype(form)::guard;
   bool bad = false;
-  int cur = 0, i = next(first);
-  if (i < last) stage(i, smem);
-  while (i < last) {
-    const int j = next(i + 1);
+  int cur = 0, i = first;
+  if (units > 0) stage(i, smem);
+  for (int left = units; left > 0; --left) {
+    const int j = left > 1 ? next(i) : i;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     const char* sQ = smem + cur * STAGE;
     const char* sG = sQ + TB * T::ROW;
     const float* sL = (const float*)(sG + TB * T::ROW);
     cur ^= 1;
-    if (j < last) stage(j, smem + cur * STAGE);
+    if (left > 1) stage(j, smem + cur * STAGE);
     const int gi = i / nqt, qt = i - gi * nqt, head = khead * group + gi;
     const float slope = a.map.biased ? a.slopes[head] * 1.4426950408889634f : 0.f;
     i = j;
@@ -627,7 +755,7 @@ __global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dkv_kernel(c
   }
   return bad;
   };
-  if (__syncthreads_or(walk(Plain()))) {
+  if (any_wave(walk(Plain()), wave, span)) {
 #pragma unroll
     for (int i = 0; i < DT; ++i)
 #pragma unroll
@@ -688,12 +816,22 @@ int dkv_splits(int B, int H, int Hk, int Nq, int Nk) {
   return (int)(s < 1 ? 1 : s > 8 ? 8 : s);
 }
 
+// workgroups of the row kernels that fit a CU (registers and LDS)
+int row_occupancy(int DHP) { return DHP <= 64 ? 3 : DHP <= 128 ? 2 : 1; }
+
+// ranked workgroups: where they are few enough for the order to matter and for the ranking to be cheap
+void order_blocks(Ranged& a) {
+  const int64_t n = (int64_t)a.blocks * a.H * a.B;
+  a.ordered = a.ranges && n <= 4ll * a.cus && (int64_t)a.B * a.blocks * a.parts <= ORDER_ITEMS;
+  a.snake = n <= (int64_t)row_occupancy(pad_head(a.D)) * a.cus;
+}
+
 int ranged_check(const lbmk_ranged_attn_desc* p, bool bwd) {
   LBMK_REQUIRE(p, "ranged_attn: null descriptor");
   LBMK_REQUIRE(p->D >= 8 && p->D <= 160 && p->D % 8 == 0, "ranged_attn: head_dim %d (8 ... 160, a multiple of 8)", p->D);
   LBMK_REQUIRE(p->H > 0 && p->Hk > 0 && p->H % p->Hk == 0, "ranged_attn: %d heads over %d key heads", p->H, p->Hk);
   LBMK_REQUIRE(p->B >= 0 && p->Nq >= 0 && p->Nk >= 0, "ranged_attn: negative sizes");
-  LBMK_REQUIRE((int64_t)p->B * p->H * ((p->Nq + RB - 1) / RB) < (1ll << 31) && (int64_t)p->B * p->Hk * ((p->Nk + RB - 1) / RB) < (1ll << 31) &&
+  LBMK_REQUIRE(2ll * p->B * p->H * ((p->Nq + RB - 1) / RB) < (1ll << 31) && (int64_t)p->B * p->Hk * ((p->Nk + RB - 1) / RB) < (1ll << 31) &&
                    p->Nq < (1 << 30) && p->Nk < (1 << 30) && (int64_t)(p->H / p->Hk) * ((p->Nq + TB - 1) / TB) < (1ll << 31),
                "ranged_attn: sizes");
   LBMK_REQUIRE(p->scale > 0.f && p->cap >= 0.f, "ranged_attn: scale %g, cap %g", (double)p->scale, (double)p->cap);
@@ -729,6 +867,8 @@ Ranged ranged_args(const lbmk_ranged_attn_desc* p) {
   a.ldq = p->ldq; a.ldk = p->ldk; a.ldv = p->ldv; a.ldo = p->ldo; a.ldg = p->ldg;
   a.B = p->B; a.H = p->H; a.Hk = p->Hk; a.Nq = p->Nq; a.Nk = p->Nk; a.D = p->D;
   a.splits = 1;
+  a.parts = p->ranges ? 2 : 1;
+  a.cus = lbmk_num_cus();
   a.scale = p->scale;
   const float log2e = 1.4426950408889634f;
   a.map.scale = p->scale * log2e;
@@ -739,13 +879,13 @@ Ranged ranged_args(const lbmk_ranged_attn_desc* p) {
   return a;
 }
 
-#define BY_HEAD(DHP, KERNEL, GRID)                                                               \
-  switch (DHP) {                                                                                 \
-    case 32: hipLaunchKernelGGL((KERNEL<32>), GRID, dim3(256), 0, s, a); break;                  \
-    case 64: hipLaunchKernelGGL((KERNEL<64>), GRID, dim3(256), 0, s, a); break;                  \
-    case 96: hipLaunchKernelGGL((KERNEL<96>), GRID, dim3(256), 0, s, a); break;                  \
-    case 128: hipLaunchKernelGGL((KERNEL<128>), GRID, dim3(256), 0, s, a); break;                \
-    default: hipLaunchKernelGGL((KERNEL<160>), GRID, dim3(256), 0, s, a); break;                 \
+#define BY_HEAD(DHP, LAUNCH)     \
+  switch (DHP) {                 \
+    case 32: LAUNCH(32); break;  \
+    case 64: LAUNCH(64); break;  \
+    case 96: LAUNCH(96); break;  \
+    case 128: LAUNCH(128); break; \
+    default: LAUNCH(160); break; \
   }
 
 __global__ __launch_bounds__(256) void sum_splits_kernel(const float* __restrict__ part, bf16_t* dk, bf16_t* dv, int64_t n, int splits) {
@@ -779,9 +919,12 @@ extern "C" int lbmk_ranged_attn(const lbmk_ranged_attn_desc* p, void* stream) {
   if (rc != LBMK_OK) return rc;
   if (p->B == 0 || p->Nq == 0) return LBMK_OK;
   Ranged a = ranged_args(p);
-  a.blocks = (a.Nq + RB - 1) / RB;
   hipStream_t s = (hipStream_t)stream;
-  BY_HEAD(pad_head(a.D), ranged_fwd_kernel, dim3(a.blocks * a.H * a.B));
+  a.blocks = (a.Nq + RB - 1) / RB;
+  order_blocks(a);
+#define FWD(DHP) hipLaunchKernelGGL((ranged_fwd_kernel<DHP>), dim3((unsigned)((int64_t)a.blocks * a.parts * a.H * a.B)), dim3(256), 0, s, a)
+  BY_HEAD(pad_head(a.D), FWD)
+#undef FWD
   return lbmk_check_launch("ranged_attn");
 }
 
@@ -802,11 +945,16 @@ extern "C" int lbmk_ranged_attn_bwd(const lbmk_ranged_attn_desc* p, void* stream
   a.tiles = (int4*)(p->scratch + ((int64_t)a.B * a.H * a.Nq + 3) / 4 * 4);
   hipStream_t s = (hipStream_t)stream;
   a.blocks = (a.Nq + RB - 1) / RB;
-  BY_HEAD(pad_head(a.D), ranged_bwd_dq_kernel, dim3(a.blocks * a.H * a.B));
+  order_blocks(a);
+#define DQ(DHP) hipLaunchKernelGGL((ranged_bwd_dq_kernel<DHP>), dim3((unsigned)((int64_t)a.blocks * a.parts * a.H * a.B)), dim3(256), 0, s, a)
+  BY_HEAD(pad_head(a.D), DQ)
+#undef DQ
   if (a.Nk > 0) {
     a.splits = dkv_splits(a.B, a.H, a.Hk, a.Nq, a.Nk);
     a.part = (float*)(a.tiles + (int64_t)a.B * ((a.Nq + 31) / 32));
-    BY_HEAD(pad_head(a.D), ranged_bwd_dkv_kernel, dim3((a.Nk + RB - 1) / RB * a.Hk * a.B, a.splits));
+#define DKV(DHP) hipLaunchKernelGGL((ranged_bwd_dkv_kernel<DHP>), dim3((a.Nk + RB - 1) / RB * a.Hk * a.B, a.splits), dim3(256), 0, s, a)
+    BY_HEAD(pad_head(a.D), DKV)
+#undef DKV
     if (a.splits > 1) {
       const int64_t n = (int64_t)a.B * a.Nk * a.Hk * a.D;
       hipLaunchKernelGGL(sum_splits_kernel, dim3((unsigned)((2 * n / 4 + 255) / 256)), dim3(256), 0, s, a.part, a.dk, a.dv, n, a.splits);
