@@ -287,7 +287,7 @@ typedef struct lbmk_ranged_attn_desc {
   float scale, cap;
 } lbmk_ranged_attn_desc;
 int lbmk_ranged_attn(const lbmk_ranged_attn_desc* d, void* stream);
-int64_t lbmk_ranged_attn_bwd_scratch_floats(int B, int H, int Hk, int Nq, int Nk, int D);
+int64_t lbmk_ranged_attn_bwd_scratch_floats(int B, int H, int Hk, int Nq, int Nk, int D, int ranged /* ranges != NULL */);
 int lbmk_ranged_attn_bwd(const lbmk_ranged_attn_desc* d, void* stream);
 
 /* The intervals of a batch: query i of row b stands at position p = i + Nk - Nq and sees

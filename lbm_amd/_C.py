@@ -98,7 +98,7 @@ SIGNATURES = {
     "lbmk_norm_rope_bwd_scratch_floats": (i64, [i32]),
     "lbmk_norm_rope_bwd": (i32, [C.POINTER(NormRopeDesc), vp, vp, vp, vp]),
     "lbmk_ranged_attn": (i32, [C.POINTER(RangedAttnDesc), vp]),
-    "lbmk_ranged_attn_bwd_scratch_floats": (i64, [i32] * 6),
+    "lbmk_ranged_attn_bwd_scratch_floats": (i64, [i32] * 7),
     "lbmk_ranged_attn_bwd": (i32, [C.POINTER(RangedAttnDesc), vp]),
     "lbmk_key_ranges": (i32, [vp, vp, i32, i64, vp, vp, i32, i32, i32, i32, i32, vp]),
     "lbmk_cached_attn_scratch_floats": (i64, [i32] * 6),

@@ -77,18 +77,17 @@ __global__ __launch_bounds__(256) void cached_attn_kernel(const Cached a) {
   float m_run = M_NONE, l_run = 0.f;
   constexpr float LAG = 8.f;
 
-  unsigned koffs[NI], voffs[NI];
-  T::template offsets<NI>(lane, 64, a.ldk, a.D, koffs);
-  T::template offsets<NI>(lane, 64, a.ldv, a.D, voffs);
-  int kr[KS], clo[DT], chi[DT];
+  unsigned place[NI];
+  T::template places<NI, CT>(lane, 64, a.D, place);
+  int kr[T::RK], clo[T::CD], chi[T::CD];
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) kr[ks] = T::row_off(r, ks, h);
+  for (int ks = 0; ks < T::RK; ++ks) kr[ks] = T::row_off(r, ks, h);
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) T::col_off(lane, dt, clo[dt], chi[dt]);
+  for (int dt = 0; dt < T::CD; ++dt) T::col_off(lane, dt, clo[dt], chi[dt]);
   char* mine = smem + wave * WAVE;
   auto stage = [&](int kv0, int buf) __attribute__((always_inline)) {
-    T::template stage<NI, CT>(K, kv0, c1, a.ldk, a.D, koffs, 0, 1, mine + buf * 2 * TILE);
-    T::template stage<NI, CT>(V, kv0, c1, a.ldv, a.D, voffs, 0, 1, mine + buf * 2 * TILE + TILE);
+    T::template stage<NI, CT>(K, kv0, c1, a.ldk, a.D, place, 0, 1, mine + buf * 2 * TILE);
+    T::template stage<NI, CT>(V, kv0, c1, a.ldv, a.D, place, 0, 1, mine + buf * 2 * TILE + TILE);
   };
 
   // a wave walks alone, so it alone repeats its walk where masked places held values that are not finite
@@ -113,7 +112,7 @@ __global__ __launch_bounds__(256) void cached_attn_kernel(const Cached a) {
     const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
-      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sK, kr[ks]), qf[ks], ks == 0 ? zero : s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sK, T::row_at(kr, ks)), qf[ks], ks == 0 ? zero : s, 0, 0, 0);
     if (a.map.cap_out != 0.f) {
       asm volatile("" ::: "memory");
 #pragma unroll
@@ -166,7 +165,7 @@ __global__ __launch_bounds__(256) void cached_attn_kernel(const Cached a) {
       for (int dt = 0; dt < DT; ++dt) {
         f32x16 hit = zero;
 #pragma unroll
-        for (int m = 0; m < 2; ++m) mfma_guarded(T::col_frag(sV + 16 * m * T::ROW, clo[dt], chi[dt]), pf[m], o[dt], hit);
+        for (int m = 0; m < 2; ++m) mfma_guarded(T::col_frag(sV + 16 * m * T::ROW, T::col_at(clo, dt), T::col_at(chi, dt)), pf[m], o[dt], hit);
         poison(o[dt], hit);
       }
       continue;
@@ -176,7 +175,7 @@ __global__ __launch_bounds__(256) void cached_attn_kernel(const Cached a) {
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int m = 0; m < 2; ++m)
-        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::col_frag(sV + 16 * m * T::ROW, clo[dt], chi[dt]), pf[m], o[dt], 0, 0, 0);
+        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::col_frag(sV + 16 * m * T::ROW, T::col_at(clo, dt), T::col_at(chi, dt)), pf[m], o[dt], 0, 0, 0);
   }
   return bad;
   };
@@ -290,7 +289,7 @@ extern "C" int lbmk_cached_attn(const lbmk_cached_attn_desc* p, void* stream) {
   const int ld[3] = {p->ldq, p->ldk, p->ldv};
   const int64_t st[3] = {p->sq, p->sk, p->sv};
   for (int i = 0; i < 3; ++i)
-    LBMK_REQUIRE(ld[i] % 8 == 0 && ld[i] >= (i ? p->Hk : p->H) * p->D && ld[i] <= (1 << 23) && st[i] % 8 == 0 && st[i] >= 0,
+    LBMK_REQUIRE(ld[i] % 8 == 0 && ld[i] >= (i ? p->Hk : p->H) * p->D && ld[i] <= (1 << 22) && st[i] % 8 == 0 && st[i] >= 0,
                  "cached_attn: row stride %d, batch stride %lld", ld[i], (long long)st[i]);
   Cached a = {};
   a.q = (const bf16_t*)p->q; a.k = (const bf16_t*)p->k; a.v = (const bf16_t*)p->v; a.o = (bf16_t*)p->o;

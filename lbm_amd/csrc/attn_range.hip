@@ -18,19 +18,28 @@ namespace {
 constexpr int RB = 128;   // rows (queries or keys) of a workgroup
 constexpr int TB = 64;    // tokens per tile of the walked operand
 
+typedef __attribute__((address_space(3))) char* lds_ptr;
+
 struct Ranged {
   const bf16_t *q, *k, *v, *dout;
   bf16_t *o, *rest, *dq, *dk, *dv;     // rest: [B][Nq][H * D], what rounding took from o
   float *lse, *delta, *part;          // part: f32 [2][splits][B][Nk][Hk * D] when splits > 1
   const int32_t* ranges;              // [B][Nq][2] or null: every key
   const float* slopes;                // [H]
-  int4* tiles;                        // [B][ceil(Nq / 32)] smallest lo, largest hi, largest lo, smallest hi of 32 queries
+  int4* tiles;                        // [B][2 ceil(Nq / 64)] smallest lo, largest hi, largest lo, smallest hi of 32 queries
   int64_t sq, sk, sv, so, sg;         // batch strides
   int ldq, ldk, ldv, ldo, ldg;
   int B, H, Hk, Nq, Nk, D, blocks, parts, splits, cus, ordered, snake;
   float scale;
   ScoreMap map;
 };
+
+// a kernel's arguments by the address of its argument segment: a function that it calls reads them there (scalar loads) instead of
+// taking a copy on the stack
+__device__ __forceinline__ const Ranged& kernel_args(uint64_t at) {
+  const uint64_t p = (uint64_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
+  return *(const Ranged*)(const __attribute__((address_space(4))) Ranged*)p;
+}
 
 // lowest start of a running maximum: below every score that matters, and finite, so that a row that has seen nothing yet
 // needs no special case (its exponents are -inf, its sums 0)
@@ -158,12 +167,11 @@ __device__ __forceinline__ bool any_wave(bool x, int wave, int* sm) {
   return __builtin_amdgcn_readfirstlane(sm[0] | sm[1] | sm[2] | sm[3]) != 0;
 }
 
-template <int DH>
-__global__ __launch_bounds__(256, DH <= 64 ? 3 : 2) void ranged_fwd_kernel(const Ranged a) {
+template <int DH, class Form>
+__device__ __forceinline__ bool ranged_fwd_body(const Ranged& a, char* smem) {
+  constexpr bool GUARD = Form::guard;
   using T = Tile<DH>;
   constexpr int KS = T::KS, DT = T::DT, NI = T::CPR / 4, STAGE = 2 * TB * T::ROW;
-  // two stages of (K tile, V tile), and a few words of the waves' own
-  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE + 64];
   int* span = (int*)(smem + 2 * STAGE);
 
   const int t = threadIdx.x, lane = t & 63;
@@ -177,7 +185,7 @@ __global__ __launch_bounds__(256, DH <= 64 ? 3 : 2) void ranged_fwd_kernel(const
   const int2 range = row_range(a, b, qr);
   const bool mine = of_part(a, b, qb * RB, part, range);
   const Walk w = walk_of(range, mine, wave, span);
-  if (!w.any) return;
+  if (!w.any) return false;
   const bf16_t* K = a.k + b * a.sk + (int64_t)khead * a.D;
   const bf16_t* V = a.v + b * a.sv + (int64_t)khead * a.D;
 
@@ -196,23 +204,19 @@ __global__ __launch_bounds__(256, DH <= 64 ? 3 : 2) void ranged_fwd_kernel(const
   // the maximum may lag behind a row's by 2^LAG: p <= 256, and the accumulators are rescaled a few times per row, not per tile
   constexpr float LAG = 8.f;
 
-  unsigned koffs[NI], voffs[NI];
-  T::template offsets<NI>(t, 256, a.ldk, a.D, koffs);
-  T::template offsets<NI>(t, 256, a.ldv, a.D, voffs);
-  int kr[KS], clo[DT], chi[DT];
+  unsigned place[NI];
+  T::template places<NI, TB>(t, 256, a.D, place);
+  int kr[T::RK], clo[T::CD], chi[T::CD];
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) kr[ks] = T::row_off(r, ks, h);
+  for (int ks = 0; ks < T::RK; ++ks) kr[ks] = T::row_off(r, ks, h);
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) T::col_off(lane, dt, clo[dt], chi[dt]);
+  for (int dt = 0; dt < T::CD; ++dt) T::col_off(lane, dt, clo[dt], chi[dt]);
 
   auto stage = [&](int kv0, char* buf) __attribute__((always_inline)) {
-    T::template stage<NI, TB>(K, kv0, w.end, a.ldk, a.D, koffs, wave, 4, buf);
-    T::template stage<NI, TB>(V, kv0, w.end, a.ldv, a.D, voffs, wave, 4, buf + TB * T::ROW);
+    T::template stage<NI, TB>(K, kv0, w.end, a.ldk, a.D, place, wave, 4, buf);
+    T::template stage<NI, TB>(V, kv0, w.end, a.ldv, a.D, place, wave, 4, buf + TB * T::ROW);
   };
-  // the walk over the keys; true: a masked tile holds values that are not finite, and the sums are worth nothing
-  auto walk = [&](auto form) __attribute__((always_inline)) {
-  constexpr bool GUARD = decltype(form)::guard;
-  bool bad = false;
+  bool bad = false;                  // a masked tile holds values that are not finite, and the sums are worth nothing
   if (w.begin < w.end) stage(w.begin, smem);
   int cur = 0;
   for (int kv0 = w.begin; kv0 < w.end; kv0 += TB) {
@@ -231,7 +235,7 @@ __global__ __launch_bounds__(256, DH <= 64 ? 3 : 2) void ranged_fwd_kernel(const
       const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
-        s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sK + kt * 32 * T::ROW, kr[ks]), qf[ks], ks == 0 ? zero : s[kt], 0, 0, 0);
+        s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sK + kt * 32 * T::ROW, T::row_at(kr, ks)), qf[ks], ks == 0 ? zero : s[kt], 0, 0, 0);
     }
     if (a.map.cap_out != 0.f) {
       asm volatile("" ::: "memory");           // (keeps these uniform conditions branches)
@@ -301,7 +305,7 @@ __global__ __launch_bounds__(256, DH <= 64 ? 3 : 2) void ranged_fwd_kernel(const
       for (int dt = 0; dt < DT; ++dt) {
         f32x16 hit = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int m = 0; m < 4; ++m) mfma_guarded(T::col_frag(sV + 16 * m * T::ROW, clo[dt], chi[dt]), pf[m >> 1][m & 1], o[dt], hit);
+        for (int m = 0; m < 4; ++m) mfma_guarded(T::col_frag(sV + 16 * m * T::ROW, T::col_at(clo, dt), T::col_at(chi, dt)), pf[m >> 1][m & 1], o[dt], hit);
         poison(o[dt], hit);
       }
       continue;
@@ -312,19 +316,9 @@ __global__ __launch_bounds__(256, DH <= 64 ? 3 : 2) void ranged_fwd_kernel(const
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int m = 0; m < 4; ++m)
-        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::col_frag(sV + 16 * m * T::ROW, clo[dt], chi[dt]), pf[m >> 1][m & 1], o[dt], 0, 0, 0);
+        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::col_frag(sV + 16 * m * T::ROW, T::col_at(clo, dt), T::col_at(chi, dt)), pf[m >> 1][m & 1], o[dt], 0, 0, 0);
   }
-  return bad;
-  };
-  if (any_wave(walk(Plain()), wave, span)) {
-#pragma unroll
-    for (int i = 0; i < DT; ++i)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
-    m_run = M_NONE;
-    l_run = 0.f;
-    walk(Guarded());
-  }
+  if (!GUARD && any_wave(bad, wave, span)) return true;
 
   const float l = l_run + __shfl_xor(l_run, 32, 64);
   const bool none = range.x >= range.y;
@@ -350,6 +344,19 @@ __global__ __launch_bounds__(256, DH <= 64 ? 3 : 2) void ranged_fwd_kernel(const
         }
       }
   }
+  return false;
+}
+
+// the walk again, guarded: a call, so that its registers are not the kernel's
+template <int DH>
+__device__ __attribute__((noinline)) void ranged_fwd_again(uint64_t args, lds_ptr smem) {
+  ranged_fwd_body<DH, Guarded>(kernel_args(args), (char*)smem);
+}
+
+template <int DH>
+__global__ __launch_bounds__(256, DH <= 96 ? 3 : DH <= 128 ? 2 : 1) void ranged_fwd_kernel(const Ranged a) {
+  __shared__ __attribute__((aligned(16))) char smem[2 * (2 * TB * Tile<DH>::ROW) + 64];
+  if (ranged_fwd_body<DH, Plain>(a, smem)) ranged_fwd_again<DH>((uint64_t)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr(), (lds_ptr)smem);
 }
 
 template <int DT>
@@ -385,11 +392,11 @@ __device__ __forceinline__ void put_rows_f32(float* op, const f32x16 (&acc)[DT],
 }
 
 // dQ and delta; also writes, for the second kernel, what the ranges of each 32 queries have in common
-template <int DH>
-__global__ __launch_bounds__(256, DH <= 64 ? 3 : DH <= 96 ? 2 : 1) void ranged_bwd_dq_kernel(const Ranged a) {
+template <int DH, class Form>
+__device__ __forceinline__ bool ranged_bwd_dq_body(const Ranged& a, char* smem) {
+  constexpr bool GUARD = Form::guard;
   using T = Tile<DH>;
   constexpr int KS = T::KS, DT = T::DT, NI = T::CPR / 4, STAGE = 2 * TB * T::ROW;
-  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE + 64];
   int* span = (int*)(smem + 2 * STAGE);
 
   const int t = threadIdx.x, lane = t & 63;
@@ -401,15 +408,16 @@ __global__ __launch_bounds__(256, DH <= 64 ? 3 : DH <= 96 ? 2 : 1) void ranged_b
   const int q0 = qb * RB + wave * 32, q = q0 + r, qr = min(q, a.Nq - 1);
 
   const int2 range = row_range(a, b, qr);
-  if (head == 0 && part == 0 && q0 < a.Nq) {
-    const bool none = range.x >= range.y;
+  const int groups = (a.Nq + TB - 1) / TB * 2;            // of 32 queries, the last one empty where they are an odd number
+  if (a.ranges && head == 0 && part == 0 && q0 / 32 < groups) {
+    const bool none = range.x >= range.y || q0 >= a.Nq;
     const int4 all = make_int4(wave_min_i(none ? 0x7fffffff : range.x), wave_max_i(none ? 0 : range.y), wave_max_i(none ? 0x7fffffff : range.x),
                                wave_min_i(none ? 0 : range.y));
-    if (lane == 0) a.tiles[(int64_t)b * ((a.Nq + 31) / 32) + q0 / 32] = all;
+    if (lane == 0) a.tiles[(int64_t)b * groups + q0 / 32] = all;
   }
   const bool mine = of_part(a, b, qb * RB, part, range);
   const Walk w = walk_of(range, mine, wave, span);
-  if (!w.any) return;
+  if (!w.any) return false;
   const bf16_t* K = a.k + b * a.sk + (int64_t)khead * a.D;
   const bf16_t* V = a.v + b * a.sv + (int64_t)khead * a.D;
 
@@ -445,21 +453,18 @@ __global__ __launch_bounds__(256, DH <= 64 ? 3 : DH <= 96 ? 2 : 1) void ranged_b
   for (int i = 0; i < DT; ++i)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
-  unsigned koffs[NI], voffs[NI];
-  T::template offsets<NI>(t, 256, a.ldk, a.D, koffs);
-  T::template offsets<NI>(t, 256, a.ldv, a.D, voffs);
-  int kr[KS], clo[DT], chi[DT];
+  unsigned place[NI];
+  T::template places<NI, TB>(t, 256, a.D, place);
+  int kr[T::RK], clo[T::CD], chi[T::CD];
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) kr[ks] = T::row_off(r, ks, h);
+  for (int ks = 0; ks < T::RK; ++ks) kr[ks] = T::row_off(r, ks, h);
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) T::col_off(lane, dt, clo[dt], chi[dt]);
+  for (int dt = 0; dt < T::CD; ++dt) T::col_off(lane, dt, clo[dt], chi[dt]);
 
   auto stage = [&](int kv0, char* buf) __attribute__((always_inline)) {
-    T::template stage<NI, TB>(K, kv0, w.end, a.ldk, a.D, koffs, wave, 4, buf);
-    T::template stage<NI, TB>(V, kv0, w.end, a.ldv, a.D, voffs, wave, 4, buf + TB * T::ROW);
+    T::template stage<NI, TB>(K, kv0, w.end, a.ldk, a.D, place, wave, 4, buf);
+    T::template stage<NI, TB>(V, kv0, w.end, a.ldv, a.D, place, wave, 4, buf + TB * T::ROW);
   };
-  auto walk = [&](auto form) __attribute__((always_inline)) {
-  constexpr bool GUARD = decltype(form)::guard;
   bool bad = false;
   if (w.begin < w.end) stage(w.begin, smem);
   int cur = 0;
@@ -480,10 +485,10 @@ __global__ __launch_bounds__(256, DH <= 64 ? 3 : DH <= 96 ? 2 : 1) void ranged_b
       f32x16 s, dp;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
-        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sK + kt * 32 * T::ROW, kr[ks]), qf[ks], ks == 0 ? zero : s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sK + kt * 32 * T::ROW, T::row_at(kr, ks)), qf[ks], ks == 0 ? zero : s, 0, 0, 0);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
-        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sV + kt * 32 * T::ROW, kr[ks]), gf[ks], ks == 0 ? zero : dp, 0, 0, 0);
+        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sV + kt * 32 * T::ROW, T::row_at(kr, ks)), gf[ks], ks == 0 ? zero : dp, 0, 0, 0);
 #pragma unroll
       for (int e = 0; e < 16; ++e) dp[e] -= delta;
       if (a.map.cap_out != 0.f) {
@@ -520,7 +525,7 @@ __global__ __launch_bounds__(256, DH <= 64 ? 3 : DH <= 96 ? 2 : 1) void ranged_b
         for (int dt = 0; dt < DT; ++dt) {
           f32x16 hit = zero;
 #pragma unroll
-          for (int ss = 0; ss < 2; ++ss) mfma_guarded(T::col_frag(sk + 16 * ss * T::ROW, clo[dt], chi[dt]), df[ss], acc[dt], hit);
+          for (int ss = 0; ss < 2; ++ss) mfma_guarded(T::col_frag(sk + 16 * ss * T::ROW, T::col_at(clo, dt), T::col_at(chi, dt)), df[ss], acc[dt], hit);
           poison(acc[dt], hit);
         }
         continue;
@@ -529,37 +534,105 @@ __global__ __launch_bounds__(256, DH <= 64 ? 3 : DH <= 96 ? 2 : 1) void ranged_b
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int ss = 0; ss < 2; ++ss)
-          acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::col_frag(sk + 16 * ss * T::ROW, clo[dt], chi[dt]), df[ss], acc[dt], 0, 0, 0);
+          acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::col_frag(sk + 16 * ss * T::ROW, T::col_at(clo, dt), T::col_at(chi, dt)), df[ss], acc[dt], 0, 0, 0);
     }
   }
-  return bad;
-  };
-  if (any_wave(walk(Plain()), wave, span)) {
-#pragma unroll
-    for (int i = 0; i < DT; ++i)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
-    walk(Guarded());
-  }
+  if (!GUARD && any_wave(bad, wave, span)) return true;
   if (q < a.Nq && mine) put_rows<DT>(a.dq + ((int64_t)b * a.Nq + q) * a.H * a.D + (int64_t)head * a.D, acc, a.scale, h, a.D);
+  return false;
+}
+
+// the walk again, guarded: a call, so that its registers are not the kernel's
+template <int DH>
+__device__ __attribute__((noinline)) void ranged_bwd_dq_again(uint64_t args, lds_ptr smem) {
+  ranged_bwd_dq_body<DH, Guarded>(kernel_args(args), (char*)smem);
+}
+
+template <int DH>
+__global__ __launch_bounds__(256, DH <= 64 ? 3 : DH <= 96 ? 2 : 1) void ranged_bwd_dq_kernel(const Ranged a) {
+  __shared__ __attribute__((aligned(16))) char smem[2 * (2 * TB * Tile<DH>::ROW) + 64];
+  if (ranged_bwd_dq_body<DH, Plain>(a, smem)) ranged_bwd_dq_again<DH>((uint64_t)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr(), (lds_ptr)smem);
+}
+
+// Which (row of the batch, block of keys, key head, part of the walk) a workgroup of the key kernel takes: as block_of, ranked by
+// the number of 32-query groups that see the block, which the first kernel has summarised.
+constexpr int ORDER_GROUPS = 4096;
+__device__ __forceinline__ void keys_of(const Ranged& a, char* smem, int& b, int& kb, int& khead, int& cut) {
+  const int blocks = (a.Nk + RB - 1) / RB, items = a.B * blocks, total = items * a.Hk * a.splits;
+  int id = blockIdx.x;
+  if (a.ordered) {
+    const int nsub = (a.Nq + TB - 1) / TB * 2;
+    int2* span = (int2*)smem;
+    int* key = (int*)(smem + ORDER_GROUPS * 8 - (ORDER_ITEMS / 2 + 16) * 4);
+    int& taken = key[ORDER_ITEMS / 2];
+    const int round = id / a.cus, first = round * a.cus;
+    if (a.snake && (round & 1) && first + a.cus <= total) id = first + a.cus - 1 - (id - first);
+    for (int i = threadIdx.x; i < a.B * nsub; i += 256) {
+      const int4 x = a.tiles[i];
+      span[i] = make_int2(x.x, x.y);
+    }
+    __syncthreads();
+    const int t = threadIdx.x;
+    int mine = -1;
+    if (t < items) {
+      const int tb = t / blocks, k0 = (t - tb * blocks) * RB, k1 = min(k0 + RB, a.Nk);
+      int n = 0;
+#pragma unroll 8
+      for (int i = 0; i < nsub; ++i) {
+        const int2 x = span[tb * nsub + i];
+        n += x.x < k1 && x.y > k0;
+      }
+      mine = (n << 8) + (ORDER_ITEMS / 2 - 1 - t);
+    }
+    __syncthreads();                      // (the keys lie over the last spans)
+    key[t] = mine;
+    __syncthreads();
+    if (t < items) {
+      int rank = 0;
+      for (int i = 0; i < items; i += 16) {
+        int4 k[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) k[j] = *(const int4*)(key + i + 4 * j);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) rank += (k[j].x > mine) + (k[j].y > mine) + (k[j].z > mine) + (k[j].w > mine);
+      }
+      if (rank == id / (a.Hk * a.splits)) taken = t;
+    }
+    __syncthreads();
+    const int item = __builtin_amdgcn_readfirstlane(taken), rest = id % (a.Hk * a.splits);
+    __syncthreads();                      // (the tiles go over it)
+    b = item / blocks;
+    kb = item - b * blocks;
+    khead = rest % a.Hk;
+    cut = rest / a.Hk;
+  } else {      // the first keys first: with a causal mask most queries see them
+    const int per = a.Hk * a.B * a.splits, rest = id % per;
+    kb = id / per;
+    cut = rest / (a.Hk * a.B);
+    b = rest / a.Hk % a.B;
+    khead = rest % a.Hk;
+  }
+  b = __builtin_amdgcn_readfirstlane(b);
+  kb = __builtin_amdgcn_readfirstlane(kb);
+  khead = __builtin_amdgcn_readfirstlane(khead);
+  cut = __builtin_amdgcn_readfirstlane(cut);
 }
 
 // dK and dV of 128 keys: walks the query tiles of every head that shares the key head.  With few workgroups the walk is cut
 // into `splits` parts whose sums are added afterwards in their order.
-template <int DH>
-__global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dkv_kernel(const Ranged a) {
+template <int DH, class Form>
+__device__ __forceinline__ bool ranged_bwd_dkv_body(const Ranged& a, char* smem) {
+  constexpr bool GUARD = Form::guard;
   using T = Tile<DH>;
   constexpr int KS = T::KS, DT = T::DT, NI = T::CPR / 4, STAGE = 2 * TB * T::ROW + 4 * TB * 4;
-  // two stages of (Q, dO, and lse, delta, lo, hi of the rows)
-  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE + 64];
   int* span = (int*)(smem + 2 * STAGE);
 
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int r = lane & 31, h = lane >> 5;
-  const int heads = a.Hk * a.B, group = a.H / a.Hk;
-  const int hb = blockIdx.x % heads, kb = blockIdx.x / heads;       // the first keys first: with a causal mask most rows see them
-  const int b = hb / a.Hk, khead = hb - b * a.Hk;
+  const int group = a.H / a.Hk;
+  int b, kb, khead, cut;
+  keys_of(a, smem, b, kb, khead, cut);
   const int k0 = kb * RB, kw = k0 + wave * 32, key = kw + r, kc = min(key, a.Nk - 1);
   const int kend = min(k0 + RB, a.Nk);
 
@@ -572,86 +645,121 @@ __global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dkv_kernel(c
 #pragma unroll
     for (int e = 0; e < 16; ++e) dk[i][e] = dv[i][e] = 0.f;
 
-  unsigned qoffs[NI], goffs[NI];
-  T::template offsets<NI>(t, 256, a.ldq, a.D, qoffs);
-  T::template offsets<NI>(t, 256, a.ldg, a.D, goffs);
-  int rr[KS], clo[DT], chi[DT];
+  unsigned place[NI];
+  T::template places<NI, TB>(t, 256, a.D, place);
+  int rr[T::RK], clo[T::CD], chi[T::CD];
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) rr[ks] = T::row_off(r, ks, h);
+  for (int ks = 0; ks < T::RK; ++ks) rr[ks] = T::row_off(r, ks, h);
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) T::col_off(lane, dt, clo[dt], chi[dt]);
+  for (int dt = 0; dt < T::CD; ++dt) T::col_off(lane, dt, clo[dt], chi[dt]);
 
-  const int nqt = (a.Nq + TB - 1) / TB, nsub = (a.Nq + 31) / 32;
-  const int4* tiles = a.ranges ? a.tiles + (int64_t)b * nsub : nullptr;
-
-  // whether some of the 64 queries of tile qt sees one of this workgroup's keys
-  auto sees = [&](int qt) __attribute__((always_inline)) {
-    if (!tiles) return true;
-    const int4 x = tiles[2 * qt];
-    int lo = x.x, hi = x.y;
-    if (2 * qt + 1 < nsub) {
-      const int4 y = tiles[2 * qt + 1];
-      lo = min(lo, y.x);
-      hi = max(hi, y.y);
-    }
-    return lo < kend && hi > k0;
+  const int nqt = (a.Nq + TB - 1) / TB;
+  // the summaries of a tile's two groups of 32 queries, by scalar loads (uniform, and written by the kernel before)
+  typedef int i32x4 __attribute__((ext_vector_type(4)));
+  typedef const __attribute__((address_space(4))) i32x4* summary_t;
+  const bool ranged = a.ranges != nullptr;
+  const summary_t tiles = (summary_t)(uintptr_t)(a.tiles + (int64_t)b * 2 * nqt);
+  const int4* lane_tiles = a.tiles + (int64_t)b * 2 * nqt;
+  struct Seen {
+    i32x4 u[2];
   };
-  // a unit of work is a tile of one of the group's heads, i = head in the group * nqt + tile.  The parts get equal numbers of the
-  // tiles that see these keys: the first of this part, and how many
-  int first = 0, units;
+  auto summary = [&](int qt) __attribute__((always_inline)) {
+    Seen x = {};
+    if (ranged) {
+      x.u[0] = tiles[2 * qt];
+      x.u[1] = tiles[2 * qt + 1];
+    }
+    return x;
+  };
+  // whether some of the 64 queries sees one of this workgroup's keys
+  auto sees = [&](const Seen& x) __attribute__((always_inline)) {
+    return !ranged || (min(x.u[0][0], x.u[1][0]) < kend && max(x.u[0][1], x.u[1][1]) > k0);
+  };
+  auto lane_sees = [&](int i) __attribute__((always_inline)) {
+    if (i >= nqt) return false;
+    if (!ranged) return true;
+    const int4 x = lane_tiles[2 * (nqt - 1 - i)], y = lane_tiles[2 * (nqt - 1 - i) + 1];
+    return min(x.x, y.x) < kend && max(x.y, y.y) > k0;
+  };
+  // a unit of work is a tile of one of the group's heads; each head's tiles are taken from the last one on: under a causal mask
+  // the workgroups of a head all see the last tiles, and so read them at the same time.  The parts get equal numbers of the tiles
+  // that see these keys: the first of this part, and how many
+  struct Unit {
+    int head, tile;
+  };
+  Unit first = {0, nqt - 1};
+  int units;
   {
     int count = 0;
     for (int t0 = 0; t0 < nqt; t0 += 64)
-      count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(t0 + lane < nqt && sees(min(t0 + lane, nqt - 1))));
+      count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(lane_sees(t0 + lane)));
     const int64_t all = (int64_t)group * count;
-    const int u0 = (int)(all * blockIdx.y / a.splits);
-    units = (int)(all * (blockIdx.y + 1) / a.splits) - u0;
+    const int u0 = (int)(all * cut / a.splits);
+    units = (int)(all * (cut + 1) / a.splits) - u0;
     if (units > 0) {
       int skip = u0 % count;
       for (int t0 = 0;; t0 += 64) {
-        uint64_t m = __builtin_amdgcn_ballot_w64(t0 + lane < nqt && sees(min(t0 + lane, nqt - 1)));
+        uint64_t m = __builtin_amdgcn_ballot_w64(lane_sees(t0 + lane));
         const int c = __builtin_popcountll(m);
         if (skip >= c) {
           skip -= c;
           continue;
         }
         for (; skip > 0; --skip) m &= m - 1;
-        first = u0 / count * nqt + t0 + __builtin_ctzll(m);
+        first.head = u0 / count;
+        first.tile = nqt - 1 - (t0 + __builtin_ctzll(m));
         break;
       }
     }
-    first = __builtin_amdgcn_readfirstlane(first);
+    first.head = __builtin_amdgcn_readfirstlane(first.head);
+    first.tile = __builtin_amdgcn_readfirstlane(first.tile);
     units = __builtin_amdgcn_readfirstlane(units);
   }
-  // the next unit behind i (there is one)
-  auto next = [&](int i) __attribute__((always_inline)) {
-    do ++i;
-    while (!sees(i % nqt));
-    return __builtin_amdgcn_readfirstlane(i);
+  auto behind = [&](Unit u) __attribute__((always_inline)) {
+    const bool wrap = u.tile == 0;
+    return Unit{u.head + wrap, wrap ? nqt - 1 : u.tile - 1};
   };
-  auto stage = [&](int i, char* buf) __attribute__((always_inline)) {
-    const int gi = i / nqt, qt = i - gi * nqt, head = khead * group + gi, q0 = qt * TB;
-    T::template stage<NI, TB>(a.q + b * a.sq + (int64_t)head * a.D, q0, a.Nq, a.ldq, a.D, qoffs, wave, 4, buf);
-    T::template stage<NI, TB>(a.dout + b * a.sg + (int64_t)head * a.D, q0, a.Nq, a.ldg, a.D, goffs, wave, 4, buf + TB * T::ROW);
-    // one wave per row statistic; rows past the end read zeros (their q and dO are zeros too: they add nothing)
-    const int rows = min(TB, a.Nq - q0);
-    const int64_t st = ((int64_t)b * a.H + head) * a.Nq + q0;
-    if (wave < 2 || a.ranges) {
-      const void* base = wave == 0 ? (const void*)(a.lse + st) : wave == 1 ? (const void*)(a.delta + st)
-                                                                           : (const void*)(a.ranges + ((int64_t)b * a.Nq + q0) * 2);
-      const unsigned off = wave < 2 ? lane * 4u : lane * 8u + (wave == 3 ? 4u : 0u);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)base, 0, rows * (wave < 2 ? 4 : 8), 0x00020000),
-                                               (__attribute__((address_space(3))) void*)(buf + 2 * TB * T::ROW + wave * TB * 4), 4, off, 0, 0, 0);
+  // from unit i on (there is one), the first that sees the keys; x: its summaries
+  auto settle = [&](Unit& i, Seen& x) __attribute__((always_inline)) {
+    while (!sees(x)) {
+      i = behind(i);
+      x = summary(i.tile);
     }
   };
+  // row statistics, one kind per wave: lse and delta of the head, first and last key of the batch row's queries
+  const bf16_t* qh = a.q + b * a.sq + (int64_t)khead * group * a.D;
+  const bf16_t* gh = a.dout + b * a.sg + (int64_t)khead * group * a.D;
+  const int stat_row = wave < 2 ? 4 : 8;                 // bytes per query
+  const int64_t stat_head = wave < 2 ? (int64_t)a.Nq * 4 : 0;
+  const char* stat = wave < 2 ? (const char*)((wave == 0 ? a.lse : a.delta) + ((int64_t)b * a.H + khead * group) * a.Nq)
+                              : (const char*)(a.ranges + (int64_t)b * a.Nq * 2);
+  const unsigned stat_lane = (unsigned)(lane * stat_row + (wave == 3 ? 4 : 0));
+  const bool stat_wanted = wave < 2 || ranged;
+  auto stage = [&](Unit i, char* buf) __attribute__((always_inline)) {
+    const int q0 = i.tile * TB;
+    T::template stage<NI, TB>(qh + (int64_t)i.head * a.D, q0, a.Nq, a.ldq, a.D, place, wave, 4, buf);
+    T::template stage<NI, TB>(gh + (int64_t)i.head * a.D, q0, a.Nq, a.ldg, a.D, place, wave, 4, buf + TB * T::ROW);
+    // rows past the end read zeros (their q and dO are zeros too: they add nothing)
+    if (stat_wanted)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          __builtin_amdgcn_make_buffer_rsrc((void*)(stat + i.head * stat_head + (int64_t)q0 * stat_row), 0, min(TB, a.Nq - q0) * stat_row, 0x00020000),
+          (__attribute__((address_space(3))) void*)(buf + 2 * TB * T::ROW + wave * TB * 4), 4, stat_lane, 0, 0, 0);
+  };
 
-  auto walk = [&](auto form) __attribute__((always_inline)) {
-  constexpr bool GUARD = decltype(form)::guard;
   bool bad = false;
-  int cur = 0, i = first;
-  if (units > 0) stage(i, smem);
+  int cur = 0, head = -1;
+  Unit i = first, j = behind(first);
+  float slope = 0.f;
+  Seen x = {}, y = {};
+  if (units > 0) {
+    stage(i, smem);
+    x = summary(i.tile);
+    if (units > 1) {
+      y = summary(j.tile);
+      settle(j, y);
+    }
+  }
   for (int left = units; left > 0; --left) {
-    const int j = left > 1 ? next(i) : i;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     const char* sQ = smem + cur * STAGE;
@@ -659,27 +767,30 @@ __global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dkv_kernel(c
     const float* sL = (const float*)(sG + TB * T::ROW);
     cur ^= 1;
     if (left > 1) stage(j, smem + cur * STAGE);
-    const int gi = i / nqt, qt = i - gi * nqt, head = khead * group + gi;
-    const float slope = a.map.biased ? a.slopes[head] * 1.4426950408889634f : 0.f;
+    const int qt = i.tile;
+    if (a.map.biased && head != i.head) slope = a.slopes[khead * group + i.head] * 1.4426950408889634f;
+    head = i.head;
+    const Seen now = x;
     i = j;
+    x = y;
+    j = behind(j);
+    if (left > 2) y = summary(j.tile);                  // used after this tile's products
 
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       bool masked = false;
-      if (tiles) {
-        if (2 * qt + u >= nsub) continue;
-        const int4 x = tiles[2 * qt + u];
-        if (x.x >= kw + 32 || x.y <= kw) continue;          // none of these queries sees a key of this wave
-        masked = x.z > kw || x.w < kw + 32;
+      if (ranged) {
+        if (now.u[u][0] >= kw + 32 || now.u[u][1] <= kw) continue;      // none of these queries sees a key of this wave
+        masked = now.u[u][2] > kw || now.u[u][3] < kw + 32;
       }
       const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       f32x16 s, dp;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
-        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sQ + u * 32 * T::ROW, rr[ks]), kf[ks], ks == 0 ? zero : s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sQ + u * 32 * T::ROW, T::row_at(rr, ks)), kf[ks], ks == 0 ? zero : s, 0, 0, 0);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
-        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sG + u * 32 * T::ROW, rr[ks]), vf[ks], ks == 0 ? zero : dp, 0, 0, 0);
+        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sG + u * 32 * T::ROW, T::row_at(rr, ks)), vf[ks], ks == 0 ? zero : dp, 0, 0, 0);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const f32x4 d4 = *(const f32x4*)(sL + TB + 32 * u + 8 * g + 4 * h);
@@ -735,8 +846,8 @@ __global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dkv_kernel(c
           f32x16 hq = zero, hg = zero;
 #pragma unroll
           for (int ss = 0; ss < 2; ++ss) {
-            mfma_guarded(T::col_frag(sg + 16 * ss * T::ROW, clo[dt], chi[dt]), pf[ss], dv[dt], hg);
-            mfma_guarded(T::col_frag(sq + 16 * ss * T::ROW, clo[dt], chi[dt]), df[ss], dk[dt], hq);
+            mfma_guarded(T::col_frag(sg + 16 * ss * T::ROW, T::col_at(clo, dt), T::col_at(chi, dt)), pf[ss], dv[dt], hg);
+            mfma_guarded(T::col_frag(sq + 16 * ss * T::ROW, T::col_at(clo, dt), T::col_at(chi, dt)), df[ss], dk[dt], hq);
           }
           poison(dv[dt], hg);
           poison(dk[dt], hq);
@@ -745,34 +856,41 @@ __global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dkv_kernel(c
       }
       if (!GUARD && masked) bad |= tile_not_finite<32 * T::ROW>(sq, lane) | tile_not_finite<32 * T::ROW>(sg, lane);
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
+      for (int dt = 0; dt < DT; ++dt) {
 #pragma unroll
         for (int ss = 0; ss < 2; ++ss) {
-          dv[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::col_frag(sg + 16 * ss * T::ROW, clo[dt], chi[dt]), pf[ss], dv[dt], 0, 0, 0);
-          dk[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::col_frag(sq + 16 * ss * T::ROW, clo[dt], chi[dt]), df[ss], dk[dt], 0, 0, 0);
+          dv[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::col_frag(sg + 16 * ss * T::ROW, T::col_at(clo, dt), T::col_at(chi, dt)), pf[ss], dv[dt], 0, 0, 0);
+          dk[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::col_frag(sq + 16 * ss * T::ROW, T::col_at(clo, dt), T::col_at(chi, dt)), df[ss], dk[dt], 0, 0, 0);
         }
+      }
     }
+    if (left > 2) settle(j, y);
   }
-  return bad;
-  };
-  if (any_wave(walk(Plain()), wave, span)) {
-#pragma unroll
-    for (int i = 0; i < DT; ++i)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) dk[i][e] = dv[i][e] = 0.f;
-    walk(Guarded());
-  }
+  if (!GUARD && any_wave(bad, wave, span)) return true;
   if (key < a.Nk) {
     const int64_t at = ((int64_t)b * a.Nk + key) * a.Hk * a.D + (int64_t)khead * a.D;
     if (a.splits > 1) {
       const int64_t all = (int64_t)a.B * a.Nk * a.Hk * a.D;
-      put_rows_f32<DT>(a.part + (int64_t)blockIdx.y * all + at, dk, a.scale, h, a.D);
-      put_rows_f32<DT>(a.part + (int64_t)(a.splits + blockIdx.y) * all + at, dv, 1.f, h, a.D);
+      put_rows_f32<DT>(a.part + (int64_t)cut * all + at, dk, a.scale, h, a.D);
+      put_rows_f32<DT>(a.part + (int64_t)(a.splits + cut) * all + at, dv, 1.f, h, a.D);
     } else {
       put_rows<DT>(a.dk + at, dk, a.scale, h, a.D);
       put_rows<DT>(a.dv + at, dv, 1.f, h, a.D);
     }
   }
+  return false;
+}
+
+// the walk again, guarded: a call, so that its registers are not the kernel's
+template <int DH>
+__device__ __attribute__((noinline)) void ranged_bwd_dkv_again(uint64_t args, lds_ptr smem) {
+  ranged_bwd_dkv_body<DH, Guarded>(kernel_args(args), (char*)smem);
+}
+
+template <int DH>
+__global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dkv_kernel(const Ranged a) {
+  __shared__ __attribute__((aligned(16))) char smem[2 * (2 * TB * Tile<DH>::ROW + 4 * TB * 4) + 64];
+  if (ranged_bwd_dkv_body<DH, Plain>(a, smem)) ranged_bwd_dkv_again<DH>((uint64_t)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr(), (lds_ptr)smem);
 }
 
 // The interval of keys that each query of a packed, padded or generated batch sees (see lbmk_key_ranges)
@@ -808,11 +926,16 @@ __global__ __launch_bounds__(256) void key_ranges_kernel(int32_t* out, const int
 
 int pad_head(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 160; }
 
-// splits of the key kernel's walk: enough workgroups for two per CU, at least four tiles each, at most eight parts
-int dkv_splits(int B, int H, int Hk, int Nq, int Nk) {
+// parts of the key kernel's walk: enough workgroups for every CU to hold its fill (two of up to 96 channels, one wider).  Where
+// ranges make the walks unequal and they are long, twice as many, so that the next part goes to the CU that is done first.  A part
+// costs its f32 sums (8 bytes per element of dK and dV written and read): never more than eight, none below eight tiles.
+int dkv_splits(bool ranged, int B, int H, int Hk, int Nq, int Nk, int D) {
   const int64_t blocks = (int64_t)((Nk + RB - 1) / RB) * Hk * B, work = (int64_t)(H / Hk) * ((Nq + TB - 1) / TB);
-  int64_t s = (2ll * lbmk_num_cus() + blocks - 1) / (blocks > 0 ? blocks : 1);
-  if (s > work / 4) s = work / 4;
+  const int64_t slots = (D <= 96 ? 2ll : 1ll) * lbmk_num_cus();
+  if (blocks <= 0) return 1;
+  int64_t s = (slots + blocks - 1) / blocks;
+  if (ranged && blocks * s < 2 * slots && work / s >= 64) s *= 2;
+  if (s > work / 8) s = work / 8;
   return (int)(s < 1 ? 1 : s > 8 ? 8 : s);
 }
 
@@ -831,7 +954,7 @@ int ranged_check(const lbmk_ranged_attn_desc* p, bool bwd) {
   LBMK_REQUIRE(p->D >= 8 && p->D <= 160 && p->D % 8 == 0, "ranged_attn: head_dim %d (8 ... 160, a multiple of 8)", p->D);
   LBMK_REQUIRE(p->H > 0 && p->Hk > 0 && p->H % p->Hk == 0, "ranged_attn: %d heads over %d key heads", p->H, p->Hk);
   LBMK_REQUIRE(p->B >= 0 && p->Nq >= 0 && p->Nk >= 0, "ranged_attn: negative sizes");
-  LBMK_REQUIRE(2ll * p->B * p->H * ((p->Nq + RB - 1) / RB) < (1ll << 31) && (int64_t)p->B * p->Hk * ((p->Nk + RB - 1) / RB) < (1ll << 31) &&
+  LBMK_REQUIRE(2ll * p->B * p->H * ((p->Nq + RB - 1) / RB) < (1ll << 31) && 8ll * p->B * p->Hk * ((p->Nk + RB - 1) / RB) < (1ll << 31) &&
                    p->Nq < (1 << 30) && p->Nk < (1 << 30) && (int64_t)(p->H / p->Hk) * ((p->Nq + TB - 1) / TB) < (1ll << 31),
                "ranged_attn: sizes");
   LBMK_REQUIRE(p->scale > 0.f && p->cap >= 0.f, "ranged_attn: scale %g, cap %g", (double)p->scale, (double)p->cap);
@@ -845,7 +968,7 @@ int ranged_check(const lbmk_ranged_attn_desc* p, bool bwd) {
     LBMK_REQUIRE(ptr[i] && lbmk_aligned(ptr[i], 16), "ranged_attn: null or misaligned pointer (rows start on 16 bytes)");
     if (i == 3 || i >= 6) continue;
     const int64_t wide = (int64_t)(i < 4 ? p->H : p->Hk) * p->D;
-    LBMK_REQUIRE(ld[i] % 8 == 0 && ld[i] >= wide && ld[i] <= (1 << 23) && st[i] % 8 == 0 && st[i] >= 0, "ranged_attn: row stride %d, batch stride %lld",
+    LBMK_REQUIRE(ld[i] % 8 == 0 && ld[i] >= wide && ld[i] <= (1 << 22) && st[i] % 8 == 0 && st[i] >= 0, "ranged_attn: row stride %d, batch stride %lld",
                  ld[i], (long long)st[i]);
   }
   LBMK_REQUIRE(!p->ranges || lbmk_aligned(p->ranges, 8), "ranged_attn: misaligned ranges");
@@ -929,10 +1052,10 @@ extern "C" int lbmk_ranged_attn(const lbmk_ranged_attn_desc* p, void* stream) {
 }
 
 // delta [B][H][Nq], the summaries of the queries' ranges, and the parts of the key kernel
-extern "C" int64_t lbmk_ranged_attn_bwd_scratch_floats(int B, int H, int Hk, int Nq, int Nk, int D) {
+extern "C" int64_t lbmk_ranged_attn_bwd_scratch_floats(int B, int H, int Hk, int Nq, int Nk, int D, int ranged) {
   if (B <= 0 || H <= 0 || Hk <= 0 || Nq <= 0 || H % Hk) return 0;
-  const int64_t delta = ((int64_t)B * H * Nq + 3) / 4 * 4, tiles = (int64_t)B * ((Nq + 31) / 32) * 4;
-  const int splits = dkv_splits(B, H, Hk, Nq, Nk);
+  const int64_t delta = ((int64_t)B * H * Nq + 3) / 4 * 4, tiles = (int64_t)B * ((Nq + TB - 1) / TB) * 8;
+  const int splits = dkv_splits(ranged != 0, B, H, Hk, Nq, Nk, D);
   return delta + tiles + (splits > 1 ? 2ll * splits * B * Nk * Hk * D : 0);
 }
 
@@ -950,14 +1073,18 @@ extern "C" int lbmk_ranged_attn_bwd(const lbmk_ranged_attn_desc* p, void* stream
   BY_HEAD(pad_head(a.D), DQ)
 #undef DQ
   if (a.Nk > 0) {
-    a.splits = dkv_splits(a.B, a.H, a.Hk, a.Nq, a.Nk);
-    a.part = (float*)(a.tiles + (int64_t)a.B * ((a.Nq + 31) / 32));
-#define DKV(DHP) hipLaunchKernelGGL((ranged_bwd_dkv_kernel<DHP>), dim3((a.Nk + RB - 1) / RB * a.Hk * a.B, a.splits), dim3(256), 0, s, a)
+    a.splits = dkv_splits(a.ranges != nullptr, a.B, a.H, a.Hk, a.Nq, a.Nk, a.D);
+    const int64_t kblocks = (a.Nk + RB - 1) / RB, n = kblocks * a.Hk * a.B * a.splits;
+    // (32 KB of LDS for the queries' spans: a stage pair of the narrowest heads is smaller)
+    a.ordered = a.ranges && a.D > 32 && n <= 8ll * a.cus && kblocks * a.B <= ORDER_ITEMS / 2 && (int64_t)a.B * ((a.Nq + TB - 1) / TB) * 2 <= ORDER_GROUPS - 256;
+    a.snake = n <= (a.D <= 96 ? 2ll : 1ll) * a.cus;
+    a.part = (float*)(a.tiles + (int64_t)a.B * ((a.Nq + TB - 1) / TB) * 2);
+#define DKV(DHP) hipLaunchKernelGGL((ranged_bwd_dkv_kernel<DHP>), dim3((unsigned)((int64_t)((a.Nk + RB - 1) / RB) * a.Hk * a.B * a.splits)), dim3(256), 0, s, a)
     BY_HEAD(pad_head(a.D), DKV)
 #undef DKV
     if (a.splits > 1) {
-      const int64_t n = (int64_t)a.B * a.Nk * a.Hk * a.D;
-      hipLaunchKernelGGL(sum_splits_kernel, dim3((unsigned)((2 * n / 4 + 255) / 256)), dim3(256), 0, s, a.part, a.dk, a.dv, n, a.splits);
+      const int64_t all = (int64_t)a.B * a.Nk * a.Hk * a.D;
+      hipLaunchKernelGGL(sum_splits_kernel, dim3((unsigned)((2 * all / 4 + 255) / 256)), dim3(256), 0, s, a.part, a.dk, a.dv, all, a.splits);
     }
   }
   return lbmk_check_launch("ranged_attn_bwd");

@@ -13,8 +13,6 @@ namespace {
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((ext_vector_type(8))) short s16x8;
 
-constexpr unsigned TILE_OOB = 0x80000000u;     // a byte offset that every descriptor refuses: the chunk reads as zeros
-
 template <int DH>
 struct Tile {
   static constexpr int CPR = DH / 8;           // 16-byte chunks per row
@@ -22,30 +20,41 @@ struct Tile {
   static constexpr int KS = DH / 16;           // 16-deep MFMA steps over the channels
   static constexpr int DT = DH / 32;           // 32-channel tiles
 
+  // Distinct read offsets a lane keeps: at widths that are no multiple of 64 the swizzle stays within 64-byte groups, so the
+  // offset of a later step is an earlier one's plus an immediate
+  static constexpr int RK = DH % 64 == 0 ? KS : 2, CD = DH % 64 == 0 ? DT : 1;
+  static __device__ __forceinline__ int row_at(const int (&r)[RK], int ks) { return RK == KS ? r[ks] : r[ks & 1] + 64 * (ks >> 1); }
+  static __device__ __forceinline__ int col_at(const int (&c)[CD], int dt) { return CD == DT ? c[dt] : c[0] + 64 * dt; }
+
   // 256 bytes of banks hold 256 / ROW rows: the swizzle supplies the bits that the row offset does not
   static __device__ __forceinline__ int swz(int row) {
     if constexpr (DH % 128 == 0) return ((row & 3) << 2) | ((row >> 2) & 3);
     else if constexpr (DH % 64 == 0) return ((row & 2) << 1) | ((row >> 2) & 3);
     else return (row >> 2) & 3;
   }
-  // byte offsets of this thread's chunks within a tile of the source (D real channels, row stride ld)
-  template <int NI>
-  static __device__ __forceinline__ void offsets(int t, int threads, int ld, int D, unsigned (&off)[NI]) {
+  // where this thread's chunks lie in a tile of R rows: row | byte column << 16.  Row and column rather than byte offsets: one
+  // set serves operands of any row stride.  Channels from D on: row R, which is past the end of every tile
+  template <int NI, int R>
+  static __device__ __forceinline__ void places(int t, int threads, int D, unsigned (&place)[NI]) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int idx = i * threads + t, row = idx / CPR, c = (idx % CPR) ^ swz(row);
-      off[i] = c * 8 < D ? (unsigned)row * (unsigned)ld * 2u + (unsigned)c * 16u : TILE_OOB;
+      place[i] = c * 8 < D ? (unsigned)row | (unsigned)c << 20 : (unsigned)R;
     }
   }
   // stages rows [row0, min(row0 + R, end)) of src; rows from `end` on read as zeros.  `wave` is wave-uniform
   template <int NI, int R>
-  static __device__ __forceinline__ void stage(const bf16_t* src, int64_t row0, int end, int ld, int D, const unsigned (&off)[NI],
+  static __device__ __forceinline__ void stage(const bf16_t* src, int64_t row0, int end, int ld, int D, const unsigned (&place)[NI],
                                                int wave, int waves, char* dst) {
     const int rows = min(R, end - (int)row0);
     const int bytes = ((rows - 1) * ld + D) * 2;
     const bf16_t* base = src + row0 * ld;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) buffer_lds16(base, bytes, off[i], 0, dst + (i * waves + wave) * 1024);
+    for (int i = 0; i < NI; ++i) {
+      // (one 24-bit multiply-add: rows of at most 2^23 bytes, below 2^31 in all; a chunk past the last row, or of row R, is past `bytes`)
+      const unsigned off = __umul24(place[i] & 0xffffu, (unsigned)ld * 2u) + (place[i] >> 16);
+      buffer_lds16(base, bytes, off, 0, dst + (i * waves + wave) * 1024);
+    }
   }
   // operand with the channel along k: row `row`, channels 16 ks + 8 h .. + 7
   static __device__ __forceinline__ int row_off(int row, int ks, int h) { return row * ROW + (((2 * ks + h) ^ swz(row)) << 4); }

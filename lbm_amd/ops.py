@@ -1609,7 +1609,7 @@ def _attn_rows(name, t, heads, head_dim, B, dtype=bf16):
     _want(t.dtype == dtype, f"{name}: {t.dtype} (the kernels over key ranges take bf16)")
     _want(t.dim() == 3 and (B is None or t.shape[0] == B), f"{name}: [{'B' if B is None else B}, N, {heads * head_dim}] expected, got {tuple(t.shape)}")
     t = _token_rows(name, t, heads, head_dim)
-    _want(_ld(t) <= 1 << 23, f"{name}: row stride {_ld(t)}")
+    _want(_ld(t) <= 1 << 22, f"{name}: row stride {_ld(t)}")
     return t
 
 
@@ -1668,7 +1668,7 @@ def ranged_attn_bwd(q, k, v, o, do, lse, heads: int, kv_heads: int, head_dim: in
     _same_device(q, o, do, lse, rest)
     new = torch.empty if d.Nq and d.B else torch.zeros      # without queries the keys' gradients are zeros that no kernel writes
     dq, dk, dv = (new(t.shape, dtype=bf16, device=q.device) for t in (q, k, v))
-    scratch = torch.empty(lib.lbmk_ranged_attn_bwd_scratch_floats(d.B, heads, kv_heads, d.Nq, d.Nk, head_dim), dtype=torch.float32, device=q.device)
+    scratch = torch.empty(lib.lbmk_ranged_attn_bwd_scratch_floats(d.B, heads, kv_heads, d.Nq, d.Nk, head_dim, 0 if ranges is None else 1), dtype=torch.float32, device=q.device)
     d.o, d.rest, d.dout, d.lse, d.scratch = o.data_ptr(), _ptr(rest), do.data_ptr(), lse.data_ptr(), scratch.data_ptr()
     d.dq, d.dk, d.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
     d.ldo, d.ldg, d.so, d.sg = _ld(o), _ld(do), _sb(o), _sb(do)
