@@ -3,7 +3,7 @@
 //   y[m] = x[m] W^T + bias + t[m] B_a^T          t[m] = s_a x[m] A_a^T          a = index[request of row m]
 //
 // The factor products are a few per cent of the shared one, so what costs is reading x again and every launch.  Two steps:
-//   * adapter_down: t, bf16 (its half step is relative to the adapter's own share of y).  16 rows x 16 ranks per wave on
+//   * adapter_down: t, bf16 (its half step is relative to the adapter's own share of y).  16 rows x 32 ranks per workgroup on
 //     v_mfma_f32_16x16x32_bf16, both operands K-contiguous and read straight into registers; the four waves of a workgroup
 //     split K and are joined in LDS in a fixed order, because there are too few row groups to fill the chip otherwise.
 //   * the shared product with t B_a^T added to its accumulators before the one rounding of y: many rows in lbmk_igemm
@@ -18,44 +18,54 @@ __device__ __forceinline__ bf16x8 zero8() {
   return __builtin_bit_cast(bf16x8, z);
 }
 
-constexpr int DOWN_WAVES = 4;
+constexpr int DOWN_WAVES = 4, DOWN_GROUPS = 2;      // waves over K; groups of 16 ranks that share one reading of x
 
-// grid: (ceil(rank / 16), ceil(rows / 16) * requests)
+// grid: (columns of t / 32, ceil(rows / 16) * requests)
 __global__ __launch_bounds__(64 * DOWN_WAVES) void adapter_down_kernel(const bf16_t* __restrict__ x, const bf16_t* __restrict__ down,
                                                                       const int32_t* __restrict__ index, const float* __restrict__ scaling,
                                                                       bf16_t* __restrict__ t, int rows, int K, int64_t ldx, int rank, int tk,
                                                                       int count) {
-  __shared__ f32x4 part[DOWN_WAVES][64];
+  __shared__ f32x4 part[DOWN_WAVES][DOWN_GROUPS][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 15, lq = lane >> 4;
-  const int groups = (rows + 15) / 16, request = blockIdx.y / groups, m0 = (blockIdx.y - request * groups) * 16, r0 = blockIdx.x * 16;
+  const int groups = (rows + 15) / 16, request = blockIdx.y / groups, m0 = (blockIdx.y - request * groups) * 16, r0 = blockIdx.x * 32;
   const int a = index[request];
   if ((unsigned)a >= (unsigned)count) return;                  // no adapter: nobody reads these rows of t
-  const int m = min(m0 + lr, rows - 1), n = min(r0 + lr, rank - 1);
+  const int m = min(m0 + lr, rows - 1);
   const bf16_t* xr = x + ((int64_t)request * rows + m) * ldx + 8 * lq;
-  const bf16_t* dr = down + ((int64_t)a * rank + n) * K + 8 * lq;
+  const bf16_t* dr[DOWN_GROUPS];
+#pragma unroll
+  for (int g = 0; g < DOWN_GROUPS; ++g) dr[g] = down + ((int64_t)a * rank + min(r0 + 16 * g + lr, rank - 1)) * K + 8 * lq;
   // K in chunks of 32: an equal, contiguous share per wave
   const int chunks = (K + 31) / 32, per = (chunks + DOWN_WAVES - 1) / DOWN_WAVES;
   const int c0 = wave * per, c1 = min(c0 + per, chunks);
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  f32x4 acc[DOWN_GROUPS];
+#pragma unroll
+  for (int g = 0; g < DOWN_GROUPS; ++g) acc[g] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 5
   for (int c = c0; c < c1; ++c) {
     const bool in = 32 * c + 8 * lq < K;                       // K % 8 == 0
-    const bf16x8 fd = in ? *(const bf16x8*)(dr + 32 * c) : zero8(), fx = in ? *(const bf16x8*)(xr + 32 * c) : zero8();
-    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fd, fx, acc, 0, 0, 0);
-  }
-  part[wave][lane] = acc;
-  __syncthreads();
-  if (wave != 0) return;
+    const bf16x8 fx = in ? *(const bf16x8*)(xr + 32 * c) : zero8();
 #pragma unroll
-  for (int w = 1; w < DOWN_WAVES; ++w) acc += part[w][lane];
-  if (m0 + lr >= rows) return;
+    for (int g = 0; g < DOWN_GROUPS; ++g) {
+      const bf16x8 fd = in ? *(const bf16x8*)(dr[g] + 32 * c) : zero8();
+      acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fd, fx, acc[g], 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < DOWN_GROUPS; ++g) part[wave][g][lane] = acc[g];
+  __syncthreads();
+  if (wave >= DOWN_GROUPS || m0 + lr >= rows) return;
+  // wave g joins group g.  Lane: row m0 + lr, ranks 4 lq .. + 3 of the group; ranks from `rank` on are zeros
+  f32x4 v = part[0][wave][lane];
+#pragma unroll
+  for (int w = 1; w < DOWN_WAVES; ++w) v += part[w][wave][lane];
   const float s = scaling ? scaling[a] : 1.f;
-  // lane: row m0 + lr, ranks r0 + 4 lq .. + 3; ranks from `rank` on are zeros
+  const int n = r0 + 16 * wave + 4 * lq;
   u16x4 o;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) o.v[e] = f2bf(r0 + 4 * lq + e < rank ? acc[e] * s : 0.f);
-  *(u16x4*)(t + ((int64_t)request * rows + m0 + lr) * tk + r0 + 4 * lq) = o;
+  for (int e = 0; e < 4; ++e) o.v[e] = f2bf(n + e < rank ? v[e] * s : 0.f);
+  *(u16x4*)(t + ((int64_t)request * rows + m0 + lr) * tk + n) = o;
 }
 
 constexpr int FEW_WAVES = 8, FEW_ROWS = 64;
@@ -149,7 +159,7 @@ extern "C" int lbmk_adapter_down(const void* x, const void* down, const int32_t*
   LBMK_REQUIRE(most > 0, "adapter_down: %d rows per request (at most %d)", rows, 65535 * 16);
   for (int r = 0; r < requests; r += most) {
     const int n = requests - r < most ? requests - r : most;
-    hipLaunchKernelGGL(adapter_down_kernel, dim3(tk / 16, n * per), dim3(64 * DOWN_WAVES), 0, (hipStream_t)stream,
+    hipLaunchKernelGGL(adapter_down_kernel, dim3(tk / 32, n * per), dim3(64 * DOWN_WAVES), 0, (hipStream_t)stream,
                        (const bf16_t*)x + (int64_t)r * rows * ldx, (const bf16_t*)down, index + r, scaling, (bf16_t*)t + (int64_t)r * rows * tk, rows, K,
                        ldx, rank, tk, count);
   }

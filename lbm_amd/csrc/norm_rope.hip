@@ -17,7 +17,7 @@
 namespace {
 
 constexpr int NR_THREADS = 256;
-constexpr int NR_BATCH = 4, NR_BATCH_BWD = 2;        // heads in flight per lane group
+constexpr int NR_HEADS = 4;        // heads per lane group and token where there are many tokens
 
 struct NormRope {
   const void *x[2], *w[2], *dy[2];
@@ -52,7 +52,7 @@ struct Chunk {
     }
   }
   __device__ __forceinline__ void get(float (&v)[VEC]) {
-    // opaque to the compiler: it would unpack at the load, and hold every head in flight at twice the registers
+    // opaque to the compiler: it would unpack at the load, and carry a head in flight in twice the registers
 #pragma unroll
     for (int i = 0; i < WORDS; ++i) asm volatile("" : "+v"(w[i]));
 #pragma unroll
@@ -169,17 +169,26 @@ __device__ __forceinline__ void nr_rotate(float (&va)[VEC], float (&vb)[VEC], co
   }
 }
 
+// sum over L neighbouring lanes, on the vector ALU's lane permutes: quad swaps, then mirrors inside 8 and 16 lanes (by then all
+// lanes of a quad, or half, hold the same sum); an LDS permute per step would be the longest part of a head's chain
+template <int CTRL>
+__device__ __forceinline__ float nr_dpp(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
 template <int L>
 __device__ __forceinline__ float nr_sum(float v) {
-#pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  if constexpr (L >= 2) v = nr_dpp<0xb1>(v);      // quad_perm [1, 0, 3, 2]
+  if constexpr (L >= 4) v = nr_dpp<0x4e>(v);      // quad_perm [2, 3, 0, 1]
+  if constexpr (L >= 8) v = nr_dpp<0x141>(v);     // row_half_mirror
+  if constexpr (L >= 16) v = nr_dpp<0x140>(v);    // row_mirror
+  if constexpr (L >= 32) v += __shfl_xor(v, 16, 64);
   return v;
 }
 
 // blockIdx.y: 0 the queries, 1 the keys
 template <typename T, int VEC, bool INTER, int L, bool BWD>
 __global__ __launch_bounds__(NR_THREADS) void norm_rope_kernel(NormRope d) {
-  constexpr int GROUPS = NR_THREADS / L, NB = BWD ? NR_BATCH_BWD : NR_BATCH;
+  constexpr int GROUPS = NR_THREADS / L;
   const int t = threadIdx.x, u = t % L, group = t / L, z = blockIdx.y;
   const int tpb = GROUPS / d.gpt;                       // tokens per block and step
   const int sub = group % d.gpt;                        // this group's first head
@@ -227,33 +236,32 @@ __global__ __launch_bounds__(NR_THREADS) void norm_rope_kernel(NormRope d) {
     const T* xr = (const T*)d.x[z] + bb * d.sx[z] + nn * d.ldx[z];
     const T* gr = BWD ? (const T*)d.dy[z] + bb * d.sdy[z] + nn * d.lddy[z] : nullptr;
     T* yr = (T*)d.y[z] + bb * d.sy[z] + nn * d.ldy[z];
-    Chunk<T, VEC> xa[NB], xb[NB], ga[BWD ? NB : 1], gb[BWD ? NB : 1];
-    auto load = [&](int h0) __attribute__((always_inline)) {
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const int h = h0 + i * d.gpt;
-        const int hc = h < H ? h : min(sub, H - 1);     // a row in bounds, not used
-        xa[i].load(xr + hc * d.D + pa);
-        xb[i].load(xr + hc * d.D + pb);
-        if constexpr (BWD) {
-          ga[i].load(gr + hc * d.D + pa);
-          gb[i].load(gr + hc * d.D + pb);
-        }
-      }
+    struct Head {
+      Chunk<T, VEC> xa, xb, ga, gb;
     };
+    auto load = [&](int h) __attribute__((always_inline)) {
+      Head r;
+      r.xa.load(xr + h * d.D + pa);
+      r.xb.load(xr + h * d.D + pb);
+      if constexpr (BWD) {
+        r.ga.load(gr + h * d.D + pa);
+        r.gb.load(gr + h * d.D + pb);
+      }
+      return r;
+    };
+    if (sub >= H) continue;                             // more groups than heads
+    Head next = load(sub);                              // in flight while the angles are fetched
     float c[VEC], s[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) c[e] = s[e] = 0.f;
-    for (int h0 = sub; h0 < H; h0 += NB * d.gpt) {
-      load(h0);
-      if (h0 == sub) nr_angles<VEC, INTER>(d, tk, ca, cb, ta, tb, c, s);      // under the first loads
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const int h = h0 + i * d.gpt;
-        const bool put = live && h < H;
+    nr_angles<VEC, INTER>(d, tk, ca, cb, ta, tb, c, s);
+#pragma unroll 1
+    for (int h = sub; h < H; h += d.gpt) {
+        Head now = next;
+        if (h + d.gpt < H) next = load(h + d.gpt);      // in flight under this head's arithmetic
         float va[VEC], vb[VEC], qa = 0.f, qb = 0.f;
-        xa[i].get(va);
-        xb[i].get(vb);
+        now.xa.get(va);
+        now.xb.get(vb);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           qa = fmaf(va[e], va[e], qa);
@@ -271,14 +279,14 @@ __global__ __launch_bounds__(NR_THREADS) void norm_rope_kernel(NormRope d) {
           nr_rotate<VEC, INTER>(va, vb, c, s, ta, tb, 1.f);
         } else {
           float ua[VEC], ub[VEC], da = 0.f, db = 0.f;
-          ga[i].get(ua);
-          gb[i].get(ub);
+          now.ga.get(ua);
+          now.gb.get(ub);
           nr_rotate<VEC, INTER>(ua, ub, c, s, ta, tb, -1.f);
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
             va[e] *= rstd;
             vb[e] *= rstd;
-            if (put) {
+            if (live) {
               dwa[e] = fmaf(ua[e], va[e], dwa[e]);
               dwb[e] = fmaf(ub[e], vb[e], dwb[e]);
             }
@@ -294,9 +302,8 @@ __global__ __launch_bounds__(NR_THREADS) void norm_rope_kernel(NormRope d) {
             vb[e] = rstd * (ub[e] - vb[e] * m);
           }
         }
-        if (put && ca >= 0) nr_store<T, VEC>(yr + h * d.D + ca, va);
-        if (put && cb >= 0) nr_store<T, VEC>(yr + h * d.D + cb, vb);
-      }
+        if (live && ca >= 0) nr_store<T, VEC>(yr + h * d.D + ca, va);
+        if (live && cb >= 0) nr_store<T, VEC>(yr + h * d.D + cb, vb);
     }
   }
 
@@ -386,7 +393,7 @@ int nr_run(NormRope& d, int f32, int interleaved, bool bwd, hipStream_t s) {
   // lane groups per token: with many tokens four or five heads per group, so that the token's angles are read once for
   // several heads; with few tokens as many groups as there are heads
   const int heads = d.H[0] > d.H[1] ? d.H[0] : d.H[1];
-  const int per = (int64_t)d.tokens * heads >= 65536 ? NR_BATCH : 1;
+  const int per = (int64_t)d.tokens * heads >= 65536 ? NR_HEADS : 1;
   int gpt = 1;
   while (gpt < groups && gpt * per < heads) gpt <<= 1;
   d.gpt = gpt;

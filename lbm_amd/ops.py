@@ -1414,109 +1414,154 @@ def lpips_head_bwd(f0, f1, w, keep, gout: torch.Tensor) -> torch.Tensor:
 
 
 # --------------------------------------------------------------------------------------
-# token operators: head norms with the position rotation
+# token operators: what they share
 # --------------------------------------------------------------------------------------
-def _want(cond, msg: str):
-    if not cond:
-        raise ValueError(msg)
+# (These run once per token of a served request: messages are formatted only when they are raised, a tensor's shape and strides
+# are read once, and descriptors are filled in one call.)
+def _one_device(t: torch.Tensor, *others) -> int:
+    """index of the device that all operands are on (-1: the CPU)"""
+    d = t.get_device()
+    for o in others:
+        if o is not None and o.get_device() != d:
+            raise ValueError(f"operands on {t.device} and {o.device}")
+    return d
 
 
-def _same_device(first: torch.Tensor, *ts):
-    for t in ts:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"operands on {first.device} and {t.device}")
+def _launch(device: int, what: str, fn, *args):
+    """``fn(*args, stream)`` with ``device`` current and on its current stream"""
+    if device < 0:
+        raise RuntimeError("lbm_amd kernels run on the GPU only (got a CPU tensor); there is no CPU fallback")
+    # (the raw stream handle: a Stream object around it costs 3 us, a fifth of a single-token call)
+    if device == torch.cuda.current_device():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if status:
+        check(status, what)
 
 
-def _on(t: torch.Tensor):
-    """the context in which ``t``'s device is the current one (launches and streams follow the current device)"""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-
-def _token_rows(name: str, t: torch.Tensor, heads: Optional[int], head_dim: int) -> torch.Tensor:
-    """``t`` as [B, N, heads * head_dim] with unit channel stride and rows on 16 bytes; column windows of wider rows pass"""
-    _want(t.dim() in (2, 3), f"{name}: [B, N, C] or [N, C] expected, got {tuple(t.shape)}")
-    t = t if t.dim() == 3 else t[None]
-    c = t.shape[2]
-    _want(c % head_dim == 0 and c > 0 and (heads is None or c == heads * head_dim),
-          f"{name}: {c} channels are not {'' if heads is None else heads} heads of {head_dim}")
-    unit = 16 // t.element_size()
-    ok = (t.stride(2) == 1 and t.data_ptr() % 16 == 0 and (t.shape[1] <= 1 or (t.stride(1) % unit == 0 and c <= t.stride(1) < 1 << 31))
-          and (t.shape[0] <= 1 or (t.stride(0) % unit == 0 and t.stride(0) >= 0)))
-    _want(ok or t.numel() == 0, f"{name}: strides {t.stride()} at address {t.data_ptr():#x}: channels must be adjacent and every "
-                                "token's row must start on 16 bytes")
-    return t
+def _token_rows(name: str, t: torch.Tensor, heads: Optional[int], head_dim: int, batched: bool = False):
+    """(pointer, B, N, channels, token stride, batch stride) of [B, N, heads * head_dim] (or [N, ...]) with adjacent channels and
+    rows on 16 bytes; column windows of wider rows pass"""
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 3:
+        B, N, c = shape
+        sb, ld, unit = stride
+    elif len(shape) == 2 and not batched:
+        B, (N, c), sb, (ld, unit) = 1, shape, 0, stride
+    else:
+        raise ValueError(f"{name}: [B, N, C]{'' if batched else ' or [N, C]'} expected, got {tuple(shape)}")
+    if c % head_dim or c == 0 or (heads is not None and c != heads * head_dim):
+        raise ValueError(f"{name}: {c} channels are not {'' if heads is None else heads} heads of {head_dim}")
+    if N <= 1:
+        ld = c
+    if B <= 1:
+        sb = 0
+    p = t.data_ptr()
+    part = 16 // t.element_size() - 1
+    if (unit != 1 or p & 15 or ld & part or sb & part or ld < c or ld >> 31 or sb < 0) and B * N:
+        raise ValueError(f"{name}: strides {stride} at address {p:#x}: channels must be adjacent and every token's row must start on 16 bytes")
+    return p, B, N, c, ld, sb
 
 
 def token_rows_ready(t: torch.Tensor) -> torch.Tensor:
     """``t``, or a contiguous copy where the kernels cannot read it in place (an output gradient that autograd expanded
     from a scalar or cut out of another tensor)"""
-    unit = 16 // t.element_size()
-    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % unit == 0 for s in t.stride()[:-1]) and \
-        (t.dim() < 2 or t.shape[-2] <= 1 or t.stride(-2) >= t.shape[-1])
-    return t if ok else t.contiguous()
+    if t.is_contiguous() and t.data_ptr() & 15 == 0:
+        return t
+    part = 16 // t.element_size() - 1
+    *lead, unit = t.stride()
+    if unit == 1 and t.data_ptr() & 15 == 0 and not any(s & part for s in lead) and (not lead or t.shape[-2] <= 1 or lead[-1] >= t.shape[-1]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
-def _ld(t: torch.Tensor) -> int:
-    return t.stride(1) if t.shape[1] > 1 else t.shape[2]
-
-
-def _sb(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else 0
-
-
+# --------------------------------------------------------------------------------------
+# token operators: head norms with the position rotation
+# --------------------------------------------------------------------------------------
 def rope_table(positions: int, pairs: int, theta: float = 10000.0, device=None) -> torch.Tensor:
     """cosine and sine of position * theta^(-j / pairs): f32 [positions, pairs, 2], computed in 64 bits (an angle of a
     far position has no digits left for its fraction of a turn in f32)"""
-    _want(positions > 0 and pairs > 0 and theta > 0, f"rope_table: {positions} positions, {pairs} pairs, theta {theta}")
+    if positions < 1 or pairs < 1 or not theta > 0:
+        raise ValueError(f"rope_table: {positions} positions, {pairs} pairs, theta {theta}")
     ang = torch.arange(positions, dtype=torch.float64)[:, None] * theta ** (-torch.arange(pairs, dtype=torch.float64) / pairs)
     return torch.stack((ang.cos(), ang.sin()), -1).to(torch.float32).to(device if device is not None else "cuda").contiguous()
 
 
-def _norm_rope_desc(q, k, head_dim, q_weight, k_weight, table, positions, eps, interleaved):
-    _same_device(q, k, q_weight, k_weight, table, positions)
-    _want(q.dtype in (bf16, torch.float32) and k.dtype == q.dtype, f"qk_norm_rope: q {q.dtype}, k {k.dtype} (both bf16 or both f32)")
-    q3, k3 = _token_rows("q", q, None, head_dim), _token_rows("k", k, None, head_dim)
-    _want(q3.shape[:2] == k3.shape[:2] and q.dim() == k.dim(), f"qk_norm_rope: q {tuple(q.shape)}, k {tuple(k.shape)}")
-    B, N = q3.shape[:2]
-    d = NormRopeDesc()
+def _norm_rope(q, k, head_dim, q_weight, k_weight, table, positions, eps, interleaved, out, grads):
+    """checks the operands and launches the forward kernel, or with ``grads`` (of the outputs) the backward ones;
+    (first output, second output, scratch and gains' gradients)"""
+    dt = q.dtype
+    if dt not in (bf16, torch.float32) or k.dtype != dt:
+        raise ValueError(f"qk_norm_rope: q {dt}, k {k.dtype} (both bf16 or both f32)")
+    if head_dim % 8 or not 8 <= head_dim <= 256:
+        raise ValueError(f"qk_norm_rope: head_dim {head_dim} (8 ... 256, a multiple of 8)")
+    qp, B, N, qc, ldq, sq = _token_rows("q", q, None, head_dim)
+    kp, Bk, Nk, kc, ldk, sk = _token_rows("k", k, None, head_dim)
+    if Bk != B or Nk != N or q.dim() != k.dim():
+        raise ValueError(f"qk_norm_rope: q {tuple(q.shape)}, k {tuple(k.shape)}")
+    wdt = None
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        _want(w is None or (w.shape == (head_dim,) and w.is_contiguous() and w.dtype in (bf16, torch.float32)),
-              f"{name}: a bf16 or f32 vector of {head_dim}")
-    _want(q_weight is None or k_weight is None or q_weight.dtype == k_weight.dtype, "qk_norm_rope: the two weights have one dtype")
-    w = q_weight if q_weight is not None else k_weight
-    d.wq, d.wk, d.w_f32 = _ptr(q_weight), _ptr(k_weight), 1 if w is not None and w.dtype == torch.float32 else 0
-    _want((table is None) == (positions is None), "qk_norm_rope: table and positions go together")
+        if w is None:
+            continue
+        if w.shape != (head_dim,) or not w.is_contiguous() or w.dtype not in (bf16, torch.float32):
+            raise ValueError(f"{name}: a bf16 or f32 vector of {head_dim}")
+        if wdt is not None and wdt != w.dtype:
+            raise ValueError("qk_norm_rope: the two weights have one dtype")
+        wdt = w.dtype
+    if (table is None) != (positions is None):
+        raise ValueError("qk_norm_rope: table and positions go together")
+    rot = axes = rows = 0
     if table is not None:
-        _want(table.dtype == torch.float32 and table.dim() == 3 and table.shape[2] == 2 and table.is_contiguous() and table.numel() > 0,
-              "table: contiguous f32 [positions, pairs, 2] (rope_table)")
-        _want(positions.dtype == torch.int32 and positions.is_contiguous(), "positions: contiguous int32")
-        lead = tuple(q.shape[:-1])
-        axes = 1 if tuple(positions.shape) == lead else positions.shape[-1] if tuple(positions.shape[:-1]) == lead else 0
-        _want(axes >= 1, f"positions {tuple(positions.shape)}: {lead} or {lead} x axes")
-        d.table, d.pos, d.axes, d.positions = table.data_ptr(), positions.data_ptr(), axes, table.shape[0]
-        d.rot = 2 * axes * table.shape[1]
-        _want(d.rot <= head_dim and d.rot % 8 == 0,
-              f"qk_norm_rope: {axes} axes of {table.shape[1]} pairs rotate {d.rot} of {head_dim} channels (a multiple of 8)")
-    _want(head_dim % 8 == 0 and 8 <= head_dim <= 256, f"qk_norm_rope: head_dim {head_dim} (8 ... 256, a multiple of 8)")
-    _want(eps >= 0, f"qk_norm_rope: eps {eps}")
-    _need_gpu(q)
-    d.q, d.k = q3.data_ptr(), k3.data_ptr()
-    d.B, d.N, d.Hq, d.Hk, d.D = B, N, q3.shape[2] // head_dim, k3.shape[2] // head_dim, head_dim
-    d.ldq, d.ldk, d.sq, d.sk = _ld(q3), _ld(k3), _sb(q3), _sb(k3)
-    d.f32, d.interleaved, d.eps = 1 if q.dtype == torch.float32 else 0, 1 if interleaved else 0, eps
-    return d
-
-
-def _norm_rope_out(d, q, k, out, head_dim):
-    """fills in the outputs: ``out`` or new contiguous tensors"""
-    qo, ko = out if out is not None else (torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device))
-    _same_device(q, qo, ko)
-    _want(qo.dtype == q.dtype and ko.dtype == q.dtype and qo.shape == q.shape and ko.shape == k.shape, "out: shapes and dtype of q and k")
-    q3, k3 = _token_rows("out[0]", qo, None, head_dim), _token_rows("out[1]", ko, None, head_dim)
-    _want((q3.shape[0] <= 1 or q3.stride(0) > 0) and (k3.shape[0] <= 1 or k3.stride(0) > 0), "out: a broadcast batch cannot be written")
-    d.q_out, d.k_out = q3.data_ptr(), k3.data_ptr()
-    d.ldqo, d.ldko, d.sqo, d.sko = _ld(q3), _ld(k3), _sb(q3), _sb(k3)
-    return qo, ko
+        if table.dtype != torch.float32 or table.dim() != 3 or table.shape[2] != 2 or not table.is_contiguous() or table.numel() == 0:
+            raise ValueError("table: contiguous f32 [positions, pairs, 2] (rope_table)")
+        if positions.dtype != torch.int32 or not positions.is_contiguous():
+            raise ValueError("positions: contiguous int32")
+        lead, at = q.shape[:-1], positions.shape
+        axes = 1 if at == lead else at[-1] if at[:-1] == lead else 0
+        if axes < 1:
+            raise ValueError(f"positions {tuple(at)}: {tuple(lead)} or {tuple(lead)} x axes")
+        rows, rot = table.shape[0], 2 * axes * table.shape[1]
+        if rot > head_dim or rot % 8:
+            raise ValueError(f"qk_norm_rope: {axes} axes of {table.shape[1]} pairs rotate {rot} of {head_dim} channels (a multiple of 8)")
+    if not eps >= 0:
+        raise ValueError(f"qk_norm_rope: eps {eps}")
+    device = _one_device(q, k, q_weight, k_weight, table, positions)
+    gqp = gkp = None
+    lgq = lgk = sgq = sgk = 0
+    if grads is not None:
+        gq, gk = grads
+        if gq.dtype != dt or gk.dtype != dt or gq.shape != q.shape or gk.shape != k.shape:
+            raise ValueError("qk_norm_rope_bwd: gradients have the shapes and dtype of q and k")
+        gqp, _, _, _, lgq, sgq = _token_rows("dq_out", gq, None, head_dim)
+        gkp, _, _, _, lgk, sgk = _token_rows("dk_out", gk, None, head_dim)
+        _one_device(q, gq, gk)
+    if device < 0:
+        _need_gpu(q)
+    if out is None:
+        qo, ko = torch.empty(q.shape, dtype=dt, device=q.device), torch.empty(k.shape, dtype=dt, device=q.device)
+        qop, kop, ldqo, ldko, sqo, sko = qo.data_ptr(), ko.data_ptr(), qc, kc, N * qc, N * kc
+    else:
+        qo, ko = out
+        if qo.dtype != dt or ko.dtype != dt or qo.shape != q.shape or ko.shape != k.shape:
+            raise ValueError("out: shapes and dtype of q and k")
+        _one_device(q, qo, ko)
+        qop, _, _, _, ldqo, sqo = _token_rows("out[0]", qo, None, head_dim)
+        kop, _, _, _, ldko, sko = _token_rows("out[1]", ko, None, head_dim)
+        if B > 1 and (sqo == 0 or sko == 0):
+            raise ValueError("out: a broadcast batch cannot be written")
+    d = NormRopeDesc(qp, kp, _ptr(q_weight), _ptr(k_weight), gqp, gkp, qop, kop, _ptr(table), _ptr(positions), B, N, qc // head_dim,
+                     kc // head_dim, head_dim, rot, axes, rows, ldq, ldk, ldqo, ldko, lgq, lgk, sq, sk, sqo, sko, sgq, sgk,
+                     1 if dt == torch.float32 else 0, 1 if wdt == torch.float32 else 0, 1 if interleaved else 0, eps)
+    if grads is None:
+        _launch(device, "lbmk_norm_rope", lib.lbmk_norm_rope, C.byref(d))
+        return qo, ko
+    scratch = torch.empty(lib.lbmk_norm_rope_bwd_scratch_floats(head_dim), dtype=torch.float32, device=q.device)
+    dwq = None if q_weight is None else torch.empty_like(q_weight)
+    dwk = None if k_weight is None else torch.empty_like(k_weight)
+    _launch(device, "lbmk_norm_rope_bwd", lib.lbmk_norm_rope_bwd, C.byref(d), scratch.data_ptr(), _ptr(dwq), _ptr(dwk))
+    return qo, ko, dwq, dwk
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, head_dim: int, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
@@ -1530,11 +1575,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, head_dim: int, q_weight: Opti
     takes axis j // F and column j % F, and is channels (j, j + axes * F), or (2j, 2j + 1) when ``interleaved``.  A
     position outside the table gives NaN.  No table: the norm alone.  ``out``: (q', k') destinations, also q and k
     themselves.  Not differentiable: models.layers.qk_norm_rope is."""
-    d = _norm_rope_desc(q, k, head_dim, q_weight, k_weight, table, positions, eps, interleaved)
-    qo, ko = _norm_rope_out(d, q, k, out, head_dim)
-    with _on(q):
-        check(lib.lbmk_norm_rope(C.byref(d), _stream()), "lbmk_norm_rope")
-    return qo, ko
+    return _norm_rope(q, k, head_dim, q_weight, k_weight, table, positions, eps, interleaved, out, None)
 
 
 def qk_norm_rope_bwd(q, k, dq_out, dk_out, head_dim: int, q_weight, k_weight, table=None, positions=None, *, eps: float = 1e-6,
@@ -1542,19 +1583,7 @@ def qk_norm_rope_bwd(q, k, dq_out, dk_out, head_dim: int, q_weight, k_weight, ta
     """Gradients of ``qk_norm_rope`` for its inputs q, k and the gradients of its outputs -> (dq, dk, dq_weight, dk_weight);
     the weights' gradients (None for a weight that is None) have the weights' dtype and are summed in a fixed order.
     ``out``: (dq, dk) destinations."""
-    d = _norm_rope_desc(q, k, head_dim, q_weight, k_weight, table, positions, eps, interleaved)
-    _same_device(q, dq_out, dk_out)
-    _want(dq_out.dtype == q.dtype and dk_out.dtype == q.dtype and dq_out.shape == q.shape and dk_out.shape == k.shape,
-          "qk_norm_rope_bwd: gradients have the shapes and dtype of q and k")
-    g3, h3 = _token_rows("dq_out", dq_out, None, head_dim), _token_rows("dk_out", dk_out, None, head_dim)
-    d.dq_out, d.dk_out = g3.data_ptr(), h3.data_ptr()
-    d.lddq, d.lddk, d.sdq, d.sdk = _ld(g3), _ld(h3), _sb(g3), _sb(h3)
-    dq, dk = _norm_rope_out(d, q, k, out, head_dim)
-    scratch = torch.empty(lib.lbmk_norm_rope_bwd_scratch_floats(head_dim), dtype=torch.float32, device=q.device)
-    dwq, dwk = (None if w is None else torch.empty_like(w) for w in (q_weight, k_weight))
-    with _on(q):
-        check(lib.lbmk_norm_rope_bwd(C.byref(d), scratch.data_ptr(), _ptr(dwq), _ptr(dwk), _stream()), "lbmk_norm_rope_bwd")
-    return dq, dk, dwq, dwk
+    return _norm_rope(q, k, head_dim, q_weight, k_weight, table, positions, eps, interleaved, out, (dq_out, dk_out))
 
 
 # --------------------------------------------------------------------------------------
@@ -1571,67 +1600,60 @@ def key_ranges(B: int, Nq: int, Nk: Optional[int] = None, *, causal: bool = Fals
     int32 [B]): the first tokens of each document are seen by all its queries.  lens: int32 [B], keys from there on are
     padding."""
     Nk = Nq if Nk is None else Nk
-    _want(B >= 0 and Nq >= 0 and Nk >= 0 and window >= 0, f"key_ranges: B {B}, Nq {Nq}, Nk {Nk}, window {window}")
-    _want(causal or (window == 0 and prefix is None), "key_ranges: window and prefix go with causal")
-    _want(window == 0 or prefix is None, "key_ranges: a window with a prefix is no interval")
-    given = [t for t in (prefix, documents, lens) if t is not None]
+    if B < 0 or Nq < 0 or Nk < 0 or window < 0:
+        raise ValueError(f"key_ranges: B {B}, Nq {Nq}, Nk {Nk}, window {window}")
+    if not causal and (window or prefix is not None):
+        raise ValueError("key_ranges: window and prefix go with causal")
+    if window and prefix is not None:
+        raise ValueError("key_ranges: a window with a prefix is no interval")
     for name, t in (("prefix", prefix), ("lens", lens)):
-        _want(t is None or (t.dtype == torch.int32 and t.shape == (B,) and t.is_contiguous()), f"{name}: contiguous int32 [{B}]")
-    if documents is not None:
-        _want(documents.dtype == torch.int32 and documents.is_contiguous() and documents.shape[-1] >= 2 and
-              (documents.dim() == 1 or (documents.dim() == 2 and documents.shape[0] == B)),
-              f"documents: contiguous int32 [n + 1] or [{B}, n + 1] token counts")
+        if t is not None and (t.dtype != torch.int32 or t.shape != (B,) or not t.is_contiguous()):
+            raise ValueError(f"{name}: contiguous int32 [{B}]")
+    if documents is not None and (documents.dtype != torch.int32 or not documents.is_contiguous() or documents.dim() not in (1, 2) or
+                                  documents.shape[-1] < 2 or (documents.dim() == 2 and documents.shape[0] != B)):
+        raise ValueError(f"documents: contiguous int32 [n + 1] or [{B}, n + 1] token counts")
+    given = [t for t in (prefix, documents, lens) if t is not None]
     if given:
-        _same_device(given[0], *given[1:])
-        _want(device is None or torch.device(device).type == given[0].device.type, f"key_ranges: operands on {given[0].device}, device {device}")
+        _one_device(*given)
+        if device is not None and torch.device(device).type != given[0].device.type:
+            raise ValueError(f"key_ranges: operands on {given[0].device}, device {device}")
     dev = given[0].device if given else torch.device(device if device is not None else "cuda")
     if dev.type != "cuda":
         raise RuntimeError("lbm_amd kernels run on the GPU only; there is no CPU fallback")
     out = torch.empty(B, Nq, 2, dtype=torch.int32, device=dev)
     docs = documents.shape[-1] - 1 if documents is not None else 0
-    with _on(out):
-        check(lib.lbmk_key_ranges(out.data_ptr(), _ptr(documents), docs, docs + 1 if documents is not None and documents.dim() == 2 else 0,
-                                  _ptr(prefix), _ptr(lens), B, Nq, Nk, 1 if causal else 0, window, _stream()), "lbmk_key_ranges")
+    _launch(out.get_device(), "lbmk_key_ranges", lib.lbmk_key_ranges, out.data_ptr(), _ptr(documents), docs,
+            docs + 1 if documents is not None and documents.dim() == 2 else 0, _ptr(prefix), _ptr(lens), B, Nq, Nk, 1 if causal else 0, window)
     return out
 
 
-def _score_args(name, d, head_dim, scale, cap, slopes, heads, like):
-    scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
-    _want(0 < scale < math.inf, f"{name}: scale {scale} (positive)")
-    _want(0 <= cap < math.inf, f"{name}: cap {cap} (0: none)")
-    if slopes is not None:
-        _want(slopes.dtype == torch.float32 and slopes.shape == (heads,) and slopes.is_contiguous(), f"slopes: contiguous f32 [{heads}]")
-        _same_device(like, slopes)
-    d.scale, d.cap, d.slopes = scale, float(cap), _ptr(slopes)
+def _attn_rows(name: str, t: torch.Tensor, heads: int, head_dim: int):
+    if t.dtype != bf16:
+        raise ValueError(f"{name}: {t.dtype} (the kernels over key ranges take bf16)")
+    r = _token_rows(name, t, heads, head_dim, True)
+    if r[4] > 1 << 22:
+        raise ValueError(f"{name}: row stride {r[4]}")
+    return r
 
 
-def _attn_rows(name, t, heads, head_dim, B, dtype=bf16):
-    _want(t.dtype == dtype, f"{name}: {t.dtype} (the kernels over key ranges take bf16)")
-    _want(t.dim() == 3 and (B is None or t.shape[0] == B), f"{name}: [{'B' if B is None else B}, N, {heads * head_dim}] expected, got {tuple(t.shape)}")
-    t = _token_rows(name, t, heads, head_dim)
-    _want(_ld(t) <= 1 << 22, f"{name}: row stride {_ld(t)}")
-    return t
+def _attn_args(what, heads, kv_heads, head_dim, scale, cap, slopes):
+    if head_dim % 8 or not 8 <= head_dim <= 160:
+        raise ValueError(f"{what}: head_dim {head_dim} (8 ... 160, a multiple of 8)")
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError(f"{what}: {heads} heads over {kv_heads} key heads")
+    scale = head_dim ** -0.5 if scale is None else float(scale)
+    if not 0 < scale < math.inf:
+        raise ValueError(f"{what}: scale {scale} (positive)")
+    if not 0 <= cap < math.inf:
+        raise ValueError(f"{what}: cap {cap} (0: none)")
+    if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (heads,) or not slopes.is_contiguous()):
+        raise ValueError(f"slopes: contiguous f32 [{heads}]")
+    return scale
 
 
-def _ranged_desc(q, k, v, heads, kv_heads, head_dim, ranges, scale, cap, slopes) -> RangedAttnDesc:
-    _want(head_dim % 8 == 0 and 8 <= head_dim <= 160, f"ranged_attn: head_dim {head_dim} (8 ... 160, a multiple of 8)")
-    _want(heads > 0 and kv_heads > 0 and heads % kv_heads == 0, f"ranged_attn: {heads} heads over {kv_heads} key heads")
-    q = _attn_rows("q", q, heads, head_dim, None)
-    B = q.shape[0]
-    k, v = _attn_rows("k", k, kv_heads, head_dim, B), _attn_rows("v", v, kv_heads, head_dim, B)
-    _want(k.shape == v.shape, f"ranged_attn: k {tuple(k.shape)}, v {tuple(v.shape)}")
-    _same_device(q, k, v, ranges)
-    d = RangedAttnDesc()
-    if ranges is not None:
-        _want(ranges.dtype == torch.int32 and tuple(ranges.shape) == (B, q.shape[1], 2) and ranges.is_contiguous() and ranges.data_ptr() % 8 == 0,
-              f"ranges: contiguous int32 [{B}, {q.shape[1]}, 2] (key_ranges)")
-        d.ranges = ranges.data_ptr()
-    _score_args("ranged_attn", d, head_dim, scale, cap, slopes, heads, q)
-    _need_gpu(q)
-    d.q, d.k, d.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    d.B, d.H, d.Hk, d.Nq, d.Nk, d.D = B, heads, kv_heads, q.shape[1], k.shape[1], head_dim
-    d.ldq, d.ldk, d.ldv, d.sq, d.sk, d.sv = _ld(q), _ld(k), _ld(v), _sb(q), _sb(k), _sb(v)
-    return d
+def _ranges_arg(ranges, B, Nq):
+    if ranges is not None and (ranges.dtype != torch.int32 or ranges.shape != (B, Nq, 2) or not ranges.is_contiguous() or ranges.data_ptr() & 7):
+        raise ValueError(f"ranges: contiguous int32 [{B}, {Nq}, 2] (key_ranges)")
 
 
 def ranged_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, kv_heads: int, head_dim: int,
@@ -1646,13 +1668,22 @@ def ranged_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, k
     h // (heads // kv_heads) serves head h; D a multiple of 8 up to 160.  ``return_lse``: also the f32 [B, heads, Nq]
     log2-sum-exp rows that ``ranged_attn_bwd`` takes; ``return_rest`` (with it): and what rounding took from o, bf16 like it,
     which makes the gradients of q and k more exact.  Not differentiable: models.layers.ranged_attention is."""
-    d = _ranged_desc(q, k, v, heads, kv_heads, head_dim, ranges, scale, cap, slopes)
-    o = torch.empty(d.B, d.Nq, heads * head_dim, dtype=bf16, device=q.device)
-    lse = torch.empty(d.B, heads, d.Nq, dtype=torch.float32, device=q.device) if return_lse else None
+    scale = _attn_args("ranged_attn", heads, kv_heads, head_dim, scale, cap, slopes)
+    qp, B, Nq, C_, ldq, sq = _attn_rows("q", q, heads, head_dim)
+    kp, Bk, Nk, _, ldk, sk = _attn_rows("k", k, kv_heads, head_dim)
+    vp, _, _, _, ldv, sv = _attn_rows("v", v, kv_heads, head_dim)
+    if Bk != B or k.shape != v.shape:
+        raise ValueError(f"ranged_attn: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: one batch expected, k and v alike")
+    _ranges_arg(ranges, B, Nq)
+    device = _one_device(q, k, v, ranges, slopes)
+    if device < 0:
+        _need_gpu(q)
+    o = torch.empty(B, Nq, C_, dtype=bf16, device=q.device)
+    lse = torch.empty(B, heads, Nq, dtype=torch.float32, device=q.device) if return_lse or return_rest else None
     rest = torch.empty_like(o) if return_rest else None
-    d.o, d.rest, d.lse, d.ldo, d.so = o.data_ptr(), _ptr(rest), _ptr(lse), heads * head_dim, o.stride(0)
-    with _on(q):
-        check(lib.lbmk_ranged_attn(C.byref(d), _stream()), "lbmk_ranged_attn")
+    d = RangedAttnDesc(qp, kp, vp, None, o.data_ptr(), _ptr(rest), None, None, None, _ptr(lse), _ptr(ranges), _ptr(slopes), None,
+                       B, heads, kv_heads, Nq, Nk, head_dim, ldq, ldk, ldv, C_, 0, sq, sk, sv, Nq * C_, 0, scale, cap)
+    _launch(device, "lbmk_ranged_attn", lib.lbmk_ranged_attn, C.byref(d))
     return (o, lse, rest) if return_rest else (o, lse) if return_lse else o
 
 
@@ -1660,20 +1691,32 @@ def ranged_attn_bwd(q, k, v, o, do, lse, heads: int, kv_heads: int, head_dim: in
                     cap: float = 0.0, slopes=None, rest=None):
     """Gradients (dq, dk, dv) of ``ranged_attn`` for its output ``o`` (and ``rest``), the output's gradient ``do`` and the rows
     ``lse``; the gradients of shared key heads are summed in a fixed order."""
-    d = _ranged_desc(q, k, v, heads, kv_heads, head_dim, ranges, scale, cap, slopes)
-    o, do = _attn_rows("o", o, heads, head_dim, d.B), _attn_rows("do", do, heads, head_dim, d.B)
-    _want(o.shape == q.shape and do.shape == q.shape, "ranged_attn_bwd: o and do have q's shape")
-    _want(lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (d.B, heads, d.Nq), f"lse: contiguous f32 [{d.B}, {heads}, {d.Nq}]")
-    _want(rest is None or (rest.dtype == bf16 and rest.shape == q.shape and rest.is_contiguous()), "rest: contiguous bf16 of q's shape")
-    _same_device(q, o, do, lse, rest)
-    new = torch.empty if d.Nq and d.B else torch.zeros      # without queries the keys' gradients are zeros that no kernel writes
-    dq, dk, dv = (new(t.shape, dtype=bf16, device=q.device) for t in (q, k, v))
-    scratch = torch.empty(lib.lbmk_ranged_attn_bwd_scratch_floats(d.B, heads, kv_heads, d.Nq, d.Nk, head_dim, 0 if ranges is None else 1), dtype=torch.float32, device=q.device)
-    d.o, d.rest, d.dout, d.lse, d.scratch = o.data_ptr(), _ptr(rest), do.data_ptr(), lse.data_ptr(), scratch.data_ptr()
-    d.dq, d.dk, d.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-    d.ldo, d.ldg, d.so, d.sg = _ld(o), _ld(do), _sb(o), _sb(do)
-    with _on(q):
-        check(lib.lbmk_ranged_attn_bwd(C.byref(d), _stream()), "lbmk_ranged_attn_bwd")
+    scale = _attn_args("ranged_attn_bwd", heads, kv_heads, head_dim, scale, cap, slopes)
+    qp, B, Nq, C_, ldq, sq = _attn_rows("q", q, heads, head_dim)
+    kp, Bk, Nk, Ck, ldk, sk = _attn_rows("k", k, kv_heads, head_dim)
+    vp, _, _, _, ldv, sv = _attn_rows("v", v, kv_heads, head_dim)
+    if Bk != B or k.shape != v.shape:
+        raise ValueError(f"ranged_attn_bwd: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: one batch expected, k and v alike")
+    op, _, _, _, ldo, so = _attn_rows("o", o, heads, head_dim)
+    gp, _, _, _, ldg, sg = _attn_rows("do", do, heads, head_dim)
+    if o.shape != q.shape or do.shape != q.shape:
+        raise ValueError("ranged_attn_bwd: o and do have q's shape")
+    if lse.dtype != torch.float32 or not lse.is_contiguous() or lse.shape != (B, heads, Nq):
+        raise ValueError(f"lse: contiguous f32 [{B}, {heads}, {Nq}]")
+    if rest is not None and (rest.dtype != bf16 or rest.shape != q.shape or not rest.is_contiguous()):
+        raise ValueError("rest: contiguous bf16 of q's shape")
+    _ranges_arg(ranges, B, Nq)
+    device = _one_device(q, k, v, o, do, lse, rest, ranges, slopes)
+    if device < 0:
+        _need_gpu(q)
+    new = torch.empty if Nq and B else torch.zeros      # without queries the keys' gradients are zeros that no kernel writes
+    dev = q.device
+    dq, dk, dv = new(B, Nq, C_, dtype=bf16, device=dev), new(B, Nk, Ck, dtype=bf16, device=dev), new(B, Nk, Ck, dtype=bf16, device=dev)
+    scratch = torch.empty(lib.lbmk_ranged_attn_bwd_scratch_floats(B, heads, kv_heads, Nq, Nk, head_dim, 0 if ranges is None else 1),
+                          dtype=torch.float32, device=dev)
+    d = RangedAttnDesc(qp, kp, vp, gp, op, _ptr(rest), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), lse.data_ptr(), _ptr(ranges), _ptr(slopes),
+                       scratch.data_ptr(), B, heads, kv_heads, Nq, Nk, head_dim, ldq, ldk, ldv, ldo, ldg, sq, sk, sv, so, sg, scale, cap)
+    _launch(device, "lbmk_ranged_attn_bwd", lib.lbmk_ranged_attn_bwd, C.byref(d))
     return dq, dk, dv
 
 
@@ -1685,32 +1728,36 @@ def cached_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, l
     tokens in each cache with the new ones (clipped to [0, rows]).  New token i stands at lens - n + i and sees the keys up to
     itself (``window`` > 0: the last ``window`` of them); a token in front of the cache's start gets zeros.  Cache rows from
     lens on are not read.  The keys are split over workgroups by the device's own lengths, so a captured call follows them."""
-    _want(head_dim % 8 == 0 and 8 <= head_dim <= 160, f"cached_attn: head_dim {head_dim} (8 ... 160, a multiple of 8)")
-    _want(heads > 0 and kv_heads > 0 and heads % kv_heads == 0, f"cached_attn: {heads} heads over {kv_heads} key heads")
-    _want(window >= 0, f"cached_attn: window {window}")
-    q = _attn_rows("q", q, heads, head_dim, None)
-    B, n = q.shape[:2]
-    k, v = _attn_rows("k_cache", k_cache, kv_heads, head_dim, B), _attn_rows("v_cache", v_cache, kv_heads, head_dim, B)
-    _want(k.shape == v.shape, f"cached_attn: k_cache {tuple(k.shape)}, v_cache {tuple(v.shape)}")
-    _want(lens.dtype == torch.int32 and tuple(lens.shape) == (B,) and lens.is_contiguous(), f"lens: contiguous int32 [{B}]")
-    _same_device(q, k, v, lens)
-    d = CachedAttnDesc()
-    _score_args("cached_attn", d, head_dim, scale, cap, slopes, heads, q)
-    _need_gpu(q)
-    o = torch.empty(B, n, heads * head_dim, dtype=bf16, device=q.device)
-    nfl = lib.lbmk_cached_attn_scratch_floats(B, heads, kv_heads, n, k.shape[1], head_dim)
+    scale = _attn_args("cached_attn", heads, kv_heads, head_dim, scale, cap, slopes)
+    if window < 0:
+        raise ValueError(f"cached_attn: window {window}")
+    qp, B, n, C_, ldq, sq = _attn_rows("q", q, heads, head_dim)
+    kp, Bk, rows, _, ldk, sk = _attn_rows("k_cache", k_cache, kv_heads, head_dim)
+    vp, _, _, _, ldv, sv = _attn_rows("v_cache", v_cache, kv_heads, head_dim)
+    if Bk != B or k_cache.shape != v_cache.shape:
+        raise ValueError(f"cached_attn: q {tuple(q.shape)}, k_cache {tuple(k_cache.shape)}, v_cache {tuple(v_cache.shape)}: one batch expected, "
+                         "the caches alike")
+    if lens.dtype != torch.int32 or lens.shape != (B,) or not lens.is_contiguous():
+        raise ValueError(f"lens: contiguous int32 [{B}]")
+    device = _one_device(q, k_cache, v_cache, lens, slopes)
+    if device < 0:
+        _need_gpu(q)
+    o = torch.empty(B, n, C_, dtype=bf16, device=q.device)
+    nfl = lib.lbmk_cached_attn_scratch_floats(B, heads, kv_heads, n, rows, head_dim)
     scratch = torch.empty(nfl, dtype=torch.float32, device=q.device) if nfl else None
-    d.q, d.k, d.v, d.o, d.lens, d.scratch = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lens.data_ptr(), _ptr(scratch)
-    d.B, d.H, d.Hk, d.n, d.cap_rows, d.D, d.window = B, heads, kv_heads, n, k.shape[1], head_dim, window
-    d.ldq, d.ldk, d.ldv, d.sq, d.sk, d.sv = _ld(q), _ld(k), _ld(v), _sb(q), _sb(k), _sb(v)
-    with _on(q):
-        check(lib.lbmk_cached_attn(C.byref(d), _stream()), "lbmk_cached_attn")
+    d = CachedAttnDesc(qp, kp, vp, o.data_ptr(), lens.data_ptr(), _ptr(slopes), _ptr(scratch), B, heads, kv_heads, n, rows, head_dim, window,
+                       ldq, ldk, ldv, sq, sk, sv, scale, cap)
+    _launch(device, "lbmk_cached_attn", lib.lbmk_cached_attn, C.byref(d))
     return o
 
 
 # --------------------------------------------------------------------------------------
 # token operators: a linear layer with the low-rank adapters of many requests
 # --------------------------------------------------------------------------------------
+# rows up to which the shared weight is streamed through registers instead of a tiled product
+ADAPTER_FEW_ROWS = lib.lbmk_adapter_few_rows()
+
+
 def linear_adapters(x: torch.Tensor, pw: PackedWeight, down: torch.Tensor, up: torch.Tensor, index: torch.Tensor,
                     scaling: Optional[torch.Tensor] = None, *, tile: int = -1) -> torch.Tensor:
     """y = x W^T + b + scaling[a] (x down[a]^T) up[a]^T with a = index[request]: one shared layer, each request with its own
@@ -1720,53 +1767,64 @@ def linear_adapters(x: torch.Tensor, pw: PackedWeight, down: torch.Tensor, up: t
     (``pack_linear_weight``); down: bf16 [count, rank, K], up: bf16 [count, N, rank] (rank 1 ... 256), scaling: f32 [count] or
     None; index: int32 [requests] on the device.  The adapter's share is added in f32, before y's one rounding; a row's result does
     not depend on the other requests' adapters.  Serving only: no gradients."""
-    _want(x.dim() in (2, 3), f"linear_adapters: x [requests, rows, K] or [requests, K] expected, got {tuple(x.shape)}")
-    x3 = x if x.dim() == 3 else x[:, None]
-    R, rows, K = x3.shape
-    _want(x.dtype == bf16 and pw.w.dtype == bf16 and down.dtype == bf16 and up.dtype == bf16,
-          f"linear_adapters: x {x.dtype}, weight {pw.w.dtype}, adapters {down.dtype} / {up.dtype} (all bf16)")
-    _want(not pw.geglu and pw.KH == 1 and pw.KW == 1, "linear_adapters: a plain linear layer")
-    _want(K == pw.K and K % 8 == 0 and pw.N % 8 == 0, f"linear_adapters: x has {K} channels, the layer is {pw.K} -> {pw.N} (multiples of 8)")
-    _want(down.dim() == 3 and up.dim() == 3 and down.shape[0] == up.shape[0] > 0 and down.shape[2] == K and up.shape[1] == pw.N and
-          down.shape[1] == up.shape[2] and 1 <= up.shape[2] <= 256 and down.is_contiguous() and up.is_contiguous() and
-          down.data_ptr() % 16 == 0 and up.data_ptr() % 16 == 0,
-          f"linear_adapters: down {tuple(down.shape)}, up {tuple(up.shape)} (contiguous [count, rank, {K}], [count, {pw.N}, rank], rank 1 ... 256)")
-    count, rank = down.shape[:2]
-    _want(index.dtype == torch.int32 and tuple(index.shape) == (R,) and index.is_contiguous(), f"index: contiguous int32 [{R}]")
-    _want(scaling is None or (scaling.dtype == torch.float32 and tuple(scaling.shape) == (count,) and scaling.is_contiguous()),
-          f"scaling: contiguous f32 [{count}]")
-    _same_device(x, pw.w, pw.bias, down, up, index, scaling)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, down, up, scaling)):
+    shape, stride, w = x.shape, x.stride(), pw.w
+    if len(shape) == 3:
+        R, rows, K = shape
+        sr, ldx, unit = stride
+    elif len(shape) == 2:
+        (R, K), rows, (sr, unit) = shape, 1, stride
+        ldx = sr
+    else:
+        raise ValueError(f"linear_adapters: x [requests, rows, K] or [requests, K] expected, got {tuple(shape)}")
+    if x.dtype != bf16 or w.dtype != bf16 or down.dtype != bf16 or up.dtype != bf16:
+        raise ValueError(f"linear_adapters: x {x.dtype}, weight {w.dtype}, adapters {down.dtype} / {up.dtype} (all bf16)")
+    N = pw.N
+    if pw.geglu or pw.KH != 1 or pw.KW != 1:
+        raise ValueError("linear_adapters: a plain linear layer")
+    if K != pw.K or K % 8 or N % 8:
+        raise ValueError(f"linear_adapters: x has {K} channels, the layer is {pw.K} -> {N} (multiples of 8)")
+    dsh, ush = down.shape, up.shape
+    dp, upp = down.data_ptr(), up.data_ptr()
+    if (len(dsh) != 3 or len(ush) != 3 or dsh[0] < 1 or dsh[0] != ush[0] or dsh[2] != K or ush[1] != N or dsh[1] != ush[2] or not 1 <= dsh[1] <= 256 or
+            not down.is_contiguous() or not up.is_contiguous() or dp & 15 or upp & 15):
+        raise ValueError(f"linear_adapters: down {tuple(dsh)}, up {tuple(ush)} (contiguous [count, rank, {K}], [count, {N}, rank], rank 1 ... 256)")
+    count, rank = dsh[0], dsh[1]
+    if index.dtype != torch.int32 or index.shape != (R,) or not index.is_contiguous():
+        raise ValueError(f"index: contiguous int32 [{R}]")
+    if scaling is not None and (scaling.dtype != torch.float32 or scaling.shape != (count,) or not scaling.is_contiguous()):
+        raise ValueError(f"scaling: contiguous f32 [{count}]")
+    device = _one_device(x, w, pw.bias, down, up, index, scaling)
+    if torch.is_grad_enabled() and (x.requires_grad or down.requires_grad or up.requires_grad or (scaling is not None and scaling.requires_grad)):
         raise NotImplementedError("linear_adapters is inference-only: call it under torch.no_grad() or detach its operands")
     # one row stride for all rows (a request's rows follow the previous one's)
-    ldx = x3.stride(1) if rows > 1 else x3.stride(0) if R > 1 else K
-    ok = x3.stride(2) == 1 and x.data_ptr() % 16 == 0 and ldx % 8 == 0 and ldx >= K and (rows <= 1 or R <= 1 or x3.stride(0) == rows * ldx)
-    _want(ok or x.numel() == 0, f"linear_adapters: strides {x.stride()}: channels adjacent, one stride of a multiple of 8 between all rows")
-    _need_gpu(x)
-    T, N = R * rows, pw.N
-    out = torch.empty(*x.shape[:-1], N, dtype=bf16, device=x.device)
+    if rows <= 1:
+        ldx = sr
+    if R * rows <= 1:
+        ldx = K
+    xp = x.data_ptr()
+    if (unit != 1 or xp & 15 or ldx & 7 or ldx < K or ldx >> 31 or (rows > 1 and R > 1 and sr != rows * ldx)) and R * rows:
+        raise ValueError(f"linear_adapters: strides {stride}: channels adjacent, one stride of a multiple of 8 between all rows")
+    if device < 0:
+        _need_gpu(x)
+    T = R * rows
+    out = torch.empty(*shape[:-1], N, dtype=bf16, device=x.device)
     if T == 0:
         return out
-    tk = ceil_to(rank, 32)
+    tk = (rank + 31) // 32 * 32
     t = torch.empty(T, tk, dtype=bf16, device=x.device)
-    with _on(x):
-        s = _stream()
-        check(lib.lbmk_adapter_down(x.data_ptr(), down.data_ptr(), index.data_ptr(), _ptr(scaling), t.data_ptr(), R, rows, K, ldx, rank, tk, count, s),
-              "lbmk_adapter_down")
-        if tile < 0 and T <= ADAPTER_FEW_ROWS:
-            check(lib.lbmk_adapter_linear_few(x.data_ptr(), pw.w.data_ptr(), _ptr(pw.bias), t.data_ptr(), up.data_ptr(), index.data_ptr(),
-                                              out.data_ptr(), R, rows, N, K, ldx, pw.Kp, N, rank, tk, count, s), "lbmk_adapter_linear_few")
-            return out
-        d = IgemmDesc()
-        d.a, d.w, d.out, d.bias = x.data_ptr(), pw.w.data_ptr(), out.data_ptr(), _ptr(pw.bias)
-        d.M, d.N, d.K, d.Kp, d.Cin, d.a_cs = T, N, K, pw.Kp, K, ldx
-        d.IH = d.IW = d.OH = d.OW = d.KH = d.KW = d.stride = 1
-        d.ldo, d.act, d.alpha, d.batch, d.tile = N, ACT_NONE, 1.0, 1, tile
-        d.lr_t, d.lr_up, d.lr_index = t.data_ptr(), up.data_ptr(), index.data_ptr()
-        d.lr_rank, d.lr_k, d.lr_rows, d.lr_count = rank, tk, rows, count
+    bias, ip, tp = _ptr(pw.bias), index.data_ptr(), t.data_ptr()
+    _launch(device, "lbmk_adapter_down", lib.lbmk_adapter_down, xp, dp, ip, _ptr(scaling), tp, R, rows, K, ldx, rank, tk, count)
+    if tile < 0 and T <= ADAPTER_FEW_ROWS:
+        _launch(device, "lbmk_adapter_linear_few", lib.lbmk_adapter_linear_few, xp, w.data_ptr(), bias, tp, upp, ip, out.data_ptr(), R, rows, N, K,
+                ldx, pw.Kp, N, rank, tk, count)
+        return out
+    d = IgemmDesc()
+    d.a, d.w, d.out, d.bias = xp, w.data_ptr(), out.data_ptr(), bias
+    d.M, d.N, d.K, d.Kp, d.Cin, d.a_cs = T, N, K, pw.Kp, K, ldx
+    d.IH = d.IW = d.OH = d.OW = d.KH = d.KW = d.stride = 1
+    d.ldo, d.act, d.alpha, d.batch, d.tile = N, ACT_NONE, 1.0, 1, tile
+    d.lr_t, d.lr_up, d.lr_index = tp, upp, ip
+    d.lr_rank, d.lr_k, d.lr_rows, d.lr_count = rank, tk, rows, count
+    with contextlib.nullcontext() if device == torch.cuda.current_device() else torch.cuda.device(device):
         _igemm(d, 2.0 * T * (pw.alg_nk or N * K))
     return out
-
-
-# rows up to which the shared weight is streamed through registers instead of a tiled product
-ADAPTER_FEW_ROWS = lib.lbmk_adapter_few_rows()
