@@ -180,14 +180,14 @@ int lbmk_layernorm(const void* x, void* y, const float* gamma, const float* beta
  *   y[m] = x[m] W^T + bias + scaling[a] (x[m] down[a]^T) up[a]^T,   a = index[m / rows]  (outside [0, count): no adapter)
  * No counterpart in the reference; stands next to lbmk_igemm.  lbmk_adapter_down writes t[m] = scaling[a] x[m] down[a]^T (bf16
  * [requests * rows][tk], tk = rank rounded up to 32, columns from rank on zeros; rows without an adapter are left as they are);
- * lbmk_igemm with lr_* fields, or for up to lbmk_adapter_few_rows() rows lbmk_adapter_linear_few, adds t up[a]^T to the shared
+ * lbmk_igemm with lr_* fields, or lbmk_adapter_linear_few where lbmk_adapter_few_suits() is 1 (few rows), adds t up[a]^T to the shared
  * product in f32, before y is rounded.
  *   x : bf16 [requests * rows][ldx], K channels (a multiple of 8);  down : bf16 [count][rank][K];  up : bf16 [count][N][rank];
  *   w : bf16 [N][ldw];  bias : f32 [N] or NULL;  scaling : f32 [count] or NULL (ones);  index : int32 [requests];  rank 1 ... 256
  * ---------------------------------------------------------------------- */
 int lbmk_adapter_down(const void* x, const void* down, const int32_t* index, const float* scaling, void* t, int requests, int rows,
                       int K, int64_t ldx, int rank, int tk, int count, void* stream);
-int lbmk_adapter_few_rows(void);
+int lbmk_adapter_few_suits(int requests, int rows);
 int lbmk_adapter_linear_few(const void* x, const void* w, const float* bias, const void* t, const void* up, const int32_t* index, void* y,
                             int requests, int rows, int N, int K, int64_t ldx, int ldw, int64_t ldy, int rank, int tk, int count, void* stream);
 

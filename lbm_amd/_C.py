@@ -92,7 +92,7 @@ SIGNATURES = {
     "lbmk_groupnorm_static": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, f32, i32, vp]),
     "lbmk_layernorm": (i32, [vp, vp, vp, vp, i32, i32, f32, vp]),
     "lbmk_adapter_down": (i32, [vp] * 5 + [i32, i32, i32, i64, i32, i32, i32, vp]),
-    "lbmk_adapter_few_rows": (i32, []),
+    "lbmk_adapter_few_suits": (i32, [i32, i32]),
     "lbmk_adapter_linear_few": (i32, [vp] * 7 + [i32, i32, i32, i32, i64, i32, i64, i32, i32, i32, vp]),
     "lbmk_norm_rope": (i32, [C.POINTER(NormRopeDesc), vp]),
     "lbmk_norm_rope_bwd_scratch_floats": (i64, [i32]),

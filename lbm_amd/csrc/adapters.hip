@@ -7,8 +7,8 @@
 //     v_mfma_f32_16x16x32_bf16, both operands K-contiguous and read straight into registers; the four waves of a workgroup
 //     split K and are joined in LDS in a fixed order, because there are too few row groups to fill the chip otherwise.
 //   * the shared product with t B_a^T added to its accumulators before the one rounding of y: many rows in lbmk_igemm
-//     (lr_* fields), few rows here: with up to 64 rows the weight is read once and its bytes are the floor, so a workgroup
-//     of 8 waves takes 16 output columns, its waves split K, and W goes from memory into MFMA operands without LDS.
+//     (lr_* fields), few rows here: the weight's bytes are the floor, so a workgroup of 8 waves takes
+//     16 output columns of 64 rows, its waves split K, and W goes from memory into MFMA operands without LDS.
 #include "common.h"
 
 namespace {
@@ -68,9 +68,9 @@ __global__ __launch_bounds__(64 * DOWN_WAVES) void adapter_down_kernel(const bf1
   *(u16x4*)(t + ((int64_t)request * rows + m0 + lr) * tk + n) = o;
 }
 
-constexpr int FEW_WAVES = 8, FEW_ROWS = 64;
+constexpr int FEW_WAVES = 8, FEW_ROWS = 64;       // rows of a workgroup
 
-// MT: row groups of 16
+// MT: row groups of 16.  grid: (ceil(N / 16), ceil(M / 64))
 template <int MT>
 __global__ __launch_bounds__(64 * FEW_WAVES) void adapter_few_kernel(const bf16_t* __restrict__ x, const bf16_t* __restrict__ w,
                                                                    const float* __restrict__ bias, const bf16_t* __restrict__ t,
@@ -80,11 +80,11 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void adapter_few_kernel(const bf16_
   __shared__ f32x4 part[FEW_WAVES][MT][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 15, lq = lane >> 4;
-  const int n0 = blockIdx.x * 16;
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * FEW_ROWS;
   const bf16_t* wr = w + (int64_t)min(n0 + lr, N - 1) * ldw + 8 * lq;
   const bf16_t* xr[MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) xr[i] = x + (int64_t)min(16 * i + lr, M - 1) * ldx + 8 * lq;
+  for (int i = 0; i < MT; ++i) xr[i] = x + (int64_t)min(m0 + 16 * i + lr, M - 1) * ldx + 8 * lq;
   f32x4 acc[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -105,7 +105,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void adapter_few_kernel(const bf16_
   __syncthreads();
   // output (m, n): four neighbouring columns per thread, as they lie in the accumulators
   for (int o = threadIdx.x; o < MT * 64; o += 64 * FEW_WAVES) {
-    const int i = o >> 6, l = o & 63, m = 16 * i + (l & 15), n = n0 + 4 * (l >> 4);
+    const int i = o >> 6, l = o & 63, m = m0 + 16 * i + (l & 15), n = n0 + 4 * (l >> 4);
     if (m >= M || n >= N) continue;                            // N % 4 == 0
     f32x4 v = part[0][i][l];
 #pragma unroll
@@ -166,13 +166,20 @@ extern "C" int lbmk_adapter_down(const void* x, const void* down, const int32_t*
   return lbmk_check_launch("adapter_down");
 }
 
-extern "C" int lbmk_adapter_few_rows(void) { return FEW_ROWS; }
+// Both sides measured, the call with lbmk_igemm against the one with the few-rows kernel (layers 1280 -> 1280, 640 -> 5120,
+// 2560 -> 640, rank 16): 128 rows, of 8, 16 or 32 per request: 18 ... 30 us against 15 ... 23; 256 rows, of 4: 23 / 22 / 33
+// against 20 / 25 / 23, of 16: 19 / 18 / 29 against 21 / 25 / 24.  A tile of lbmk_igemm takes one step of its factor loop per
+// request in it, so single rows cost it most: 512 of them 44 / 44 / 61 against 29 / 50 / 39, 1024 48 / 92 / 65 against 52 / 85 / 56.
+extern "C" int lbmk_adapter_few_suits(int requests, int rows) {
+  const int64_t M = (int64_t)requests * rows;
+  return M <= 128 || (rows <= 2 && M <= 512);
+}
 
 extern "C" int lbmk_adapter_linear_few(const void* x, const void* w, const float* bias, const void* t, const void* up, const int32_t* index,
                                        void* y, int requests, int rows, int N, int K, int64_t ldx, int ldw, int64_t ldy, int rank, int tk, int count,
                                        void* stream) {
-  LBMK_REQUIRE(requests >= 0 && rows >= 0 && (int64_t)requests * rows <= FEW_ROWS, "adapter_linear_few: %d requests of %d rows (at most %d rows)",
-               requests, rows, FEW_ROWS);
+  LBMK_REQUIRE(requests >= 0 && rows >= 0 && (int64_t)requests * rows <= 65535 * FEW_ROWS, "adapter_linear_few: %d requests of %d rows (at most %d rows)",
+               requests, rows, 65535 * FEW_ROWS);
   LBMK_REQUIRE(N > 0 && N % 4 == 0 && K > 0 && K % 8 == 0 && rank > 0 && rank <= 256 && count > 0 && tk % 32 == 0 && tk >= rank, "adapter_linear_few: sizes");
   if (requests == 0 || rows == 0) return LBMK_OK;
   LBMK_REQUIRE(x && w && t && up && index && y && lbmk_aligned(x, 16) && lbmk_aligned(w, 16) && lbmk_aligned(t, 16) &&
@@ -181,7 +188,7 @@ extern "C" int lbmk_adapter_linear_few(const void* x, const void* w, const float
   LBMK_REQUIRE(ldx % 8 == 0 && ldx >= K && ldw % 8 == 0 && ldw >= K && ldy % 4 == 0 && ldy >= N, "adapter_linear_few: row strides");
   const int M = requests * rows;
 #define FEW(MT)                                                                                                                    \
-  hipLaunchKernelGGL((adapter_few_kernel<MT>), dim3((N + 15) / 16), dim3(64 * FEW_WAVES), 0, (hipStream_t)stream, (const bf16_t*)x, \
+  hipLaunchKernelGGL((adapter_few_kernel<MT>), dim3((N + 15) / 16, (M + FEW_ROWS - 1) / FEW_ROWS), dim3(64 * FEW_WAVES), 0, (hipStream_t)stream, (const bf16_t*)x, \
                      (const bf16_t*)w, bias, (const bf16_t*)t, (const bf16_t*)up, index, (bf16_t*)y, M, rows, N, K, ldx, ldw, ldy, rank, tk, count)
   switch ((M + 15) / 16) {
     case 1: FEW(1); break;

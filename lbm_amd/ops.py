@@ -1754,8 +1754,6 @@ def cached_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, l
 # --------------------------------------------------------------------------------------
 # token operators: a linear layer with the low-rank adapters of many requests
 # --------------------------------------------------------------------------------------
-# rows up to which the shared weight is streamed through registers instead of a tiled product
-ADAPTER_FEW_ROWS = lib.lbmk_adapter_few_rows()
 
 
 def linear_adapters(x: torch.Tensor, pw: PackedWeight, down: torch.Tensor, up: torch.Tensor, index: torch.Tensor,
@@ -1814,7 +1812,7 @@ def linear_adapters(x: torch.Tensor, pw: PackedWeight, down: torch.Tensor, up: t
     t = torch.empty(T, tk, dtype=bf16, device=x.device)
     bias, ip, tp = _ptr(pw.bias), index.data_ptr(), t.data_ptr()
     _launch(device, "lbmk_adapter_down", lib.lbmk_adapter_down, xp, dp, ip, _ptr(scaling), tp, R, rows, K, ldx, rank, tk, count)
-    if tile < 0 and T <= ADAPTER_FEW_ROWS:
+    if tile < 0 and lib.lbmk_adapter_few_suits(R, rows):
         _launch(device, "lbmk_adapter_linear_few", lib.lbmk_adapter_linear_few, xp, w.data_ptr(), bias, tp, upp, ip, out.data_ptr(), R, rows, N, K,
                 ldx, pw.Kp, N, rank, tk, count)
         return out

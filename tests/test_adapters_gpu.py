@@ -53,13 +53,17 @@ CASES = [  # requests, rows, K, N, adapters, rank, bias
     (3, 20, 200, 136, 2, 3, True),
     (64, 1, 2560, 640, 8, 32, True),
     (4, 16, 1280, 72, 2, 256, True),
-    (65, 1, 320, 328, 5, 16, True),            # one row per request in the tiled product
+    (65, 1, 320, 328, 5, 16, True),
     (100, 1, 328, 72, 5, 5, True),
     (5, 77, 640, 1000, 3, 8, True),
     (3, 130, 72, 200, 2, 40, False),
     (2, 300, 1280, 640, 2, 16, True),
     (7, 33, 128, 96, 3, 100, True),
     (2, 1024, 640, 640, 2, 32, True),
+    (129, 1, 320, 72, 5, 16, True),            # several workgroups' rows in the few-rows kernel, a last row alone
+    (250, 2, 328, 136, 3, 6, False),
+    (513, 1, 128, 200, 4, 8, True),            # one row per request in the tiled product
+    (43, 3, 128, 200, 4, 8, True),
 ]
 
 
@@ -200,7 +204,7 @@ def test_entry_points_refuse_what_their_kernels_do_not_take():
 
     def few(x=P, w=P, bias=P, t=P, up=P, index=P, y=P, requests=2, rows=3, N=32, K=64, ldx=64, ldw=64, ldy=32, rank=8, tk=32, count=2):
         return _C.lib.lbmk_adapter_linear_few(x, w, bias, t, up, index, y, requests, rows, N, K, ldx, ldw, ldy, rank, tk, count, None)
-    for bad in (dict(requests=65, rows=1), dict(rows=33), dict(N=30), dict(K=60), dict(ldw=56), dict(ldy=28), dict(up=P + 8), dict(y=P + 4), dict(w=0), dict(tk=16),
+    for bad in (dict(requests=1 << 20, rows=1 << 3), dict(rows=-1), dict(N=30), dict(K=60), dict(ldw=56), dict(ldy=28), dict(up=P + 8), dict(y=P + 4), dict(w=0), dict(tk=16),
                 dict(rank=33), dict(count=0), dict(bias=P + 2)):
         assert few(**bad) == 1, bad
 
