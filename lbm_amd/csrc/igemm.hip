@@ -100,7 +100,7 @@ __device__ __forceinline__ float xor32_sum(float v) {
 // knows, so a load written after a store waits for it.  The bias of all NI column groups is read once,
 // and the residual / rowvec operands of row group i+1 are in flight while row group i is stored.
 template <int MI, int NI, bool GNS>
-__device__ __forceinline__ void igemm_epilogue(const lbmk_igemm_desc& p, f32x4 (&acc)[MI][NI], int mbase,
+__device__ __forceinline__ void igemm_epilogue(const lbmk_igemm_desc& p, f32x4 (&tile)[MI][NI], int mbase,
                                                int nbase, int lane, int64_t zo, int64_t zr) {
   const int lr = lane & 15, lq = lane >> 4;
   const int ohw = p.OH * p.OW;
@@ -113,6 +113,9 @@ __device__ __forceinline__ void igemm_epilogue(const lbmk_igemm_desc& p, f32x4 (
   const bool vec_ok = ((n_out & 3) == 0) && ((p.ldo & 3) == 0) &&
                       (!res || (p.ldr & 3) == 0) && (!rowvec || (p.rowvec_ld & 3) == 0);
 
+  // the tile as scalars: kept as vectors over the branches below, every element is copied at each of them, and the copies do
+  // not fit the registers (300 bytes of spills per lane in the 256 x 256 tile; GEGLU layer 640 -> 2 x 2560, 65536 rows: 680 -> 553 us)
+  float acc[MI][NI][4];
   // fold alpha and the bias into the accumulators in place (the bias registers die right here)
   {
     float bv[NI][4];
@@ -141,7 +144,7 @@ __device__ __forceinline__ void igemm_epilogue(const lbmk_igemm_desc& p, f32x4 (
 #pragma unroll
       for (int j = 0; j < NI; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = acc[i][j][e] * p.alpha + bm + bv[j][e];
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = tile[i][j][e] * p.alpha + bm + bv[j][e];
     }
   }
 
@@ -321,7 +324,7 @@ __device__ __forceinline__ void igemm_epilogue(const lbmk_igemm_desc& p, f32x4 (
         for (int j = 0; j < NI; ++j) {
           if (geglu && (j & 1)) continue;
           const int no = out_col(j);
-          if (no < n_out) *(f32x4*)((float*)p.out + orow_off + no) = acc[i][j];
+          if (no < n_out) *(f32x4*)((float*)p.out + orow_off + no) = f32x4{acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
         }
       } else {
 #pragma unroll
