@@ -55,11 +55,12 @@ __device__ __forceinline__ int2 row_range(const Ranged& a, int b, int q) {
 //
 // Two parts per block of queries: part 1 takes the queries whose keys start behind those of the block's first query, part 0 the
 // others.  A block across two documents would walk the keys of both, one half of it idle in each, and it alone would set the
-// kernel's time; as two parts it does not.  Under a causal mask every query is of part 0, and part 1 ends at once.
+// kernel's time; as two parts it does not (the same documents in one part: 106 us instead of 67, 3000 keys with 4 heads of 160 63
+// instead of 32).  Under a causal mask every query is of part 0, and part 1 ends at once (2 ... 3 us of a short call).
 //
 // Documents and causal masks give the blocks very different numbers of keys, and a launch is often no more workgroups than the
-// chip holds at once: in any fixed order some CUs get three long ones and others three short ones.  So, with up to 512 items,
-// every workgroup ranks them by the span of keys that a few of their queries see (ties by index: a permutation, whatever the
+// chip holds at once: in any fixed order some CUs get three long ones and others three short ones.  So, over long rows and with up
+// to 512 items (order_blocks), every workgroup ranks them by the span of keys that a few of their queries see (ties by index: a permutation, whatever the
 // ranges are) and takes the item of its own rank: the longest first.  Where the chip holds the whole launch at once (snake), every
 // other round of CUs backwards, so that a CU with a long one gets a short one beside it; otherwise the next longest goes to the
 // CU that is done first, as it should.
@@ -596,8 +597,7 @@ __device__ __forceinline__ void keys_of(const Ranged& a, char* smem, int& b, int
       }
       mine = (n << 8) + (ORDER_ITEMS / 2 - 1 - t);
     }
-    __syncthreads();                      // (the keys lie over the last spans)
-    key[t] = mine;
+    key[t] = mine;                        // (behind the spans: there are at most ORDER_GROUPS - 256)
     __syncthreads();
     if (t < items) {
       int rank = 0;
@@ -941,6 +941,8 @@ int pad_head(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 1
 // parts of the key kernel's walk: enough workgroups for every CU to hold its fill (two of up to 96 channels, one wider).  Where
 // ranges make the walks unequal and they are long, twice as many, so that the next part goes to the CU that is done first.  A part
 // costs its f32 sums (8 bytes per element of dK and dV written and read): never more than eight, none below eight tiles.
+// Measured, the whole backward pass without any cut against with: 2 x 2111 tokens causal, 20 over 5 heads of 64, 317 -> 159 us, 4096
+// causal, 8 over 2 heads, 583 -> 195 us; the doubling: the documents of 9001 tokens 320 -> 282 us, 2 x 4096 with a prefix 328 -> 302.
 int dkv_splits(bool ranged, int B, int H, int Hk, int Nq, int Nk, int D) {
   const int64_t blocks = (int64_t)((Nk + RB - 1) / RB) * Hk * B, work = (int64_t)(H / Hk) * ((Nq + TB - 1) / TB);
   const int64_t slots = (D <= 96 ? 2ll : 1ll) * lbmk_num_cus();
@@ -951,14 +953,19 @@ int dkv_splits(bool ranged, int B, int H, int Hk, int Nq, int Nk, int D) {
   return (int)(s < 1 ? 1 : s > 8 ? 8 : s);
 }
 
-// workgroups of the row kernels that fit a CU (registers and LDS)
-int row_occupancy(int DHP) { return DHP <= 64 ? 3 : DHP <= 128 ? 2 : 1; }
+// workgroups of the row kernels that fit a CU (their launch bounds)
+int fwd_occupancy(int DHP) { return DHP <= 96 ? 3 : DHP <= 128 ? 2 : 1; }
+int dq_occupancy(int DHP) { return DHP <= 64 ? 3 : DHP <= 96 ? 2 : 1; }
 
-// ranked workgroups: where they are few enough for the order to matter and for the ranking to be cheap
-void order_blocks(Ranged& a) {
+// Ranked workgroups: few enough for the order to matter and for the ranking to be cheap, and walks long enough to pay for it (every
+// workgroup ranks before it starts, 2 ... 4 us).  Both sides measured: 9001 keys in 7 unequal documents, 10 heads of 64, 84 -> 67 us
+// forward, 310 -> 282 backward; up to 4096 keys it gains nothing (2 x 2111, 20 heads, causal documents: 26 -> 30 us).
+constexpr int ORDER_KEYS = 4096;
+bool order_pays(const Ranged& a, int64_t n) { return a.ranges && a.Nk > ORDER_KEYS && n <= 4ll * a.cus; }
+void order_blocks(Ranged& a, int occupancy) {
   const int64_t n = (int64_t)a.blocks * a.H * a.B;
-  a.ordered = a.ranges && n <= 4ll * a.cus && (int64_t)a.B * a.blocks * a.parts <= ORDER_ITEMS;
-  a.snake = n <= (int64_t)row_occupancy(pad_head(a.D)) * a.cus;
+  a.ordered = order_pays(a, n) && (int64_t)a.B * a.blocks * a.parts <= ORDER_ITEMS;
+  a.snake = n <= (int64_t)occupancy * a.cus;
 }
 
 int ranged_check(const lbmk_ranged_attn_desc* p, bool bwd) {
@@ -1056,7 +1063,7 @@ extern "C" int lbmk_ranged_attn(const lbmk_ranged_attn_desc* p, void* stream) {
   Ranged a = ranged_args(p);
   hipStream_t s = (hipStream_t)stream;
   a.blocks = (a.Nq + RB - 1) / RB;
-  order_blocks(a);
+  order_blocks(a, fwd_occupancy(pad_head(a.D)));
 #define FWD(DHP) hipLaunchKernelGGL((ranged_fwd_kernel<DHP>), dim3((unsigned)((int64_t)a.blocks * a.parts * a.H * a.B)), dim3(256), 0, s, a)
   BY_HEAD(pad_head(a.D), FWD)
 #undef FWD
@@ -1080,7 +1087,7 @@ extern "C" int lbmk_ranged_attn_bwd(const lbmk_ranged_attn_desc* p, void* stream
   a.tiles = (int4*)(p->scratch + ((int64_t)a.B * a.H * a.Nq + 3) / 4 * 4);
   hipStream_t s = (hipStream_t)stream;
   a.blocks = (a.Nq + RB - 1) / RB;
-  order_blocks(a);
+  order_blocks(a, dq_occupancy(pad_head(a.D)));
 #define DQ(DHP) hipLaunchKernelGGL((ranged_bwd_dq_kernel<DHP>), dim3((unsigned)((int64_t)a.blocks * a.parts * a.H * a.B)), dim3(256), 0, s, a)
   BY_HEAD(pad_head(a.D), DQ)
 #undef DQ
@@ -1088,7 +1095,7 @@ extern "C" int lbmk_ranged_attn_bwd(const lbmk_ranged_attn_desc* p, void* stream
     a.splits = dkv_splits(a.ranges != nullptr, a.B, a.H, a.Hk, a.Nq, a.Nk, a.D);
     const int64_t kblocks = (a.Nk + RB - 1) / RB, n = kblocks * a.Hk * a.B * a.splits;
     // (32 KB of LDS for the queries' spans: a stage pair of the narrowest heads is smaller)
-    a.ordered = a.ranges && a.D > 32 && n <= 8ll * a.cus && kblocks * a.B <= ORDER_ITEMS / 2 && (int64_t)a.B * ((a.Nq + TB - 1) / TB) * 2 <= ORDER_GROUPS - 256;
+    a.ordered = order_pays(a, n / 2) && a.D > 32 && kblocks * a.B <= ORDER_ITEMS / 2 && (int64_t)a.B * ((a.Nq + TB - 1) / TB) * 2 <= ORDER_GROUPS - 256;
     a.snake = n <= (a.D <= 96 ? 2ll : 1ll) * a.cus;
     a.part = (float*)(a.tiles + (int64_t)a.B * ((a.Nq + TB - 1) / TB) * 2);
 #define DKV(DHP) hipLaunchKernelGGL((ranged_bwd_dkv_kernel<DHP>), dim3((unsigned)((int64_t)((a.Nk + RB - 1) / RB) * a.Hk * a.B * a.splits)), dim3(256), 0, s, a)

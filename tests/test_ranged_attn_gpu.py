@@ -149,6 +149,37 @@ def test_forward_and_gradients(cuda, case):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("Nq,Nk,H,D,mask,times", [
+    (700, 4200, 2, 64, "random", (1, 30, 70)),           # 24, 720 and 1680 workgroups
+    (700, 4200, 2, 64, "docs", (1, 30, 70)),
+    (300, 4300, 2, 40, "causal", (1, 50)),
+    (300, 4200, 2, 96, "docs", (1, 50)),
+    (260, 4200, 1, 128, "random", (1, 90, 170)),
+    (260, 4200, 1, 160, "random", (1, 90)),
+    (200, 4200, 2, 32, "random", (1, 100)),
+])
+def test_ranked_workgroups_over_long_rows(cuda, Nq, Nk, H, D, mask, times):
+    """with few heads against the definition; the same heads many times over take other workgroups in another order, and each of
+    them has the same bits (the keys' gradients are cut into other parts: against the definition again)"""
+    from lbm_amd import ops
+    q, k, v, g, gen = make(9, 1, Nq, Nk, H, H, D)
+    ranges = ranges_of(mask, 1, Nq, Nk, gen)
+    want = definition(q, k, v, H, H, D, seen_by(ranges, Nk), (torch.arange(Nq) + Nk - Nq).expand(1, Nq), D ** -0.5, 0.0, None, g)
+    q, k, v, g, ranges = (t.to(cuda) for t in (q, k, v, g, ranges))
+    first = None
+    for n in times:
+        a, b, c, d = (t.repeat(1, 1, n) for t in (q, k, v, g))
+        o, lse, rest = ops.ranged_attn(a, b, c, n * H, n * H, D, ranges, return_lse=True, return_rest=True)
+        got = (o,) + ops.ranged_attn_bwd(a, b, c, o, d, lse, n * H, n * H, D, ranges, rest=rest)
+        first = first or got
+        for name, x, y in zip(("o", "dq", "dk", "dv"), got, first):
+            for part in (x[..., :H * D], x[..., -H * D:]):
+                check(name, part, want[name])
+            if name in ("o", "dq"):
+                assert torch.equal(x, y.repeat(1, 1, n)), (name, n)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("D", [40, 64, 128, 160])
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
 def test_values_at_places_that_are_not_seen(cuda, D, value):
