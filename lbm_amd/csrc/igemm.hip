@@ -437,6 +437,7 @@ __device__ __forceinline__ void igemm_epilogue_smx(const lbmk_igemm_desc& p, f32
 // row m belongs to, in the accumulators before the epilogue's one rounding.  The rank is a few MFMA steps deep, so the operands
 // come straight from memory (L2): no staging, and nothing in the K loop.  A 16-row group that holds rows of two requests keeps a
 // product only in the lanes of its own rows (a lane holds one row): a request never sees another one's adapter, NaN included.
+// 8 x 1024 rows, 1280 -> 3840, rank 32: 87 us, 85 without.
 template <int MI, int NI>
 __device__ __forceinline__ void igemm_low_rank(const lbmk_igemm_desc& p, f32x4 (&acc)[MI][NI], int mbase, int nbase, int lane) {
   const int lr = lane & 15, lq = lane >> 4;
