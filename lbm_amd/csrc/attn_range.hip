@@ -761,7 +761,7 @@ __device__ __forceinline__ bool ranged_bwd_dkv_body(const Ranged& a, char* smem)
     const int q0 = i.tile * TB;
     T::template stage<NI, TB>(qh + (int64_t)i.head * a.D, q0, a.Nq, a.ldq, a.D, place, wave, 4, buf);
     T::template stage<NI, TB>(gh + (int64_t)i.head * a.D, q0, a.Nq, a.ldg, a.D, place, wave, 4, buf + TB * T::ROW);
-    // rows past the end read zeros (their q and dO are zeros too: they add nothing)
+    // rows past the end read zeros
     if (stat_wanted)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           __builtin_amdgcn_make_buffer_rsrc((void*)(stat + i.head * stat_head + (int64_t)q0 * stat_row), 0, min(TB, a.Nq - q0) * stat_row, 0x00020000),
@@ -856,6 +856,13 @@ __device__ __forceinline__ bool ranged_bwd_dkv_body(const Ranged& a, char* smem)
           for (int e = 0; e < 4; ++e)
             if (kc < l[e] || kc >= g4[e]) p[4 * g + e] = ds[4 * g + e] = 0.f;
         }
+      }
+      if (qt * TB + 32 * u + 32 > a.Nq) {      // rows past the end: their statistics read as zeros, and a bias may make p infinite
+        asm volatile("" ::: "memory");
+        const int past = a.Nq - (qt * TB + 32 * u + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (acc_row(e, 0) >= past) p[e] = ds[e] = 0.f;
       }
       bf16x8 pf[2], df[2];
       pack_column(p, pf);

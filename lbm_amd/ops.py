@@ -1472,7 +1472,7 @@ def token_rows_ready(t: torch.Tensor) -> torch.Tensor:
         return t
     part = 16 // t.element_size() - 1
     *lead, unit = t.stride()
-    if unit == 1 and t.data_ptr() & 15 == 0 and not any(s & part for s in lead) and (not lead or t.shape[-2] <= 1 or lead[-1] >= t.shape[-1]):
+    if unit == 1 and t.data_ptr() & 15 == 0 and not any(s & part for s in lead) and (not lead or t.shape[-2] <= 1 or t.shape[-1] <= lead[-1] <= 1 << 22):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -1574,7 +1574,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, head_dim: int, q_weight: Opti
     [P, F, 2] and int32 ``positions`` [B, N] or [B, N, axes] rotate the first 2 * axes * F channels of a head: pair j
     takes axis j // F and column j % F, and is channels (j, j + axes * F), or (2j, 2j + 1) when ``interleaved``.  A
     position outside the table gives NaN.  No table: the norm alone.  ``out``: (q', k') destinations, also q and k
-    themselves.  Not differentiable: models.layers.qk_norm_rope is."""
+    themselves; they overlap nothing else that the call reads or writes.  Not differentiable: models.layers.qk_norm_rope is."""
     return _norm_rope(q, k, head_dim, q_weight, k_weight, table, positions, eps, interleaved, out, None)
 
 
@@ -1615,7 +1615,8 @@ def key_ranges(B: int, Nq: int, Nk: Optional[int] = None, *, causal: bool = Fals
     given = [t for t in (prefix, documents, lens) if t is not None]
     if given:
         _one_device(*given)
-        if device is not None and torch.device(device).type != given[0].device.type:
+        want = given[0].device if device is None else torch.device(device)
+        if want.type != given[0].device.type or (want.index is not None and want.index != given[0].device.index):
             raise ValueError(f"key_ranges: operands on {given[0].device}, device {device}")
     dev = given[0].device if given else torch.device(device if device is not None else "cuda")
     if dev.type != "cuda":

@@ -260,6 +260,26 @@ def test_windows_of_a_packed_projection_and_broadcast_keys(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("mask", ["none", "causal", "docs"])
+def test_slopes_that_favour_far_keys(cuda, mask):
+    """a negative slope: scores grow with the distance, far beyond exp2's range for a row that is not there (300 rows end inside a
+    tile), and the softmax's maximum alone keeps the others finite"""
+    from lbm_amd import ops
+    N, H, D = 300, 2, 64
+    q, k, v, g, gen = make(11, 1, N, N, H, H, D)
+    ranges = None if mask == "none" else ranges_of(mask, 1, N, N, gen)
+    seen = torch.ones(1, N, N, dtype=torch.bool) if ranges is None else seen_by(ranges, N)
+    slopes = torch.tensor([-1.0, -0.25])
+    want = definition(q, k, v, H, H, D, seen, torch.arange(N).expand(1, N), D ** -0.5, 0.0, slopes, g)
+    q, k, v, g, slopes = (t.to(cuda) for t in (q, k, v, g, slopes))
+    ranges = None if ranges is None else ranges.to(cuda)
+    o, lse = ops.ranged_attn(q, k, v, H, H, D, ranges, slopes=slopes, return_lse=True)
+    check("o", o, want["o"])
+    for n, x in zip(("dq", "dk", "dv"), ops.ranged_attn_bwd(q, k, v, o, g, lse, H, H, D, ranges, slopes=slopes)):
+        check(n, x, want[n])
+
+
+@pytest.mark.gpu
 def test_no_queries_no_keys(cuda):
     from lbm_amd import ops
     q, k, v, g, _ = make(4, 2, 9, 6, 2, 1, 64)
