@@ -174,11 +174,11 @@ __device__ __forceinline__ bool any_wave(bool x, int wave, int* sm) {
   return __builtin_amdgcn_readfirstlane(sm[0] | sm[1] | sm[2] | sm[3]) != 0;
 }
 
-template <int DH, class Form>
+template <int DH, int KS, class Form>
 __device__ __forceinline__ bool ranged_fwd_body(const Ranged& a, char* smem) {
   constexpr bool GUARD = Form::guard;
   using T = Tile<DH>;
-  constexpr int KS = T::KS, DT = T::DT, NI = T::CPR / 4, STAGE = 2 * TB * T::ROW;
+  constexpr int DT = T::DT, NI = T::CPR / 4, STAGE = 2 * TB * T::ROW;
   int* span = (int*)(smem + 2 * STAGE);
 
   const int t = threadIdx.x, lane = t & 63;
@@ -355,15 +355,15 @@ __device__ __forceinline__ bool ranged_fwd_body(const Ranged& a, char* smem) {
 }
 
 // the walk again, guarded: a call, so that its registers are not the kernel's
-template <int DH>
+template <int DH, int KS>
 __device__ __attribute__((noinline)) void ranged_fwd_again(uint64_t args, lds_ptr smem) {
-  ranged_fwd_body<DH, Guarded>(kernel_args(args), (char*)smem);
+  ranged_fwd_body<DH, KS, Guarded>(kernel_args(args), (char*)smem);
 }
 
-template <int DH>
+template <int DH, int KS>
 __global__ __launch_bounds__(256, DH <= 96 ? 3 : DH <= 128 ? 2 : 1) void ranged_fwd_kernel(const Ranged a) {
   __shared__ __attribute__((aligned(16))) char smem[2 * (2 * TB * Tile<DH>::ROW) + 64];
-  if (ranged_fwd_body<DH, Plain>(a, smem)) ranged_fwd_again<DH>((uint64_t)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr(), (lds_ptr)smem);
+  if (ranged_fwd_body<DH, KS, Plain>(a, smem)) ranged_fwd_again<DH, KS>((uint64_t)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr(), (lds_ptr)smem);
 }
 
 template <int DT>
@@ -403,11 +403,11 @@ __device__ __forceinline__ void put_rows_f32(float* op, const f32x16 (&acc)[DT],
 // causal documents, 20 over 5 heads of 64: 55 and 57 us).
 //
 // dQ and delta; also writes, for the second kernel, what the ranges of each 32 queries have in common
-template <int DH, class Form>
+template <int DH, int KS, class Form>
 __device__ __forceinline__ bool ranged_bwd_dq_body(const Ranged& a, char* smem) {
   constexpr bool GUARD = Form::guard;
   using T = Tile<DH>;
-  constexpr int KS = T::KS, DT = T::DT, NI = T::CPR / 4, STAGE = 2 * TB * T::ROW;
+  constexpr int DT = T::DT, NI = T::CPR / 4, STAGE = 2 * TB * T::ROW;
   int* span = (int*)(smem + 2 * STAGE);
 
   const int t = threadIdx.x, lane = t & 63;
@@ -566,15 +566,15 @@ __device__ __forceinline__ bool ranged_bwd_dq_body(const Ranged& a, char* smem) 
 }
 
 // the walk again, guarded: a call, so that its registers are not the kernel's
-template <int DH>
+template <int DH, int KS>
 __device__ __attribute__((noinline)) void ranged_bwd_dq_again(uint64_t args, lds_ptr smem) {
-  ranged_bwd_dq_body<DH, Guarded>(kernel_args(args), (char*)smem);
+  ranged_bwd_dq_body<DH, KS, Guarded>(kernel_args(args), (char*)smem);
 }
 
-template <int DH>
+template <int DH, int KS>
 __global__ __launch_bounds__(256, DH <= 64 ? 3 : DH <= 96 ? 2 : 1) void ranged_bwd_dq_kernel(const Ranged a) {
   __shared__ __attribute__((aligned(16))) char smem[2 * (2 * TB * Tile<DH>::ROW) + 64];
-  if (ranged_bwd_dq_body<DH, Plain>(a, smem)) ranged_bwd_dq_again<DH>((uint64_t)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr(), (lds_ptr)smem);
+  if (ranged_bwd_dq_body<DH, KS, Plain>(a, smem)) ranged_bwd_dq_again<DH, KS>((uint64_t)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr(), (lds_ptr)smem);
 }
 
 // Which (row of the batch, block of keys, key head, part of the walk) a workgroup of the key kernel takes: as block_of, ranked by
@@ -642,11 +642,11 @@ __device__ __forceinline__ void keys_of(const Ranged& a, char* smem, int& b, int
 
 // dK and dV of 128 keys (the heavier of the two per tile: four products, and dS and P as operands): walks the query tiles of every head that shares the key head.  With few workgroups the walk is cut
 // into `splits` parts whose sums are added afterwards in their order.
-template <int DH, class Form>
+template <int DH, int KS, class Form>
 __device__ __forceinline__ bool ranged_bwd_dkv_body(const Ranged& a, char* smem) {
   constexpr bool GUARD = Form::guard;
   using T = Tile<DH>;
-  constexpr int KS = T::KS, DT = T::DT, NI = T::CPR / 4, STAGE = 2 * TB * T::ROW + 4 * TB * 4;
+  constexpr int DT = T::DT, NI = T::CPR / 4, STAGE = 2 * TB * T::ROW + 4 * TB * 4;
   int* span = (int*)(smem + 2 * STAGE);
 
   const int t = threadIdx.x, lane = t & 63;
@@ -911,15 +911,15 @@ __device__ __forceinline__ bool ranged_bwd_dkv_body(const Ranged& a, char* smem)
 }
 
 // the walk again, guarded: a call, so that its registers are not the kernel's
-template <int DH>
+template <int DH, int KS>
 __device__ __attribute__((noinline)) void ranged_bwd_dkv_again(uint64_t args, lds_ptr smem) {
-  ranged_bwd_dkv_body<DH, Guarded>(kernel_args(args), (char*)smem);
+  ranged_bwd_dkv_body<DH, KS, Guarded>(kernel_args(args), (char*)smem);
 }
 
-template <int DH>
+template <int DH, int KS>
 __global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dkv_kernel(const Ranged a) {
   __shared__ __attribute__((aligned(16))) char smem[2 * (2 * TB * Tile<DH>::ROW + 4 * TB * 4) + 64];
-  if (ranged_bwd_dkv_body<DH, Plain>(a, smem)) ranged_bwd_dkv_again<DH>((uint64_t)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr(), (lds_ptr)smem);
+  if (ranged_bwd_dkv_body<DH, KS, Plain>(a, smem)) ranged_bwd_dkv_again<DH, KS>((uint64_t)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr(), (lds_ptr)smem);
 }
 
 // The interval of keys that each query of a packed, padded or generated batch sees (see lbmk_key_ranges)
@@ -1038,13 +1038,16 @@ Ranged ranged_args(const lbmk_ranged_attn_desc* p) {
   return a;
 }
 
-#define BY_HEAD(DHP, LAUNCH)     \
-  switch (DHP) {                 \
-    case 32: LAUNCH(32); break;  \
-    case 64: LAUNCH(64); break;  \
-    case 96: LAUNCH(96); break;  \
-    case 128: LAUNCH(128); break; \
-    default: LAUNCH(160); break; \
+// padded head width, and 16-channel steps of the products over the channels: heads of up to 80 leave out the sixth (2 x 4096 tokens,
+// 8 heads of 80 with a prefix: 100 -> 86 us forward, 290 -> 280 backward; a third instead of four steps for 40 gains nothing)
+#define BY_HEAD(D, LAUNCH)                \
+  switch (((D) + 15) / 16) {              \
+    case 1: case 2: LAUNCH(32, 2); break; \
+    case 3: case 4: LAUNCH(64, 4); break; \
+    case 5: LAUNCH(96, 5); break;         \
+    case 6: LAUNCH(96, 6); break;         \
+    case 7: case 8: LAUNCH(128, 8); break; \
+    default: LAUNCH(160, 10); break;      \
   }
 
 __global__ __launch_bounds__(256) void sum_splits_kernel(const float* __restrict__ part, bf16_t* dk, bf16_t* dv, int64_t n, int splits) {
@@ -1081,8 +1084,8 @@ extern "C" int lbmk_ranged_attn(const lbmk_ranged_attn_desc* p, void* stream) {
   hipStream_t s = (hipStream_t)stream;
   a.blocks = (a.Nq + RB - 1) / RB;
   order_blocks(a, fwd_occupancy(pad_head(a.D)));
-#define FWD(DHP) hipLaunchKernelGGL((ranged_fwd_kernel<DHP>), dim3((unsigned)((int64_t)a.blocks * a.parts * a.H * a.B)), dim3(256), 0, s, a)
-  BY_HEAD(pad_head(a.D), FWD)
+#define FWD(DHP, KSP) hipLaunchKernelGGL((ranged_fwd_kernel<DHP, KSP>), dim3((unsigned)((int64_t)a.blocks * a.parts * a.H * a.B)), dim3(256), 0, s, a)
+  BY_HEAD(a.D, FWD)
 #undef FWD
   return lbmk_check_launch("ranged_attn");
 }
@@ -1105,8 +1108,8 @@ extern "C" int lbmk_ranged_attn_bwd(const lbmk_ranged_attn_desc* p, void* stream
   hipStream_t s = (hipStream_t)stream;
   a.blocks = (a.Nq + RB - 1) / RB;
   order_blocks(a, dq_occupancy(pad_head(a.D)));
-#define DQ(DHP) hipLaunchKernelGGL((ranged_bwd_dq_kernel<DHP>), dim3((unsigned)((int64_t)a.blocks * a.parts * a.H * a.B)), dim3(256), 0, s, a)
-  BY_HEAD(pad_head(a.D), DQ)
+#define DQ(DHP, KSP) hipLaunchKernelGGL((ranged_bwd_dq_kernel<DHP, KSP>), dim3((unsigned)((int64_t)a.blocks * a.parts * a.H * a.B)), dim3(256), 0, s, a)
+  BY_HEAD(a.D, DQ)
 #undef DQ
   if (a.Nk > 0) {
     a.splits = dkv_splits(a.ranges != nullptr, a.B, a.H, a.Hk, a.Nq, a.Nk, a.D);
@@ -1115,8 +1118,8 @@ extern "C" int lbmk_ranged_attn_bwd(const lbmk_ranged_attn_desc* p, void* stream
     a.ordered = order_pays(a, n / 2) && a.D > 32 && kblocks * a.B <= ORDER_ITEMS / 2 && (int64_t)a.B * ((a.Nq + TB - 1) / TB) * 2 <= ORDER_GROUPS - 256;
     a.snake = n <= (a.D <= 96 ? 2ll : 1ll) * a.cus;
     a.part = (float*)(a.tiles + (int64_t)a.B * ((a.Nq + TB - 1) / TB) * 2);
-#define DKV(DHP) hipLaunchKernelGGL((ranged_bwd_dkv_kernel<DHP>), dim3((unsigned)((int64_t)((a.Nk + RB - 1) / RB) * a.Hk * a.B * a.splits)), dim3(256), 0, s, a)
-    BY_HEAD(pad_head(a.D), DKV)
+#define DKV(DHP, KSP) hipLaunchKernelGGL((ranged_bwd_dkv_kernel<DHP, KSP>), dim3((unsigned)((int64_t)((a.Nk + RB - 1) / RB) * a.Hk * a.B * a.splits)), dim3(256), 0, s, a)
+    BY_HEAD(a.D, DKV)
 #undef DKV
     if (a.splits > 1) {
       const int64_t all = (int64_t)a.B * a.Nk * a.Hk * a.D;
