@@ -3,15 +3,15 @@
 //   y[m] = x[m] W^T + bias + t[m] B_a^T          t[m] = s_a x[m] A_a^T          a = index[request of row m]
 //
 // The factor products are a few per cent of the shared one, so what costs is reading x again and every launch.  Two steps:
-//   * adapter_down: t, bf16 (its half step is relative to the adapter's own share of y).  16 rows x 32 ranks per workgroup on
-//     v_mfma_f32_16x16x32_bf16, both operands K-contiguous and read straight into registers; the four waves of a workgroup
+//   * adapter_down: t, bf16 (its half step is relative to the adapter's own share of y).  16 or 32 rows x 32 ranks per workgroup on
+//     v_mfma_f32_16x16x32_bf16, both operands K-contiguous and read straight into registers; the eight waves of a workgroup
 //     split K and are joined in LDS in a fixed order, because there are too few row groups to fill the chip otherwise.
 //   * the shared product with t B_a^T added to its accumulators before the one rounding of y: many rows in lbmk_igemm
 //     (lr_* fields), few rows here: the weight's bytes are the floor, so a workgroup of 8 waves takes
 //     16 output columns of 64 rows, its waves split K, and W goes from memory into MFMA operands without LDS.
 // Measured: 16 requests of one token, 1280 -> 1280, rank 16: 5.4 + 5.8 us, of which the weight's 3.3 MB are 0.7: latency of two
-// launches.  8 x 1024 rows, 1280 -> 3840, rank 32: adapter_down 10.6 us (21 MB, 2 TB/s: some 2048 workgroups of a few microseconds
-// each) before 87 us of the shared product with the factors (the product alone: 85 us).
+// launches.  8 x 1024 rows, 1280 -> 3840, rank 32: adapter_down 7.7 us (21 MB of x; the factor, 80 KB, is read from L2 by each of
+// 256 workgroups) before 87 us of the shared product with the factors (the product alone: 85 us).
 #include "common.h"
 
 namespace {
@@ -22,54 +22,64 @@ __device__ __forceinline__ bf16x8 zero8() {
 }
 
 // waves over K; groups of 16 ranks that share one reading of x (one group per workgroup: 12.3 us instead of 10.6 at rank 32)
-constexpr int DOWN_WAVES = 4, DOWN_GROUPS = 2;
+constexpr int DOWN_WAVES = 8, DOWN_GROUPS = 2;
 
-// grid: (columns of t / 32, ceil(rows / 16) * requests)
+// RG: groups of 16 rows that share one reading of the factor.  grid: (columns of t / 32, ceil(rows / (16 RG)) * requests)
+template <int RG>
 __global__ __launch_bounds__(64 * DOWN_WAVES) void adapter_down_kernel(const bf16_t* __restrict__ x, const bf16_t* __restrict__ down,
                                                                       const int32_t* __restrict__ index, const float* __restrict__ scaling,
                                                                       bf16_t* __restrict__ t, int rows, int K, int64_t ldx, int rank, int tk,
                                                                       int count) {
-  __shared__ f32x4 part[DOWN_WAVES][DOWN_GROUPS][64];
+  __shared__ f32x4 part[DOWN_WAVES][RG * DOWN_GROUPS][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 15, lq = lane >> 4;
-  const int groups = (rows + 15) / 16, request = blockIdx.y / groups, m0 = (blockIdx.y - request * groups) * 16, r0 = blockIdx.x * 32;
+  const int blocks = (rows + 16 * RG - 1) / (16 * RG), request = blockIdx.y / blocks, m0 = (blockIdx.y - request * blocks) * 16 * RG, r0 = blockIdx.x * 32;
   const int a = index[request];
   if ((unsigned)a >= (unsigned)count) return;                  // no adapter: nobody reads these rows of t
-  const int m = min(m0 + lr, rows - 1);
-  const bf16_t* xr = x + ((int64_t)request * rows + m) * ldx + 8 * lq;
-  const bf16_t* dr[DOWN_GROUPS];
+  const bf16_t *xr[RG], *dr[DOWN_GROUPS];
+#pragma unroll
+  for (int i = 0; i < RG; ++i) xr[i] = x + ((int64_t)request * rows + min(m0 + 16 * i + lr, rows - 1)) * ldx + 8 * lq;
 #pragma unroll
   for (int g = 0; g < DOWN_GROUPS; ++g) dr[g] = down + ((int64_t)a * rank + min(r0 + 16 * g + lr, rank - 1)) * K + 8 * lq;
   // K in chunks of 32: an equal, contiguous share per wave
   const int chunks = (K + 31) / 32, per = (chunks + DOWN_WAVES - 1) / DOWN_WAVES;
   const int c0 = wave * per, c1 = min(c0 + per, chunks);
-  f32x4 acc[DOWN_GROUPS];
+  f32x4 acc[RG][DOWN_GROUPS];
 #pragma unroll
-  for (int g = 0; g < DOWN_GROUPS; ++g) acc[g] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < RG; ++i)
+#pragma unroll
+    for (int g = 0; g < DOWN_GROUPS; ++g) acc[i][g] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 5
   for (int c = c0; c < c1; ++c) {
     const bool in = 32 * c + 8 * lq < K;                       // K % 8 == 0
-    const bf16x8 fx = in ? *(const bf16x8*)(xr + 32 * c) : zero8();
+    bf16x8 fx[RG];
+#pragma unroll
+    for (int i = 0; i < RG; ++i) fx[i] = in ? *(const bf16x8*)(xr[i] + 32 * c) : zero8();
 #pragma unroll
     for (int g = 0; g < DOWN_GROUPS; ++g) {
       const bf16x8 fd = in ? *(const bf16x8*)(dr[g] + 32 * c) : zero8();
-      acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fd, fx, acc[g], 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < RG; ++i) acc[i][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fd, fx[i], acc[i][g], 0, 0, 0);
     }
   }
 #pragma unroll
-  for (int g = 0; g < DOWN_GROUPS; ++g) part[wave][g][lane] = acc[g];
+  for (int i = 0; i < RG; ++i)
+#pragma unroll
+    for (int g = 0; g < DOWN_GROUPS; ++g) part[wave][i * DOWN_GROUPS + g][lane] = acc[i][g];
   __syncthreads();
-  if (wave >= DOWN_GROUPS || m0 + lr >= rows) return;
-  // wave g joins group g.  Lane: row m0 + lr, ranks 4 lq .. + 3 of the group; ranks from `rank` on are zeros
-  f32x4 v = part[0][wave][lane];
-#pragma unroll
-  for (int w = 1; w < DOWN_WAVES; ++w) v += part[w][wave][lane];
   const float s = scaling ? scaling[a] : 1.f;
-  const int n = r0 + 16 * wave + 4 * lq;
-  u16x4 o;
+  // a wave joins one group of ranks at a time.  Lane: row m0 + 16 i + lr, ranks 4 lq .. + 3 of the group; ranks from `rank` on are zeros
+  for (int j = wave; j < RG * DOWN_GROUPS; j += DOWN_WAVES) {
+    const int m = m0 + 16 * (j / DOWN_GROUPS) + lr, n = r0 + 16 * (j % DOWN_GROUPS) + 4 * lq;
+    if (m >= rows) continue;
+    f32x4 v = part[0][j][lane];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) o.v[e] = f2bf(n + e < rank ? v[e] * s : 0.f);
-  *(u16x4*)(t + ((int64_t)request * rows + m0 + lr) * tk + n) = o;
+    for (int w = 1; w < DOWN_WAVES; ++w) v += part[w][j][lane];
+    u16x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o.v[e] = f2bf(n + e < rank ? v[e] * s : 0.f);
+    *(u16x4*)(t + ((int64_t)request * rows + m) * tk + n) = o;
+  }
 }
 
 constexpr int FEW_WAVES = 8, FEW_ROWS = 64;       // rows of a workgroup
@@ -159,13 +169,20 @@ extern "C" int lbmk_adapter_down(const void* x, const void* down, const int32_t*
   const int64_t groups = (int64_t)requests * ((rows + 15) / 16);
   LBMK_REQUIRE(groups < (1ll << 31) && (int64_t)requests * rows < (1ll << 31), "adapter_down: too many rows");
   // (grid.y carries the row groups and is limited to 65535: larger batches go in slices of whole requests)
-  const int per = (rows + 15) / 16, most = 65535 / per;
+  // Two groups of rows per workgroup read the factor half as often, where that still leaves two workgroups per CU.  One against two,
+  // with eight waves: 8 requests of 1024 rows, K 1280, rank 32: 9.6 / 7.7 us; 2 of 4096, 640, 64: 9.7 / 7.6; 4 of 1024, 640, 16: 4.0 /
+  // 4.5; 20 of 33, 2560, 16: 8.0 / 10.3.  (Four groups: 10.1 us for the first.  Four waves: single tokens of K 1280 4.7 us instead of 4.3.)
+  const int rg = (int64_t)requests * ((rows + 15) / 16) >= 2ll * lbmk_num_cus() && rows > 16 ? 2 : 1, per = (rows + 16 * rg - 1) / (16 * rg), most = 65535 / per;
   LBMK_REQUIRE(most > 0, "adapter_down: %d rows per request (at most %d)", rows, 65535 * 16);
   for (int r = 0; r < requests; r += most) {
     const int n = requests - r < most ? requests - r : most;
-    hipLaunchKernelGGL(adapter_down_kernel, dim3(tk / 32, n * per), dim3(64 * DOWN_WAVES), 0, (hipStream_t)stream,
-                       (const bf16_t*)x + (int64_t)r * rows * ldx, (const bf16_t*)down, index + r, scaling, (bf16_t*)t + (int64_t)r * rows * tk, rows, K,
-                       ldx, rank, tk, count);
+#define DOWN(RG)                                                                                                                          \
+  hipLaunchKernelGGL((adapter_down_kernel<RG>), dim3(tk / 32, n * per), dim3(64 * DOWN_WAVES), 0, (hipStream_t)stream,                     \
+                     (const bf16_t*)x + (int64_t)r * rows * ldx, (const bf16_t*)down, index + r, scaling, (bf16_t*)t + (int64_t)r * rows * tk, rows, K, \
+                     ldx, rank, tk, count)
+    if (rg > 1) DOWN(2);
+    else DOWN(1);
+#undef DOWN
   }
   return lbmk_check_launch("adapter_down");
 }
