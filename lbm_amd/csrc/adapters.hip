@@ -11,7 +11,7 @@
 //     16 output columns of 64 rows, its waves split K, and W goes from memory into MFMA operands without LDS.
 // Measured: 16 requests of one token, 1280 -> 1280, rank 16: 5.4 + 5.8 us, of which the weight's 3.3 MB are 0.7: latency of two
 // launches.  8 x 1024 rows, 1280 -> 3840, rank 32: adapter_down 7.7 us (21 MB of x; the factor, 80 KB, is read from L2 by each of
-// 256 workgroups) before 87 us of the shared product with the factors (the product alone: 85 us).
+// 256 workgroups), the whole call 86.5, the shared product alone 75.5.
 #include "common.h"
 
 namespace {
