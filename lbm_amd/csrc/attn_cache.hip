@@ -75,7 +75,7 @@ __global__ __launch_bounds__(256) void cached_attn_kernel(const Cached a) {
   const bf16_t* V = a.v + b * a.sv + (int64_t)khead * a.D;
   bf16x8 qf[KS];
   load_frags<KS>(a.q + b * a.sq + (int64_t)tok * a.ldq + (int64_t)head * a.D, h, a.D, qf);
-  const float slope = a.map.biased ? a.slopes[head] * 1.4426950408889634f : 0.f;
+  const float slope = a.map.biased ? a.slopes[head] * a.map.slope : 0.f;
 
   f32x16 o[DT];
 #pragma unroll
@@ -322,6 +322,7 @@ extern "C" int lbmk_cached_attn(const lbmk_cached_attn_desc* p, void* stream) {
   a.map.cap_in = p->cap > 0.f ? 2.f * p->scale * log2e / p->cap : 0.f;
   a.map.cap_out = p->cap * log2e;
   a.map.biased = p->slopes != nullptr;
+  a.map.slope = log2e;
   a.map.mul = p->cap > 0.f || p->slopes ? 1.f : a.map.scale;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)((int64_t)a.B * a.Hk * a.row_blocks), a.splits);

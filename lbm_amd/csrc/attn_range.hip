@@ -14,15 +14,21 @@
 //
 // Bound by the vector ALU beside the matrix cores: a score costs 4 D operations of matrix work forward, and an exp2 (a quarter of
 // the rate), a fused multiply-add, a maximum, an addition and half a conversion of vector work, as long again at 64 channels; the
-// tiles come from L2.  Measured, 2 x 4096 tokens, 20 heads of 64: all keys 220 us forward (780 TFLOP/s; the operand layouts alone
-// would allow some 1100), 780 us backward (550 TFLOP/s of its 5 products); causal 122 (700) and 421 us.  8 heads of 128, causal:
-// 108 us (640), 393 us.  (A library product of 8192^3 reaches 1380 TFLOP/s on the same card.)
+// tiles come from L2.  Measured, 2 x 4096 tokens, 20 heads of 64: all keys 207 us forward (830 TFLOP/s), 715 us backward (600 TFLOP/s of its
+// 5 products); causal 122 (700) and 386 us.  8 heads of 128, causal: 102 us (670), 366 us.  (A library product of 8192^3 reaches 1380 TFLOP/s on the same card.)
 #include "attn_tile.h"
 
 namespace {
 
 constexpr int RB = 128;   // rows (queries or keys) of a workgroup
 constexpr int TB = 64;    // tokens per tile of the walked operand
+
+// How a product becomes a score: as it is; with a bias, which the product's accumulators start from (two operations per score instead
+// of three); capped (and then biased where slopes are given).  A kernel of its own for each: as uniform branches in one kernel they
+// cost registers and scheduling.  2 x 4096 tokens, 20 heads of 64, forward / backward, one kernel against three: plain 207 / 740 us
+// against 207 / 715, with a bias 234 / 779 against 214 / 725, with a cap 286 / 1004 against 281 / 971; 8 heads of 128, causal, 104 / 394
+// against 102 / 366.  (Forward, causal, plain, 64 channels alone gets slower, 117 -> 122 us.)
+constexpr int LINEAR = 0, BIASED = 1, CAPPED = 2;
 
 typedef __attribute__((address_space(3))) char* lds_ptr;
 
@@ -174,7 +180,7 @@ __device__ __forceinline__ bool any_wave(bool x, int wave, int* sm) {
   return __builtin_amdgcn_readfirstlane(sm[0] | sm[1] | sm[2] | sm[3]) != 0;
 }
 
-template <int DH, int KS, class Form>
+template <int DH, int KS, int MAP, class Form>
 __device__ __forceinline__ bool ranged_fwd_body(const Ranged& a, char* smem) {
   constexpr bool GUARD = Form::guard;
   using T = Tile<DH>;
@@ -198,7 +204,7 @@ __device__ __forceinline__ bool ranged_fwd_body(const Ranged& a, char* smem) {
 
   bf16x8 qf[KS];
   load_frags<KS>(a.q + b * a.sq + (int64_t)qr * a.ldq + (int64_t)head * a.D, h, a.D, qf);
-  const float slope = a.map.biased ? a.slopes[head] * 1.4426950408889634f : 0.f;
+  const float slope = MAP != LINEAR && a.map.biased ? a.slopes[head] * a.map.slope : 0.f;
   const int pos = qr + a.Nk - a.Nq;
   const unsigned len = mine ? (unsigned)max(range.y - range.x, 0) : 0u;
 
@@ -240,12 +246,22 @@ __device__ __forceinline__ bool ranged_fwd_body(const Ranged& a, char* smem) {
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
       const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      auto product = [&](const f32x16& from) __attribute__((always_inline)) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sK + kt * 32 * T::ROW, T::row_at(kr, ks)), qf[ks], ks == 0 ? zero : s[kt], 0, 0, 0);
+        for (int ks = 0; ks < KS; ++ks)
+          s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sK + kt * 32 * T::ROW, T::row_at(kr, ks)), qf[ks], ks == 0 ? from : s[kt], 0, 0, 0);
+      };
+      if constexpr (MAP == BIASED) {
+        f32x16 c;
+        const float d0 = (float)(pos - kv0 - 4 * h);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) c[e] = -slope * fabsf(d0 - (float)(32 * kt + acc_row(e, 0)));
+        product(c);
+      } else {
+        product(zero);
+      }
     }
-    if (a.map.cap_out != 0.f) {
-      asm volatile("" ::: "memory");           // (keeps these uniform conditions branches)
+    if constexpr (MAP == CAPPED) {
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -253,18 +269,17 @@ __device__ __forceinline__ bool ranged_fwd_body(const Ranged& a, char* smem) {
           const float x = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[kt][e] * a.map.cap_in) + 1.f);
           s[kt][e] = fmaf(-2.f * a.map.cap_out, x, a.map.cap_out);
         }
-    }
-    if (a.map.biased) {
-      asm volatile("" ::: "memory");
-      const float f = a.map.cap_out != 0.f ? 1.f : a.map.scale;
-      const float d0 = (float)(pos - kv0 - 4 * h);
+      if (a.map.biased) {
+        asm volatile("" ::: "memory");
+        const float d0 = (float)(pos - kv0 - 4 * h);
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+        for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[kt][e] = fmaf(-slope, fabsf(d0 - (float)(32 * kt + acc_row(e, 0))), s[kt][e] * f);
+          for (int e = 0; e < 16; ++e) s[kt][e] = fmaf(-slope, fabsf(d0 - (float)(32 * kt + acc_row(e, 0))), s[kt][e]);
+      }
     }
     if (masked) {
-      asm volatile("" ::: "memory");
+      asm volatile("" ::: "memory");           // (keeps the uniform condition a branch)
       const unsigned k0 = (unsigned)(kv0 + 4 * h - range.x);
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
@@ -355,15 +370,15 @@ __device__ __forceinline__ bool ranged_fwd_body(const Ranged& a, char* smem) {
 }
 
 // the walk again, guarded: a call, so that its registers are not the kernel's
-template <int DH, int KS>
+template <int DH, int KS, int MAP>
 __device__ __attribute__((noinline)) void ranged_fwd_again(uint64_t args, lds_ptr smem) {
-  ranged_fwd_body<DH, KS, Guarded>(kernel_args(args), (char*)smem);
+  ranged_fwd_body<DH, KS, MAP, Guarded>(kernel_args(args), (char*)smem);
 }
 
-template <int DH, int KS>
+template <int DH, int KS, int MAP>
 __global__ __launch_bounds__(256, DH <= 96 ? 3 : DH <= 128 ? 2 : 1) void ranged_fwd_kernel(const Ranged a) {
   __shared__ __attribute__((aligned(16))) char smem[2 * (2 * TB * Tile<DH>::ROW) + 64];
-  if (ranged_fwd_body<DH, KS, Plain>(a, smem)) ranged_fwd_again<DH, KS>((uint64_t)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr(), (lds_ptr)smem);
+  if (ranged_fwd_body<DH, KS, MAP, Plain>(a, smem)) ranged_fwd_again<DH, KS, MAP>((uint64_t)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr(), (lds_ptr)smem);
 }
 
 template <int DT>
@@ -403,7 +418,7 @@ __device__ __forceinline__ void put_rows_f32(float* op, const f32x16 (&acc)[DT],
 // causal documents, 20 over 5 heads of 64: 55 and 57 us).
 //
 // dQ and delta; also writes, for the second kernel, what the ranges of each 32 queries have in common
-template <int DH, int KS, class Form>
+template <int DH, int KS, int MAP, class Form>
 __device__ __forceinline__ bool ranged_bwd_dq_body(const Ranged& a, char* smem) {
   constexpr bool GUARD = Form::guard;
   using T = Tile<DH>;
@@ -455,7 +470,7 @@ __device__ __forceinline__ bool ranged_bwd_dq_body(const Ranged& a, char* smem) 
     if (q < a.Nq && mine && h == 0) a.delta[stat] = delta;
   }
   const float nl = -a.lse[stat];
-  const float slope = a.map.biased ? a.slopes[head] * 1.4426950408889634f : 0.f;
+  const float slope = MAP != LINEAR && a.map.biased ? a.slopes[head] * a.map.slope : 0.f;
   const int pos = qr + a.Nk - a.Nq;
   const unsigned len = mine ? (unsigned)max(range.y - range.x, 0) : 0u;
 
@@ -494,29 +509,37 @@ __device__ __forceinline__ bool ranged_bwd_dq_body(const Ranged& a, char* smem) 
     for (int kt = 0; kt < 2; ++kt) {
       const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       f32x16 s, dp;
+      const float d0 = (float)(pos - kv0 - 32 * kt - 4 * h);
+      auto product = [&](const f32x16& from) __attribute__((always_inline)) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sK + kt * 32 * T::ROW, T::row_at(kr, ks)), qf[ks], ks == 0 ? zero : s, 0, 0, 0);
+        for (int ks = 0; ks < KS; ++ks)
+          s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sK + kt * 32 * T::ROW, T::row_at(kr, ks)), qf[ks], ks == 0 ? from : s, 0, 0, 0);
+      };
+      if constexpr (MAP == BIASED) {
+        f32x16 c;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) c[e] = -slope * fabsf(d0 - (float)acc_row(e, 0));
+        product(c);
+      } else {
+        product(zero);
+      }
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
         dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sV + kt * 32 * T::ROW, T::row_at(kr, ks)), gf[ks], ks == 0 ? zero : dp, 0, 0, 0);
 #pragma unroll
       for (int e = 0; e < 16; ++e) dp[e] -= delta;
-      if (a.map.cap_out != 0.f) {
-        asm volatile("" ::: "memory");
+      if constexpr (MAP == CAPPED) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const float x = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[e] * a.map.cap_in) + 1.f);
           s[e] = fmaf(-2.f * a.map.cap_out, x, a.map.cap_out);
           dp[e] *= 4.f * x * (1.f - x);                       // 1 - tanh^2
         }
-      }
-      if (a.map.biased) {
-        asm volatile("" ::: "memory");
-        const float f = a.map.cap_out != 0.f ? 1.f : a.map.scale;
-        const float d0 = (float)(pos - kv0 - 32 * kt - 4 * h);
+        if (a.map.biased) {
+          asm volatile("" ::: "memory");
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = fmaf(-slope, fabsf(d0 - (float)acc_row(e, 0)), s[e] * f);
+          for (int e = 0; e < 16; ++e) s[e] = fmaf(-slope, fabsf(d0 - (float)acc_row(e, 0)), s[e]);
+        }
       }
       float ds[16];
 #pragma unroll
@@ -566,15 +589,15 @@ __device__ __forceinline__ bool ranged_bwd_dq_body(const Ranged& a, char* smem) 
 }
 
 // the walk again, guarded: a call, so that its registers are not the kernel's
-template <int DH, int KS>
+template <int DH, int KS, int MAP>
 __device__ __attribute__((noinline)) void ranged_bwd_dq_again(uint64_t args, lds_ptr smem) {
-  ranged_bwd_dq_body<DH, KS, Guarded>(kernel_args(args), (char*)smem);
+  ranged_bwd_dq_body<DH, KS, MAP, Guarded>(kernel_args(args), (char*)smem);
 }
 
-template <int DH, int KS>
+template <int DH, int KS, int MAP>
 __global__ __launch_bounds__(256, DH <= 64 ? 3 : DH <= 96 ? 2 : 1) void ranged_bwd_dq_kernel(const Ranged a) {
   __shared__ __attribute__((aligned(16))) char smem[2 * (2 * TB * Tile<DH>::ROW) + 64];
-  if (ranged_bwd_dq_body<DH, KS, Plain>(a, smem)) ranged_bwd_dq_again<DH, KS>((uint64_t)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr(), (lds_ptr)smem);
+  if (ranged_bwd_dq_body<DH, KS, MAP, Plain>(a, smem)) ranged_bwd_dq_again<DH, KS, MAP>((uint64_t)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr(), (lds_ptr)smem);
 }
 
 // Which (row of the batch, block of keys, key head, part of the walk) a workgroup of the key kernel takes: as block_of, ranked by
@@ -642,7 +665,7 @@ __device__ __forceinline__ void keys_of(const Ranged& a, char* smem, int& b, int
 
 // dK and dV of 128 keys (the heavier of the two per tile: four products, and dS and P as operands): walks the query tiles of every head that shares the key head.  With few workgroups the walk is cut
 // into `splits` parts whose sums are added afterwards in their order.
-template <int DH, int KS, class Form>
+template <int DH, int KS, int MAP, class Form>
 __device__ __forceinline__ bool ranged_bwd_dkv_body(const Ranged& a, char* smem) {
   constexpr bool GUARD = Form::guard;
   using T = Tile<DH>;
@@ -790,7 +813,7 @@ __device__ __forceinline__ bool ranged_bwd_dkv_body(const Ranged& a, char* smem)
     cur ^= 1;
     if (left > 1) stage(j, smem + cur * STAGE);
     const int qt = i.tile;
-    if (a.map.biased && head != i.head) slope = a.slopes[khead * group + i.head] * 1.4426950408889634f;
+    if (MAP != LINEAR && a.map.biased && head != i.head) slope = a.slopes[khead * group + i.head] * a.map.slope;
     head = i.head;
     const Seen now = x;
     i = j;
@@ -807,9 +830,20 @@ __device__ __forceinline__ bool ranged_bwd_dkv_body(const Ranged& a, char* smem)
       }
       const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       f32x16 s, dp;
+      const float d0 = (float)(qt * TB + 32 * u + 4 * h + a.Nk - a.Nq - kc);
+      auto product = [&](const f32x16& from) __attribute__((always_inline)) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sQ + u * 32 * T::ROW, T::row_at(rr, ks)), kf[ks], ks == 0 ? zero : s, 0, 0, 0);
+        for (int ks = 0; ks < KS; ++ks)
+          s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sQ + u * 32 * T::ROW, T::row_at(rr, ks)), kf[ks], ks == 0 ? from : s, 0, 0, 0);
+      };
+      if constexpr (MAP == BIASED) {
+        f32x16 c;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) c[e] = -slope * fabsf(d0 + (float)acc_row(e, 0));
+        product(c);
+      } else {
+        product(zero);
+      }
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
         dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sG + u * 32 * T::ROW, T::row_at(rr, ks)), vf[ks], ks == 0 ? zero : dp, 0, 0, 0);
@@ -819,21 +853,18 @@ __device__ __forceinline__ bool ranged_bwd_dkv_body(const Ranged& a, char* smem)
 #pragma unroll
         for (int e = 0; e < 4; ++e) dp[4 * g + e] -= d4[e];
       }
-      if (a.map.cap_out != 0.f) {
-        asm volatile("" ::: "memory");
+      if constexpr (MAP == CAPPED) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const float x = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[e] * a.map.cap_in) + 1.f);
           s[e] = fmaf(-2.f * a.map.cap_out, x, a.map.cap_out);
           dp[e] *= 4.f * x * (1.f - x);
         }
-      }
-      if (a.map.biased) {
-        asm volatile("" ::: "memory");
-        const float f = a.map.cap_out != 0.f ? 1.f : a.map.scale;
-        const float d0 = (float)(qt * TB + 32 * u + 4 * h + a.Nk - a.Nq - kc);
+        if (a.map.biased) {
+          asm volatile("" ::: "memory");
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = fmaf(-slope, fabsf(d0 + (float)acc_row(e, 0)), s[e] * f);
+          for (int e = 0; e < 16; ++e) s[e] = fmaf(-slope, fabsf(d0 + (float)acc_row(e, 0)), s[e]);
+        }
       }
       float p[16], ds[16];
 #pragma unroll
@@ -911,15 +942,15 @@ __device__ __forceinline__ bool ranged_bwd_dkv_body(const Ranged& a, char* smem)
 }
 
 // the walk again, guarded: a call, so that its registers are not the kernel's
-template <int DH, int KS>
+template <int DH, int KS, int MAP>
 __device__ __attribute__((noinline)) void ranged_bwd_dkv_again(uint64_t args, lds_ptr smem) {
-  ranged_bwd_dkv_body<DH, KS, Guarded>(kernel_args(args), (char*)smem);
+  ranged_bwd_dkv_body<DH, KS, MAP, Guarded>(kernel_args(args), (char*)smem);
 }
 
-template <int DH, int KS>
+template <int DH, int KS, int MAP>
 __global__ __launch_bounds__(256, DH <= 96 ? 2 : 1) void ranged_bwd_dkv_kernel(const Ranged a) {
   __shared__ __attribute__((aligned(16))) char smem[2 * (2 * TB * Tile<DH>::ROW + 4 * TB * 4) + 64];
-  if (ranged_bwd_dkv_body<DH, KS, Plain>(a, smem)) ranged_bwd_dkv_again<DH, KS>((uint64_t)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr(), (lds_ptr)smem);
+  if (ranged_bwd_dkv_body<DH, KS, MAP, Plain>(a, smem)) ranged_bwd_dkv_again<DH, KS, MAP>((uint64_t)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr(), (lds_ptr)smem);
 }
 
 // The interval of keys that each query of a packed, padded or generated batch sees (see lbmk_key_ranges)
@@ -1034,21 +1065,27 @@ Ranged ranged_args(const lbmk_ranged_attn_desc* p) {
   a.map.cap_in = p->cap > 0.f ? 2.f * p->scale * log2e / p->cap : 0.f;
   a.map.cap_out = p->cap * log2e;
   a.map.biased = p->slopes != nullptr;
-  a.map.mul = p->cap > 0.f || p->slopes ? 1.f : a.map.scale;
+  // without a cap the bias is in units of q.k: the product starts from it
+  a.map.slope = p->cap > 0.f ? log2e : 1.f / p->scale;
+  a.map.mul = p->cap > 0.f ? 1.f : a.map.scale;
   return a;
 }
 
 // padded head width, and 16-channel steps of the products over the channels: heads of up to 80 leave out the sixth (2 x 4096 tokens,
 // 8 heads of 80 with a prefix: 100 -> 86 us forward, 290 -> 280 backward; a third instead of four steps for 40 gains nothing)
-#define BY_HEAD(D, LAUNCH)                \
+#define BY_HEAD(D, LAUNCH, MAP)           \
   switch (((D) + 15) / 16) {              \
-    case 1: case 2: LAUNCH(32, 2); break; \
-    case 3: case 4: LAUNCH(64, 4); break; \
-    case 5: LAUNCH(96, 5); break;         \
-    case 6: LAUNCH(96, 6); break;         \
-    case 7: case 8: LAUNCH(128, 8); break; \
-    default: LAUNCH(160, 10); break;      \
+    case 1: case 2: LAUNCH(32, 2, MAP); break; \
+    case 3: case 4: LAUNCH(64, 4, MAP); break; \
+    case 5: LAUNCH(96, 5, MAP); break;         \
+    case 6: LAUNCH(96, 6, MAP); break;         \
+    case 7: case 8: LAUNCH(128, 8, MAP); break; \
+    default: LAUNCH(160, 10, MAP); break;      \
   }
+#define BY_MAP(LAUNCH)                                              \
+  if (a.map.cap_out != 0.f) { BY_HEAD(a.D, LAUNCH, CAPPED) }        \
+  else if (a.map.biased) { BY_HEAD(a.D, LAUNCH, BIASED) }           \
+  else { BY_HEAD(a.D, LAUNCH, LINEAR) }
 
 __global__ __launch_bounds__(256) void sum_splits_kernel(const float* __restrict__ part, bf16_t* dk, bf16_t* dv, int64_t n, int splits) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;       // n is a multiple of 8
@@ -1084,8 +1121,8 @@ extern "C" int lbmk_ranged_attn(const lbmk_ranged_attn_desc* p, void* stream) {
   hipStream_t s = (hipStream_t)stream;
   a.blocks = (a.Nq + RB - 1) / RB;
   order_blocks(a, fwd_occupancy(pad_head(a.D)));
-#define FWD(DHP, KSP) hipLaunchKernelGGL((ranged_fwd_kernel<DHP, KSP>), dim3((unsigned)((int64_t)a.blocks * a.parts * a.H * a.B)), dim3(256), 0, s, a)
-  BY_HEAD(a.D, FWD)
+#define FWD(DHP, KSP, MAPP) hipLaunchKernelGGL((ranged_fwd_kernel<DHP, KSP, MAPP>), dim3((unsigned)((int64_t)a.blocks * a.parts * a.H * a.B)), dim3(256), 0, s, a)
+  BY_MAP(FWD)
 #undef FWD
   return lbmk_check_launch("ranged_attn");
 }
@@ -1108,8 +1145,8 @@ extern "C" int lbmk_ranged_attn_bwd(const lbmk_ranged_attn_desc* p, void* stream
   hipStream_t s = (hipStream_t)stream;
   a.blocks = (a.Nq + RB - 1) / RB;
   order_blocks(a, dq_occupancy(pad_head(a.D)));
-#define DQ(DHP, KSP) hipLaunchKernelGGL((ranged_bwd_dq_kernel<DHP, KSP>), dim3((unsigned)((int64_t)a.blocks * a.parts * a.H * a.B)), dim3(256), 0, s, a)
-  BY_HEAD(a.D, DQ)
+#define DQ(DHP, KSP, MAPP) hipLaunchKernelGGL((ranged_bwd_dq_kernel<DHP, KSP, MAPP>), dim3((unsigned)((int64_t)a.blocks * a.parts * a.H * a.B)), dim3(256), 0, s, a)
+  BY_MAP(DQ)
 #undef DQ
   if (a.Nk > 0) {
     a.splits = dkv_splits(a.ranges != nullptr, a.B, a.H, a.Hk, a.Nq, a.Nk, a.D);
@@ -1118,8 +1155,8 @@ extern "C" int lbmk_ranged_attn_bwd(const lbmk_ranged_attn_desc* p, void* stream
     a.ordered = order_pays(a, n / 2) && a.D > 32 && kblocks * a.B <= ORDER_ITEMS / 2 && (int64_t)a.B * ((a.Nq + TB - 1) / TB) * 2 <= ORDER_GROUPS - 256;
     a.snake = n <= (a.D <= 96 ? 2ll : 1ll) * a.cus;
     a.part = (float*)(a.tiles + (int64_t)a.B * ((a.Nq + TB - 1) / TB) * 2);
-#define DKV(DHP, KSP) hipLaunchKernelGGL((ranged_bwd_dkv_kernel<DHP, KSP>), dim3((unsigned)((int64_t)((a.Nk + RB - 1) / RB) * a.Hk * a.B * a.splits)), dim3(256), 0, s, a)
-    BY_HEAD(a.D, DKV)
+#define DKV(DHP, KSP, MAPP) hipLaunchKernelGGL((ranged_bwd_dkv_kernel<DHP, KSP, MAPP>), dim3((unsigned)((int64_t)((a.Nk + RB - 1) / RB) * a.Hk * a.B * a.splits)), dim3(256), 0, s, a)
+    BY_MAP(DKV)
 #undef DKV
     if (a.splits > 1) {
       const int64_t all = (int64_t)a.B * a.Nk * a.Hk * a.D;

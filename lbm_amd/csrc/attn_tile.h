@@ -157,12 +157,13 @@ __device__ __forceinline__ int wave_max_i(int v) {
 
 // What turns a product q.k into the exponent (base 2) of the softmax:
 //   cap:  C tanh(scale q.k / cap), C = cap log2(e), tanh(x) = 1 - 2 / (exp(2 x) + 1)        bias: - slope |distance|
-// Without either the scaling is left to the fused multiply-add that subtracts the maximum.
+// Without a cap the scaling is left to the fused multiply-add that subtracts the maximum.
 struct ScoreMap {
-  float mul;        // factor still to be applied to a mapped score (scale * log2(e), or 1 when cap or bias already did)
+  float mul;        // factor still to be applied to a mapped score (scale * log2(e), or 1 when it is already in that unit)
   float scale;      // scale * log2(e)
   float cap_in;     // 2 scale log2(e) / cap
   float cap_out;    // cap log2(e); 0: no cap
+  float slope;      // factor of the slopes, in the units that the bias is added in
   int biased;
 };
 
