@@ -270,6 +270,7 @@ int lbmk_flash_attn_bwd(const void* q, const void* qt, const void* k, const void
  *   rest       : bf16 [B][Nq][H*D], what rounding took from o: written forward, read backward, where it halves the error of
  *                rowsum(dout * o) and with it a third of dq's and dk's (NULL: not wanted)
  *   scratch    : backward only, lbmk_ranged_attn_bwd_scratch_floats(...) floats, 16-byte aligned
+ *   Without queries (B or Nq 0) nothing is written: dk and dv are then the caller's to clear.
  * What an operand holds at places that a query does not see has no influence on its row, inf and NaN included; a value that is not
  * finite at a place it does see makes the sums it enters not finite (NaN).
  * D: 8 ... 160, a multiple of 8.  Any Nq, Nk.  Batch strides (elements): sq, sk, sv, so, sg.  scale > 0.
