@@ -72,10 +72,10 @@ __device__ __forceinline__ int2 row_range(const Ranged& a, int b, int q) {
 //
 // Documents and causal masks give the blocks very different numbers of keys, and a launch is often no more workgroups than the
 // chip holds at once: in any fixed order some CUs get three long ones and others three short ones.  So, over long rows and with up
-// to 512 items (order_blocks), every workgroup ranks them by the span of keys that a few of their queries see (ties by index: a permutation, whatever the
-// ranges are) and takes the item of its own rank: the longest first.  Where the chip holds the whole launch at once (snake), every
-// other round of CUs backwards, so that a CU with a long one gets a short one beside it; otherwise the next longest goes to the
-// CU that is done first, as it should.
+// to 512 items (order_blocks), every workgroup ranks them by the span of keys that a few of their queries see (ties by index: a
+// permutation, whatever the ranges are) and takes the item of its own rank: the longest first.  Where the chip holds the whole
+// launch at once (snake), every other round of CUs backwards, so that a CU with a long one gets a short one beside it; otherwise
+// the next longest goes to the CU that is done first, as it should.
 // (All LDS of a kernel is one array: with a second object the compiler waits for the tile loads in flight before it reads it.)
 constexpr int ORDER_ITEMS = 512;
 __device__ __forceinline__ void block_of(const Ranged& a, int* key, int& b, int& qb, int& part, int& head) {
@@ -118,7 +118,8 @@ __device__ __forceinline__ void block_of(const Ranged& a, int* key, int& b, int&
       if (rank == id / a.H) taken = t;
     }
     __syncthreads();
-    const int item = __builtin_amdgcn_readfirstlane(taken);
+    // (bounded: ranges that another stream changes meanwhile are no permutation, and must not lead out of the operands)
+    const int item = min(max(__builtin_amdgcn_readfirstlane(taken), 0), items - 1);
     part = item >= half;
     const int it = part ? item - half : item;
     b = it / a.blocks;
@@ -644,7 +645,7 @@ __device__ __forceinline__ void keys_of(const Ranged& a, char* smem, int& b, int
       if (rank == id / (a.Hk * a.splits)) taken = t;
     }
     __syncthreads();
-    const int item = __builtin_amdgcn_readfirstlane(taken), rest = id % (a.Hk * a.splits);
+    const int item = min(max(__builtin_amdgcn_readfirstlane(taken), 0), items - 1), rest = id % (a.Hk * a.splits);
     __syncthreads();                      // (the tiles go over it)
     b = item / blocks;
     kb = item - b * blocks;
