@@ -173,12 +173,16 @@ __device__ __forceinline__ Walk walk_of(int2 r, bool mine, int wave, int* sm) {
   return w;
 }
 
-// whether a wave of the workgroup says so (and every wave is done with what it did before)
+// whether a wave of the workgroup says so (and every wave is done with what it did before).  The last barrier: a wave that has
+// the answer starts the second walk, whose walk_of writes the same words, and a wave that had not read them yet would take its
+// own way out, its share of the tiles unstaged.
 __device__ __forceinline__ bool any_wave(bool x, int wave, int* sm) {
   __syncthreads();
   if ((threadIdx.x & 63) == 0) sm[wave] = x;
   __syncthreads();
-  return __builtin_amdgcn_readfirstlane(sm[0] | sm[1] | sm[2] | sm[3]) != 0;
+  const bool any = __builtin_amdgcn_readfirstlane(sm[0] | sm[1] | sm[2] | sm[3]) != 0;
+  __syncthreads();
+  return any;
 }
 
 template <int DH, int KS, int MAP, class Form>
