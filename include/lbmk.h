@@ -273,7 +273,8 @@ int lbmk_flash_attn_bwd(const void* q, const void* qt, const void* k, const void
  *   Without queries (B or Nq 0) nothing is written: dk and dv are then the caller's to clear.
  * What an operand holds at places that a query does not see has no influence on its row, inf and NaN included; a value that is not
  * finite at a place it does see makes the sums it enters not finite (NaN).
- * D: 8 ... 160, a multiple of 8.  Any Nq, Nk.  Batch strides (elements): sq, sk, sv, so, sg.  scale > 0.
+ * D: 8 ... 160, a multiple of 8.  Any Nq, Nk.  Batch strides (elements): sq, sk, sv, so, sg.
+ * scale: 2^-126 ... 2^126; cap: 0, or 2^-126 ... 2^126 and at least 3 scale 2^-126.
  * ---------------------------------------------------------------------- */
 typedef struct lbmk_ranged_attn_desc {
   const void *q, *k, *v, *dout;

@@ -123,10 +123,13 @@ __global__ __launch_bounds__(256) void cached_attn_kernel(const Cached a) {
       s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sK, T::row_at(kr, ks)), qf[ks], ks == 0 ? zero : s, 0, 0, 0);
     if (a.map.cap_out != 0.f) {
       asm volatile("" ::: "memory");
+      float x;
+      if (a.map.cap_out <= CAP_FAR * 1.4426950408889634f) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float x = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[e] * a.map.cap_in) + 1.f);
-        s[e] = fmaf(-2.f * a.map.cap_out, x, a.map.cap_out);
+        for (int e = 0; e < 16; ++e) s[e] = capped<false>(a.map, s[e], x);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = capped<true>(a.map, s[e], x);
       }
     }
     if (a.map.biased) {
@@ -294,7 +297,8 @@ extern "C" int lbmk_cached_attn(const lbmk_cached_attn_desc* p, void* stream) {
   LBMK_REQUIRE(p->H > 0 && p->Hk > 0 && p->H % p->Hk == 0, "cached_attn: %d heads over %d key heads", p->H, p->Hk);
   LBMK_REQUIRE(p->B >= 0 && p->n >= 0 && p->cap_rows >= 0 && p->cap_rows < (1 << 30) && p->window >= 0, "cached_attn: sizes");
   LBMK_REQUIRE((int64_t)p->B * p->H * p->n < (1ll << 31) && (int64_t)p->n * (p->H / p->Hk) < (1 << 30), "cached_attn: too many rows");
-  LBMK_REQUIRE(p->scale > 0.f && p->cap >= 0.f, "cached_attn: scale %g, cap %g", (double)p->scale, (double)p->cap);
+  Cached a = {};
+  LBMK_REQUIRE(score_map(p->scale, p->cap, a.map), "cached_attn: scale %g, cap %g", (double)p->scale, (double)p->cap);
   if (p->B == 0 || p->n == 0) return LBMK_OK;
   LBMK_REQUIRE(p->q && p->o && p->lens && (p->cap_rows == 0 || (p->k && p->v)), "cached_attn: null pointer");
   LBMK_REQUIRE(lbmk_aligned(p->q, 16) && lbmk_aligned(p->k, 16) && lbmk_aligned(p->v, 16) && lbmk_aligned(p->o, 2) && lbmk_aligned(p->lens, 4) &&
@@ -304,7 +308,6 @@ extern "C" int lbmk_cached_attn(const lbmk_cached_attn_desc* p, void* stream) {
   for (int i = 0; i < 3; ++i)
     LBMK_REQUIRE(ld[i] % 8 == 0 && ld[i] >= (i ? p->Hk : p->H) * p->D && ld[i] <= (1 << 22) && st[i] % 8 == 0 && st[i] >= 0,
                  "cached_attn: row stride %d, batch stride %lld", ld[i], (long long)st[i]);
-  Cached a = {};
   a.q = (const bf16_t*)p->q; a.k = (const bf16_t*)p->k; a.v = (const bf16_t*)p->v; a.o = (bf16_t*)p->o;
   a.lens = p->lens; a.slopes = p->slopes;
   a.sq = p->sq; a.sk = p->sk; a.sv = p->sv; a.ldq = p->ldq; a.ldk = p->ldk; a.ldv = p->ldv;
@@ -317,12 +320,8 @@ extern "C" int lbmk_cached_attn(const lbmk_cached_attn_desc* p, void* stream) {
     a.part_ml = (float2*)p->scratch;
     a.part_o = p->scratch + 2ll * a.splits * a.rows;
   }
-  const float log2e = 1.4426950408889634f;
-  a.map.scale = p->scale * log2e;
-  a.map.cap_in = p->cap > 0.f ? 2.f * p->scale * log2e / p->cap : 0.f;
-  a.map.cap_out = p->cap * log2e;
   a.map.biased = p->slopes != nullptr;
-  a.map.slope = log2e;
+  a.map.slope = 1.4426950408889634f;
   a.map.mul = p->cap > 0.f || p->slopes ? 1.f : a.map.scale;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)((int64_t)a.B * a.Hk * a.row_blocks), a.splits);

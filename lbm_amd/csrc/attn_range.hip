@@ -28,7 +28,9 @@ constexpr int TB = 64;    // tokens per tile of the walked operand
 // cost registers and scheduling.  2 x 4096 tokens, 20 heads of 64, forward / backward, one kernel against three: plain 207 / 740 us
 // against 207 / 715, with a bias 234 / 779 against 214 / 725, with a cap 286 / 1004 against 281 / 971; 8 heads of 128, causal, 104 / 394
 // against 102 / 366.  (Forward, causal, plain, 64 channels alone gets slower, 117 -> 122 us.)
-constexpr int LINEAR = 0, BIASED = 1, CAPPED = 2;
+// Caps above CAP_FAR (attn_tile.h) in a fourth: the same shapes 281 / 983 us with a cap of 50, 449 / 1285 with one of 500; 8 heads of
+// 128, all keys, 181 / 817 against 234 / 959.
+constexpr int LINEAR = 0, BIASED = 1, CAPPED = 2, CAPPED_FAR = 3;
 
 typedef __attribute__((address_space(3))) char* lds_ptr;
 
@@ -266,13 +268,13 @@ __device__ __forceinline__ bool ranged_fwd_body(const Ranged& a, char* smem) {
         product(zero);
       }
     }
-    if constexpr (MAP == CAPPED) {
+    if constexpr (MAP >= CAPPED) {
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float x = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[kt][e] * a.map.cap_in) + 1.f);
-          s[kt][e] = fmaf(-2.f * a.map.cap_out, x, a.map.cap_out);
+          float x;
+          s[kt][e] = capped<MAP == CAPPED_FAR>(a.map, s[kt][e], x);
         }
       if (a.map.biased) {
         asm volatile("" ::: "memory");
@@ -533,11 +535,11 @@ __device__ __forceinline__ bool ranged_bwd_dq_body(const Ranged& a, char* smem) 
         dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(T::row_frag(sV + kt * 32 * T::ROW, T::row_at(kr, ks)), gf[ks], ks == 0 ? zero : dp, 0, 0, 0);
 #pragma unroll
       for (int e = 0; e < 16; ++e) dp[e] -= delta;
-      if constexpr (MAP == CAPPED) {
+      if constexpr (MAP >= CAPPED) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float x = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[e] * a.map.cap_in) + 1.f);
-          s[e] = fmaf(-2.f * a.map.cap_out, x, a.map.cap_out);
+          float x;
+          s[e] = capped<MAP == CAPPED_FAR>(a.map, s[e], x);
           dp[e] *= 4.f * x * (1.f - x);                       // 1 - tanh^2
         }
         if (a.map.biased) {
@@ -858,11 +860,11 @@ __device__ __forceinline__ bool ranged_bwd_dkv_body(const Ranged& a, char* smem)
 #pragma unroll
         for (int e = 0; e < 4; ++e) dp[4 * g + e] -= d4[e];
       }
-      if constexpr (MAP == CAPPED) {
+      if constexpr (MAP >= CAPPED) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float x = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[e] * a.map.cap_in) + 1.f);
-          s[e] = fmaf(-2.f * a.map.cap_out, x, a.map.cap_out);
+          float x;
+          s[e] = capped<MAP == CAPPED_FAR>(a.map, s[e], x);
           dp[e] *= 4.f * x * (1.f - x);
         }
         if (a.map.biased) {
@@ -1029,7 +1031,8 @@ int ranged_check(const lbmk_ranged_attn_desc* p, bool bwd) {
   LBMK_REQUIRE(2ll * p->B * p->H * ((p->Nq + RB - 1) / RB) < (1ll << 31) && 8ll * p->B * p->Hk * ((p->Nk + RB - 1) / RB) < (1ll << 31) &&
                    p->Nq < (1 << 30) && p->Nk < (1 << 30) && (int64_t)(p->H / p->Hk) * ((p->Nq + TB - 1) / TB) < (1ll << 31),
                "ranged_attn: sizes");
-  LBMK_REQUIRE(p->scale > 0.f && p->cap >= 0.f, "ranged_attn: scale %g, cap %g", (double)p->scale, (double)p->cap);
+  ScoreMap map;
+  LBMK_REQUIRE(score_map(p->scale, p->cap, map), "ranged_attn: scale %g, cap %g", (double)p->scale, (double)p->cap);
   if (p->B == 0 || p->Nq == 0) return LBMK_OK;
   const void* ptr[8] = {p->q, p->o, p->dout, p->dq, p->k, p->v, p->dk, p->dv};
   const int ld[8] = {p->ldq, p->ldo, p->ldg, 0, p->ldk, p->ldv, 0, 0};
@@ -1065,13 +1068,10 @@ Ranged ranged_args(const lbmk_ranged_attn_desc* p) {
   a.parts = p->ranges ? 2 : 1;
   a.cus = lbmk_num_cus();
   a.scale = p->scale;
-  const float log2e = 1.4426950408889634f;
-  a.map.scale = p->scale * log2e;
-  a.map.cap_in = p->cap > 0.f ? 2.f * p->scale * log2e / p->cap : 0.f;
-  a.map.cap_out = p->cap * log2e;
+  score_map(p->scale, p->cap, a.map);
   a.map.biased = p->slopes != nullptr;
   // without a cap the bias is in units of q.k: the product starts from it
-  a.map.slope = p->cap > 0.f ? log2e : 1.f / p->scale;
+  a.map.slope = p->cap > 0.f ? 1.4426950408889634f : 1.f / p->scale;
   a.map.mul = p->cap > 0.f ? 1.f : a.map.scale;
   return a;
 }
@@ -1088,7 +1088,8 @@ Ranged ranged_args(const lbmk_ranged_attn_desc* p) {
     default: LAUNCH(160, 10, MAP); break;      \
   }
 #define BY_MAP(LAUNCH)                                              \
-  if (a.map.cap_out != 0.f) { BY_HEAD(a.D, LAUNCH, CAPPED) }        \
+  if (p->cap > CAP_FAR) { BY_HEAD(a.D, LAUNCH, CAPPED_FAR) }        \
+  else if (p->cap > 0.f) { BY_HEAD(a.D, LAUNCH, CAPPED) }           \
   else if (a.map.biased) { BY_HEAD(a.D, LAUNCH, BIASED) }           \
   else { BY_HEAD(a.D, LAUNCH, LINEAR) }
 

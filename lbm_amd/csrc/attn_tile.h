@@ -158,13 +158,43 @@ __device__ __forceinline__ int wave_max_i(int v) {
 // What turns a product q.k into the exponent (base 2) of the softmax:
 //   cap:  C tanh(scale q.k / cap), C = cap log2(e), tanh(x) = 1 - 2 / (exp(2 x) + 1)        bias: - slope |distance|
 // Without a cap the scaling is left to the fused multiply-add that subtracts the maximum.
+// The difference is off by a few half steps of C: 1e-5 at caps of 50, 2.5e-5 at 128, but 2e-4 at 1000 and 0.13 at 10^6.  From
+// CAP_FAR on, arguments below 1/4 take tanh's series instead, whose next term is below 2^-26 of it: a few half steps of the score.
 struct ScoreMap {
   float mul;        // factor still to be applied to a mapped score (scale * log2(e), or 1 when it is already in that unit)
   float scale;      // scale * log2(e)
   float cap_in;     // 2 scale log2(e) / cap
   float cap_out;    // cap log2(e); 0: no cap
+  float cap_u;      // scale / cap
   float slope;      // factor of the slopes, in the units that the bias is added in
   int biased;
 };
+constexpr float CAP_FAR = 128.f;
+
+// C tanh(scale s / cap), and x with 1 - tanh^2 = 4 x (1 - x)
+template <bool FAR>
+__device__ __forceinline__ float capped(const ScoreMap& m, float s, float& x) {
+  x = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * m.cap_in) + 1.f);
+  const float v = fmaf(-2.f * m.cap_out, x, m.cap_out);
+  if constexpr (!FAR) return v;
+  const float u = s * m.cap_u, t = u * u;
+  float g = 62.f / 2835.f;
+  g = fmaf(g, t, -17.f / 315.f);
+  g = fmaf(g, t, 2.f / 15.f);
+  g = fmaf(g, t, -1.f / 3.f);
+  g = fmaf(g, t, 1.f);
+  return fabsf(u) < 0.25f ? s * m.scale * g : v;
+}
+
+// a scale, a cap and what the kernels take from them: finite, and no number that f32 holds in fewer bits
+inline bool score_map(float scale, float cap, ScoreMap& m) {
+  const float log2e = 1.4426950408889634f, tiny = 1.17549435e-38f, huge = 0x1p126f;
+  if (!(scale >= tiny && scale <= huge) || !(cap == 0.f || (cap >= tiny && cap <= huge))) return false;
+  m.scale = scale * log2e;
+  m.cap_in = cap > 0.f ? 2.f * scale * log2e / cap : 0.f;
+  m.cap_out = cap * log2e;
+  m.cap_u = cap > 0.f ? scale / cap : 0.f;
+  return m.cap_in <= huge;
+}
 
 }  // namespace

@@ -1643,10 +1643,11 @@ def _attn_args(what, heads, kv_heads, head_dim, scale, cap, slopes):
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise ValueError(f"{what}: {heads} heads over {kv_heads} key heads")
     scale = head_dim ** -0.5 if scale is None else float(scale)
-    if not 0 < scale < math.inf:
-        raise ValueError(f"{what}: scale {scale} (positive)")
-    if not 0 <= cap < math.inf:
-        raise ValueError(f"{what}: cap {cap} (0: none)")
+    # (bounds: what f32 holds in all its bits, with room for the factors that the kernels take from them)
+    if not 2.0 ** -126 <= scale <= 2.0 ** 126:
+        raise ValueError(f"{what}: scale {scale} (positive, 2^-126 ... 2^126)")
+    if cap != 0 and not (2.0 ** -126 <= cap <= 2.0 ** 126 and 3 * scale <= cap * 2.0 ** 126):
+        raise ValueError(f"{what}: cap {cap} (0: none; 2^-126 ... 2^126, and at least 3 scale 2^-126)")
     if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (heads,) or not slopes.is_contiguous()):
         raise ValueError(f"slopes: contiguous f32 [{heads}]")
     return scale
