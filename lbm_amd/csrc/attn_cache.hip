@@ -172,11 +172,17 @@ __global__ __launch_bounds__(256) void cached_attn_kernel(const Cached a) {
     pack_column(p, pf);
 
     if (GUARD && masked) {
+      bf16x8 visible[2];
+      float one[16];
+      const unsigned k0 = (unsigned)(kv0 + 4 * h - lo);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) one[e] = k0 + (unsigned)acc_row(e, 0) < seen ? 1.f : 0.f;
+      pack_column(one, visible);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         f32x16 hit = zero;
 #pragma unroll
-        for (int m = 0; m < 2; ++m) mfma_guarded(T::col_frag(sV + 16 * m * T::ROW, T::col_at(clo, dt), T::col_at(chi, dt)), pf[m], o[dt], hit);
+        for (int m = 0; m < 2; ++m) mfma_guarded(T::col_frag(sV + 16 * m * T::ROW, T::col_at(clo, dt), T::col_at(chi, dt)), pf[m], visible[m], o[dt], hit);
         poison(o[dt], hit);
       }
       continue;

@@ -28,8 +28,8 @@ constexpr int TB = 64;    // tokens per tile of the walked operand
 // cost registers and scheduling.  2 x 4096 tokens, 20 heads of 64, forward / backward, one kernel against three: plain 207 / 740 us
 // against 207 / 715, with a bias 234 / 779 against 214 / 725, with a cap 286 / 1004 against 281 / 971; 8 heads of 128, causal, 104 / 394
 // against 102 / 366.  (Forward, causal, plain, 64 channels alone gets slower, 117 -> 122 us.)
-// Caps above CAP_FAR (attn_tile.h) in a fourth: the same shapes 281 / 983 us with a cap of 50, 449 / 1285 with one of 500; 8 heads of
-// 128, all keys, 181 / 817 against 234 / 959.
+// Caps above CAP_FAR (attn_tile.h) in a fourth: the same shapes 289 / 1006 us with a cap of 50, 471 / 1290 with one of 500; 8 heads of
+// 128, all keys, 186 / 821 against 237 / 961.
 constexpr int LINEAR = 0, BIASED = 1, CAPPED = 2, CAPPED_FAR = 3;
 
 typedef __attribute__((address_space(3))) char* lds_ptr;
@@ -330,11 +330,21 @@ __device__ __forceinline__ bool ranged_fwd_body(const Ranged& a, char* smem) {
     l_run += ps0 + ps1;
 
     if (GUARD && masked) {
+      bf16x8 seen[2][2];
+      const unsigned k0 = (unsigned)(kv0 + 4 * h - range.x);
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        float one[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) one[e] = k0 + (unsigned)(32 * kt + acc_row(e, 0)) < len ? 1.f : 0.f;
+        pack_column(one, seen[kt]);
+      }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         f32x16 hit = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int m = 0; m < 4; ++m) mfma_guarded(T::col_frag(sV + 16 * m * T::ROW, T::col_at(clo, dt), T::col_at(chi, dt)), pf[m >> 1][m & 1], o[dt], hit);
+        for (int m = 0; m < 4; ++m)
+          mfma_guarded(T::col_frag(sV + 16 * m * T::ROW, T::col_at(clo, dt), T::col_at(chi, dt)), pf[m >> 1][m & 1], seen[m >> 1][m & 1], o[dt], hit);
         poison(o[dt], hit);
       }
       continue;
@@ -382,8 +392,9 @@ __device__ __attribute__((noinline)) void ranged_fwd_again(uint64_t args, lds_pt
   ranged_fwd_body<DH, KS, MAP, Guarded>(kernel_args(args), (char*)smem);
 }
 
+// (the series of the far caps does not fit a third of the registers: 1033 instead of 471 us, 2 x 4096 tokens, 20 heads of 64)
 template <int DH, int KS, int MAP>
-__global__ __launch_bounds__(256, DH <= 96 ? 3 : DH <= 128 ? 2 : 1) void ranged_fwd_kernel(const Ranged a) {
+__global__ __launch_bounds__(256, DH <= 96 && MAP != CAPPED_FAR ? 3 : DH <= 128 ? 2 : 1) void ranged_fwd_kernel(const Ranged a) {
   __shared__ __attribute__((aligned(16))) char smem[2 * (2 * TB * Tile<DH>::ROW) + 64];
   if (ranged_fwd_body<DH, KS, MAP, Plain>(a, smem)) ranged_fwd_again<DH, KS, MAP>((uint64_t)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr(), (lds_ptr)smem);
 }
@@ -567,14 +578,22 @@ __device__ __forceinline__ bool ranged_bwd_dq_body(const Ranged& a, char* smem) 
       pack_column(ds, dl);
       const char* sk = sK + 32 * kt * T::ROW;
       if (GUARD && masked) {
+        bf16x8 seen[2];
+        float one[16];
+        const unsigned k0 = (unsigned)(kv0 + 32 * kt + 4 * h - range.x);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) one[e] = k0 + (unsigned)acc_row(e, 0) < len ? 1.f : 0.f;
+        pack_column(one, seen);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
           f32x16 hit = zero;
 #pragma unroll
           for (int ss = 0; ss < 2; ++ss) {
-            const bf16x8 kc = T::col_frag(sk + 16 * ss * T::ROW, T::col_at(clo, dt), T::col_at(chi, dt));
-            mfma_guarded(kc, dl[ss], acc[dt], hit);
-            mfma_guarded(kc, df[ss], acc[dt], hit);
+            bf16x8 fin, ind;
+            split_finite(T::col_frag(sk + 16 * ss * T::ROW, T::col_at(clo, dt), T::col_at(chi, dt)), fin, ind);
+            acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fin, dl[ss], acc[dt], 0, 0, 0);
+            acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fin, df[ss], acc[dt], 0, 0, 0);
+            hit = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ind, seen[ss], hit, 0, 0, 0);
           }
           poison(acc[dt], hit);
         }
@@ -873,7 +892,10 @@ __device__ __forceinline__ bool ranged_bwd_dkv_body(const Ranged& a, char* smem)
           for (int e = 0; e < 16; ++e) s[e] = fmaf(-slope, fabsf(d0 + (float)acc_row(e, 0)), s[e]);
         }
       }
-      float p[16], ds[16];
+      float p[16], ds[16], one[16];       // one: 1 where a row sees the key
+      if constexpr (GUARD)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) one[e] = 1.f;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const f32x4 l4 = *(const f32x4*)(sL + 32 * u + 8 * g + 4 * h);
@@ -892,7 +914,10 @@ __device__ __forceinline__ bool ranged_bwd_dkv_body(const Ranged& a, char* smem)
           const int l[4] = {lo.x, lo.y, lo.z, lo.w}, g4[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (kc < l[e] || kc >= g4[e]) p[4 * g + e] = ds[4 * g + e] = 0.f;
+            if (kc < l[e] || kc >= g4[e]) {
+              p[4 * g + e] = ds[4 * g + e] = 0.f;
+              if constexpr (GUARD) one[4 * g + e] = 0.f;
+            }
         }
       }
       if (qt * TB + 32 * u + 32 > a.Nq) {      // rows past the end: their statistics read as zeros, and a bias may make p infinite
@@ -900,7 +925,10 @@ __device__ __forceinline__ bool ranged_bwd_dkv_body(const Ranged& a, char* smem)
         const int past = a.Nq - (qt * TB + 32 * u + 4 * h);
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (acc_row(e, 0) >= past) p[e] = ds[e] = 0.f;
+          if (acc_row(e, 0) >= past) {
+            p[e] = ds[e] = 0.f;
+            if constexpr (GUARD) one[e] = 0.f;
+          }
       }
       bf16x8 pf[2], df[2];
       pack_column(p, pf);
@@ -908,13 +936,15 @@ __device__ __forceinline__ bool ranged_bwd_dkv_body(const Ranged& a, char* smem)
       const char* sq = sQ + 32 * u * T::ROW;
       const char* sg = sG + 32 * u * T::ROW;
       if (GUARD && masked) {
+        bf16x8 seen[2];
+        pack_column(one, seen);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
           f32x16 hq = zero, hg = zero;
 #pragma unroll
           for (int ss = 0; ss < 2; ++ss) {
-            mfma_guarded(T::col_frag(sg + 16 * ss * T::ROW, T::col_at(clo, dt), T::col_at(chi, dt)), pf[ss], dv[dt], hg);
-            mfma_guarded(T::col_frag(sq + 16 * ss * T::ROW, T::col_at(clo, dt), T::col_at(chi, dt)), df[ss], dk[dt], hq);
+            mfma_guarded(T::col_frag(sg + 16 * ss * T::ROW, T::col_at(clo, dt), T::col_at(chi, dt)), pf[ss], seen[ss], dv[dt], hg);
+            mfma_guarded(T::col_frag(sq + 16 * ss * T::ROW, T::col_at(clo, dt), T::col_at(chi, dt)), df[ss], seen[ss], dk[dt], hq);
           }
           poison(dv[dt], hg);
           poison(dk[dt], hq);
@@ -1009,7 +1039,7 @@ int dkv_splits(bool ranged, int B, int H, int Hk, int Nq, int Nk, int D) {
 }
 
 // workgroups of the row kernels that fit a CU (their launch bounds)
-int fwd_occupancy(int DHP) { return DHP <= 96 ? 3 : DHP <= 128 ? 2 : 1; }
+int fwd_occupancy(int DHP, bool far) { return DHP <= 96 && !far ? 3 : DHP <= 128 ? 2 : 1; }
 int dq_occupancy(int DHP) { return DHP <= 64 ? 3 : DHP <= 96 ? 2 : 1; }
 
 // Ranked workgroups: few enough for the order to matter and for the ranking to be cheap, and walks long enough to pay for it (every
@@ -1126,7 +1156,7 @@ extern "C" int lbmk_ranged_attn(const lbmk_ranged_attn_desc* p, void* stream) {
   Ranged a = ranged_args(p);
   hipStream_t s = (hipStream_t)stream;
   a.blocks = (a.Nq + RB - 1) / RB;
-  order_blocks(a, fwd_occupancy(pad_head(a.D)));
+  order_blocks(a, fwd_occupancy(pad_head(a.D), p->cap > CAP_FAR));
 #define FWD(DHP, KSP, MAPP) hipLaunchKernelGGL((ranged_fwd_kernel<DHP, KSP, MAPP>), dim3((unsigned)((int64_t)a.blocks * a.parts * a.H * a.B)), dim3(256), 0, s, a)
   BY_MAP(FWD)
 #undef FWD

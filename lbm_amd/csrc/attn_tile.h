@@ -106,9 +106,9 @@ __device__ __forceinline__ void pack_column(const float (&p)[16], bf16x8 (&f)[2]
 // Masked places hold 0 in one operand, and 0 * inf or 0 * NaN in the other would poison a sum that must not see them.  The walks
 // scan each tile that has masked places (a few instructions per 16 bytes, and such tiles are few); where one holds a value that
 // is not finite the whole walk is done again in a second form, whose masked tiles multiply the finite values alone and learn
-// from a product of indicators (not finite x not masked) which sums become NaN.  The first form carries none of that: with both
-// in one loop the registers spilled and the tile loads were waited for at once (2.5 x slower).  Finite sums are the same bits
-// whatever the masked places hold.
+// from a product of indicators (not finite x seen) which sums become NaN: seen by the mask, for a weight may be 0 at a place that
+// is seen.  The first form carries none of that: with both in one loop the registers spilled and the tile loads were waited for
+// at once (2.5 x slower).  Finite sums are the same bits whatever the masked places hold.
 struct Plain { static constexpr bool guard = false; };
 struct Guarded { static constexpr bool guard = true; };
 
@@ -123,17 +123,21 @@ __device__ __forceinline__ bool tile_not_finite(const char* tile, int lane) {
   }
   return __builtin_amdgcn_ballot_w64((a & 0x80008000u) != 0) != 0;
 }
-__device__ __forceinline__ void mfma_guarded(bf16x8 a, bf16x8 b, f32x16& acc, f32x16& hit) {
-  bf16x8 fin, ind, pat;
+// an operand's finite values, and ones where it holds others
+__device__ __forceinline__ void split_finite(bf16x8 a, bf16x8& fin, bf16x8& ind) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const bool ok = (__builtin_bit_cast(uint16_t, (__bf16)a[e]) & 0x7f80) != 0x7f80;
     fin[e] = ok ? (__bf16)a[e] : (__bf16)0.f;
     ind[e] = ok ? (__bf16)0.f : (__bf16)1.f;
-    pat[e] = (__builtin_bit_cast(uint16_t, (__bf16)b[e]) & 0x7fff) ? (__bf16)1.f : (__bf16)0.f;
   }
+}
+// acc += a b over a's finite values; hit: how many of the others are `seen` (ones and zeros in b's layout)
+__device__ __forceinline__ void mfma_guarded(bf16x8 a, bf16x8 b, bf16x8 seen, f32x16& acc, f32x16& hit) {
+  bf16x8 fin, ind;
+  split_finite(a, fin, ind);
   acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fin, b, acc, 0, 0, 0);
-  hit = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ind, pat, hit, 0, 0, 0);
+  hit = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ind, seen, hit, 0, 0, 0);
 }
 __device__ __forceinline__ void poison(f32x16& acc, const f32x16& hit) {
 #pragma unroll

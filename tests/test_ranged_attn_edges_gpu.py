@@ -91,3 +91,78 @@ def test_entry_points_refuse_scales_and_caps_that_f32_does_not_hold(bad):
     assert _C.lib.lbmk_ranged_attn(ctypes.byref(r), None) == 1
     assert _C.lib.lbmk_ranged_attn_bwd(ctypes.byref(r), None) == 1
     assert _C.lib.lbmk_cached_attn(ctypes.byref(c), None) == 1
+
+
+# ---- values that are not finite where they are seen ------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [40, 64, 96, 128, 160])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("at", [10, 70, 140])
+def test_a_seen_value_counts_however_small_its_weight(cuda, D, value, at):
+    """slopes of 8 take every weight from 14 tokens on below f32's range: 0 times a value that is not finite is NaN, in tiles that have
+    masked places and in tiles that have none"""
+    from lbm_amd import ops
+    B, N, H, Hk = 1, 200, 2, 1
+    q, k, v, g, gen = make(23, B, N, N, H, Hk, D)
+    ranges, slopes = ranges_of("causal", B, N, N, gen), torch.tensor([8.0, 16.0])
+    seen, pos = seen_by(ranges, N), torch.arange(N).expand(B, N)
+    want = definition(q, k, v, H, Hk, D, seen, pos, D ** -0.5, 0.0, slopes, g)
+    dev = [t.to(cuda) for t in (q, k, v, g, ranges, slopes)]
+    good = ops.ranged_attn(*dev[:3], H, Hk, D, dev[4], slopes=dev[5], return_lse=True)
+    rows = torch.arange(N)
+
+    def split(name, got, heads, bad):
+        """`bad` [N, D]: not finite there in every head, and the definition's values elsewhere"""
+        got, ref, tol = (t.detach().double().cpu().view(N, heads, D).transpose(0, 1) for t in (got, *want[name]))
+        assert not bool(torch.isfinite(got[:, bad]).any()), name
+        assert bool(((got - ref).abs() <= tol)[:, ~bad].all()), name
+
+    # a value: the rows from it on, in its channel
+    v2 = v.clone()
+    v2[0, at, 3] = value
+    bad = torch.zeros(N, D, dtype=torch.bool)
+    bad[at:, 3] = True
+    split("o", ops.ranged_attn(dev[0], dev[1], v2.to(cuda), H, Hk, D, dev[4], slopes=dev[5]), H, bad)
+    # an output gradient: the keys up to its row, in its channel of dv and everywhere in dk (its row's dP is not finite)
+    g2 = g.clone().view(B, N, H, D)
+    g2[0, at, :, 3] = value
+    dq, dk, dv = ops.ranged_attn_bwd(*dev[:3], good[0], g2.view(B, N, -1).to(cuda), good[1], H, Hk, D, dev[4], slopes=dev[5])
+    bad = torch.zeros(N, D, dtype=torch.bool)
+    bad[:at + 1, 3] = True
+    split("dv", dv, Hk, bad)
+    bad[:at + 1] = True
+    split("dk", dk, Hk, bad)
+    bad = (rows == at)[:, None].expand(N, D)
+    split("dq", dq, H, bad)
+    if value != value:
+        return
+    # a key whose scores are -inf: no weight, so no change of the output, but 0 times it in the rows' gradients
+    q2, k2 = q.clone().view(B, N, H, D), k.clone()
+    q2[0, at + 1:, :, 5] = -q2[0, at + 1:, :, 5].abs() if value > 0 else q2[0, at + 1:, :, 5].abs()
+    q2[0, at, :, 5] = 0.0                                            # (its own row: 0 * inf)
+    q2, k2[0, at, 5] = q2.view(B, N, -1), value
+    o, lse = ops.ranged_attn(q2.to(cuda), k2.to(cuda), dev[2], H, Hk, D, dev[4], slopes=dev[5], return_lse=True)
+    seen2 = seen.clone()
+    seen2[0, :, at] = False
+    k0 = k.clone()
+    k0[0, at] = 0.0
+    want = definition(q2, k0, v, H, Hk, D, seen2, pos, D ** -0.5, 0.0, slopes, g)
+    split("o", o, H, (rows == at)[:, None].expand(N, D))
+    dq, dk, dv = ops.ranged_attn_bwd(q2.to(cuda), k2.to(cuda), dev[2], o, dev[3], lse, H, Hk, D, dev[4], slopes=dev[5])
+    assert not bool(torch.isfinite(dq.cpu().view(N, H, D)[at:, :, 5]).any())
+    assert bool(torch.isfinite(dq[0, :at]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [40, 64, 128, 160])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_a_seen_value_counts_over_a_cache(cuda, D, value):
+    from lbm_amd import ops
+    B, n, H, Hk, rows = 2, 3, 4, 2, 700
+    q, k, v, _, _ = make(24, B, n, rows, H, Hk, D)
+    lens, slopes = torch.tensor([650, 90], dtype=I32), torch.full((H,), 16.0)        # weights below f32's range from 7 tokens on
+    v[0, 300, 1], v[0, 648, 2], v[0, 640, 3], v[1, 2, 4], v[1, 66, 5], v[1, 89, 6] = [value] * 6
+    o = ops.cached_attn(q.to(cuda), k.to(cuda), v.to(cuda), lens.to(cuda), H, Hk, D, slopes=slopes.to(cuda)).cpu().view(B, n, H, D)
+    bad = torch.zeros(B, n, D, dtype=torch.bool)
+    bad[0, :, 1], bad[0, 1:, 2], bad[0, :, 3], bad[1, :, 4], bad[1, :, 5], bad[1, 2:, 6] = [True] * 6
+    assert torch.equal(~torch.isfinite(o), bad[:, :, None].expand(B, n, H, D).logical_and((torch.arange(H) // (H // Hk) == 0)[:, None]))
