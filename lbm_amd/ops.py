@@ -1729,7 +1729,8 @@ def cached_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, l
     q: bf16 [B, n, heads * D]; caches: bf16 [B, rows, kv_heads * D] (any row and batch stride); lens: int32 [B] on the device,
     tokens in each cache with the new ones (clipped to [0, rows]).  New token i stands at lens - n + i and sees the keys up to
     itself (``window`` > 0: the last ``window`` of them); a token in front of the cache's start gets zeros.  Cache rows from
-    lens on are not read.  The keys are split over workgroups by the device's own lengths, so a captured call follows them."""
+    lens on are not read.  The keys are split over workgroups by the device's own lengths, so a captured call follows them.
+    Serving only: no gradients."""
     scale = _attn_args("cached_attn", heads, kv_heads, head_dim, scale, cap, slopes)
     if window < 0:
         raise ValueError(f"cached_attn: window {window}")
@@ -1742,6 +1743,8 @@ def cached_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, l
     if lens.dtype != torch.int32 or lens.shape != (B,) or not lens.is_contiguous():
         raise ValueError(f"lens: contiguous int32 [{B}]")
     device = _one_device(q, k_cache, v_cache, lens, slopes)
+    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or (slopes is not None and slopes.requires_grad)):
+        raise NotImplementedError("cached_attn is inference-only: call it under torch.no_grad() or detach its operands (layers.ranged_attention has gradients)")
     if device < 0:
         _need_gpu(q)
     o = torch.empty(B, n, C_, dtype=bf16, device=q.device)

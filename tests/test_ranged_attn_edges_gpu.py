@@ -166,3 +166,16 @@ def test_a_seen_value_counts_over_a_cache(cuda, D, value):
     bad = torch.zeros(B, n, D, dtype=torch.bool)
     bad[0, :, 1], bad[0, 1:, 2], bad[0, :, 3], bad[1, :, 4], bad[1, :, 5], bad[1, 2:, 6] = [True] * 6
     assert torch.equal(~torch.isfinite(o), bad[:, :, None].expand(B, n, H, D).logical_and((torch.arange(H) // (H // Hk) == 0)[:, None]))
+
+
+# ---- gradients that nobody computes ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("name", ["q", "k_cache", "v_cache", "slopes"])
+def test_cached_attn_has_no_gradient_and_says_so(name):
+    from lbm_amd import ops
+    a = _cpu_operands()
+    a["k_cache"], a["v_cache"], a["lens"], a["slopes"] = a.pop("k"), a.pop("v"), torch.zeros(2, dtype=I32), torch.zeros(2)
+    a[name].requires_grad_(True)
+    with pytest.raises(NotImplementedError, match="inference-only"):
+        ops.cached_attn(**a)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="GPU only"):
+        ops.cached_attn(**a)
