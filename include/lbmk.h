@@ -269,7 +269,8 @@ int lbmk_flash_attn_bwd(const void* q, const void* qt, const void* k, const void
  *                wanted), read backward
  *   rest       : bf16 [B][Nq][H*D], what rounding took from o: written forward, read backward, where it halves the error of
  *                rowsum(dout * o) and with it a third of dq's and dk's (NULL: not wanted)
- *   scratch    : backward only, lbmk_ranged_attn_bwd_scratch_floats(...) floats, 16-byte aligned
+ *   scratch    : backward only, lbmk_ranged_attn_bwd_scratch_floats(...) floats, 16-byte aligned; the size follows the current
+ *                device's compute units: ask for it with the device of the call current
  *   Without queries (B or Nq 0) nothing is written: dk and dv are then the caller's to clear.
  * What an operand holds at places that a query does not see has no influence on its row, inf and NaN included; a value that is not
  * finite at a place it does see makes the sums it enters not finite (NaN).
@@ -303,7 +304,7 @@ int lbmk_key_ranges(int32_t* ranges, const int32_t* doc_offsets, int docs, int64
  *   q, o : bf16 [B][n][ldq] (o contiguous);  k, v : bf16 [B][cap_rows][ldk / ldv];  lens : int32 [B] tokens in the cache, the
  *   new ones included (values outside [0, cap_rows] are clipped).  New token i stands at p = lens[b] - n + i and sees the keys up
  *   to p (window > 0: the last `window` of them); p < 0: a row of zeros.  Rows of the cache from lens[b] on are not read.
- *   scratch : lbmk_cached_attn_scratch_floats(...) floats, 8-byte aligned (NULL when 0). */
+ *   scratch : lbmk_cached_attn_scratch_floats(...) floats, 8-byte aligned (NULL when 0), asked for with the call's device current. */
 typedef struct lbmk_cached_attn_desc {
   const void *q, *k, *v;
   void* o;

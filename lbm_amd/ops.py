@@ -1427,6 +1427,14 @@ def _one_device(t: torch.Tensor, *others) -> int:
     return d
 
 
+def _planned(device: int, fn, *args):
+    """``fn(*args)`` with ``device`` current: the library plans by the current device's compute units"""
+    if device == torch.cuda.current_device():
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
+
+
 def _launch(device: int, what: str, fn, *args):
     """``fn(*args, stream)`` with ``device`` current and on its current stream"""
     if device < 0:
@@ -1714,7 +1722,7 @@ def ranged_attn_bwd(q, k, v, o, do, lse, heads: int, kv_heads: int, head_dim: in
     new = torch.empty if Nq and B else torch.zeros      # without queries the keys' gradients are zeros that no kernel writes
     dev = q.device
     dq, dk, dv = new(B, Nq, C_, dtype=bf16, device=dev), new(B, Nk, Ck, dtype=bf16, device=dev), new(B, Nk, Ck, dtype=bf16, device=dev)
-    scratch = torch.empty(lib.lbmk_ranged_attn_bwd_scratch_floats(B, heads, kv_heads, Nq, Nk, head_dim, 0 if ranges is None else 1),
+    scratch = torch.empty(_planned(device, lib.lbmk_ranged_attn_bwd_scratch_floats, B, heads, kv_heads, Nq, Nk, head_dim, 0 if ranges is None else 1),
                           dtype=torch.float32, device=dev)
     d = RangedAttnDesc(qp, kp, vp, gp, op, _ptr(rest), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), lse.data_ptr(), _ptr(ranges), _ptr(slopes),
                        scratch.data_ptr(), B, heads, kv_heads, Nq, Nk, head_dim, ldq, ldk, ldv, ldo, ldg, sq, sk, sv, so, sg, scale, cap)
@@ -1748,7 +1756,7 @@ def cached_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, l
     if device < 0:
         _need_gpu(q)
     o = torch.empty(B, n, C_, dtype=bf16, device=q.device)
-    nfl = lib.lbmk_cached_attn_scratch_floats(B, heads, kv_heads, n, rows, head_dim)
+    nfl = _planned(device, lib.lbmk_cached_attn_scratch_floats, B, heads, kv_heads, n, rows, head_dim)
     scratch = torch.empty(nfl, dtype=torch.float32, device=q.device) if nfl else None
     d = CachedAttnDesc(qp, kp, vp, o.data_ptr(), lens.data_ptr(), _ptr(slopes), _ptr(scratch), B, heads, kv_heads, n, rows, head_dim, window,
                        ldq, ldk, ldv, sq, sk, sv, scale, cap)

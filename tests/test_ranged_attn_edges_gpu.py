@@ -179,3 +179,35 @@ def test_cached_attn_has_no_gradient_and_says_so(name):
         ops.cached_attn(**a)
     with torch.no_grad(), pytest.raises(RuntimeError, match="GPU only"):
         ops.cached_attn(**a)
+
+
+# ---- scratch -----------------------------------------------------------------------------------------------------------
+def test_scratch_is_sized_on_the_operands_device(monkeypatch):
+    """the size follows the compute units of the current device, so it is asked for with the operands' device current, where the
+    launch asks for the same plan; a library and two devices that are not there stand in for the real ones"""
+    import contextlib
+    from lbm_amd import ops
+    current, asked = [0], []
+
+    @contextlib.contextmanager
+    def device(n):
+        before, current[0] = current[0], n
+        yield
+        current[0] = before
+
+    class Lib:
+        lbmk_ranged_attn_bwd = lbmk_cached_attn = None
+
+        def _floats(self, *sizes):
+            asked.append(current[0])
+            return 8
+        lbmk_ranged_attn_bwd_scratch_floats = lbmk_cached_attn_scratch_floats = _floats
+    monkeypatch.setattr(ops, "lib", Lib())
+    monkeypatch.setattr(ops, "_one_device", lambda *a: 1)
+    monkeypatch.setattr(ops, "_launch", lambda device, *a: None)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    a = _cpu_operands()
+    ops.ranged_attn_bwd(a["q"], a["k"], a["v"], a["q"], a["q"], torch.zeros(2, 2, 5), 2, 1, 64)
+    ops.cached_attn(a["q"], a["k"], a["v"], torch.zeros(2, dtype=I32), 2, 1, 64)
+    assert asked == [1, 1] and current == [0]
