@@ -1462,6 +1462,8 @@ def _token_rows(name: str, t: torch.Tensor, heads: Optional[int], head_dim: int,
         raise ValueError(f"{name}: [B, N, C]{'' if batched else ' or [N, C]'} expected, got {tuple(shape)}")
     if c % head_dim or c == 0 or (heads is not None and c != heads * head_dim):
         raise ValueError(f"{name}: {c} channels are not {'' if heads is None else heads} heads of {head_dim}")
+    if (B | N) >> 31:
+        raise ValueError(f"{name}: {B} x {N} tokens")
     if N <= 1:
         ld = c
     if B <= 1:
@@ -1608,8 +1610,8 @@ def key_ranges(B: int, Nq: int, Nk: Optional[int] = None, *, causal: bool = Fals
     int32 [B]): the first tokens of each document are seen by all its queries.  lens: int32 [B], keys from there on are
     padding."""
     Nk = Nq if Nk is None else Nk
-    if B < 0 or Nq < 0 or Nk < 0 or window < 0:
-        raise ValueError(f"key_ranges: B {B}, Nq {Nq}, Nk {Nk}, window {window}")
+    if B < 0 or Nq < 0 or Nk < 0 or window < 0 or Nq >> 30 or Nk >> 30:
+        raise ValueError(f"key_ranges: B {B}, Nq {Nq}, Nk {Nk} (below 2^30), window {window}")
     if not causal and (window or prefix is not None):
         raise ValueError("key_ranges: window and prefix go with causal")
     if window and prefix is not None:
@@ -1632,7 +1634,7 @@ def key_ranges(B: int, Nq: int, Nk: Optional[int] = None, *, causal: bool = Fals
     out = torch.empty(B, Nq, 2, dtype=torch.int32, device=dev)
     docs = documents.shape[-1] - 1 if documents is not None else 0
     _launch(out.get_device(), "lbmk_key_ranges", lib.lbmk_key_ranges, out.data_ptr(), _ptr(documents), docs,
-            docs + 1 if documents is not None and documents.dim() == 2 else 0, _ptr(prefix), _ptr(lens), B, Nq, Nk, 1 if causal else 0, window)
+            docs + 1 if documents is not None and documents.dim() == 2 else 0, _ptr(prefix), _ptr(lens), B, Nq, Nk, 1 if causal else 0, min(window, Nk))
     return out
 
 
@@ -1758,7 +1760,7 @@ def cached_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, l
     o = torch.empty(B, n, C_, dtype=bf16, device=q.device)
     nfl = _planned(device, lib.lbmk_cached_attn_scratch_floats, B, heads, kv_heads, n, rows, head_dim)
     scratch = torch.empty(nfl, dtype=torch.float32, device=q.device) if nfl else None
-    d = CachedAttnDesc(qp, kp, vp, o.data_ptr(), lens.data_ptr(), _ptr(slopes), _ptr(scratch), B, heads, kv_heads, n, rows, head_dim, window,
+    d = CachedAttnDesc(qp, kp, vp, o.data_ptr(), lens.data_ptr(), _ptr(slopes), _ptr(scratch), B, heads, kv_heads, n, rows, head_dim, min(window, rows),
                        ldq, ldk, ldv, sq, sk, sv, scale, cap)
     _launch(device, "lbmk_cached_attn", lib.lbmk_cached_attn, C.byref(d))
     return o
@@ -1807,6 +1809,8 @@ def linear_adapters(x: torch.Tensor, pw: PackedWeight, down: torch.Tensor, up: t
     device = _one_device(x, w, pw.bias, down, up, index, scaling)
     if torch.is_grad_enabled() and (x.requires_grad or down.requires_grad or up.requires_grad or (scaling is not None and scaling.requires_grad)):
         raise NotImplementedError("linear_adapters is inference-only: call it under torch.no_grad() or detach its operands")
+    if R * rows >> 31:
+        raise ValueError(f"linear_adapters: {R} requests of {rows} rows (below 2^31 in all)")
     # one row stride for all rows (a request's rows follow the previous one's)
     if rows <= 1:
         ldx = sr

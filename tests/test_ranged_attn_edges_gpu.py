@@ -211,3 +211,31 @@ def test_scratch_is_sized_on_the_operands_device(monkeypatch):
     ops.ranged_attn_bwd(a["q"], a["k"], a["v"], a["q"], a["q"], torch.zeros(2, 2, 5), 2, 1, 64)
     ops.cached_attn(a["q"], a["k"], a["v"], torch.zeros(2, dtype=I32), 2, 1, 64)
     assert asked == [1, 1] and current == [0]
+
+
+# ---- numbers that 32 bits do not hold ----------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("window", [2 ** 31, 2 ** 32 + 5, 2 ** 63 - 1, 10 ** 30])
+def test_a_window_wider_than_32_bits_is_no_window(cuda, window):
+    from lbm_amd import ops
+    for Nq, Nk in ((40, 40), (3, 200), (9, 4)):
+        assert torch.equal(ops.key_ranges(2, Nq, Nk, causal=True, window=window, device=cuda), ops.key_ranges(2, Nq, Nk, causal=True, device=cuda))
+    q, k, v, _, _ = make(25, 2, 2, 90, 2, 1, 64)
+    args = (q.to(cuda), k.to(cuda), v.to(cuda), torch.tensor([90, 41], dtype=I32, device=cuda), 2, 1, 64)
+    assert torch.equal(ops.cached_attn(*args, window=window), ops.cached_attn(*args))
+
+
+def test_sizes_that_32_bits_do_not_hold():
+    from lbm_amd import ops
+    for Nq, Nk in ((2 ** 32 + 5, 9), (9, 2 ** 32 + 5), (5, 2 ** 30)):
+        with pytest.raises(ValueError, match="key_ranges"):
+            ops.key_ranges(0, Nq, Nk)
+    wide = lambda *s: torch.empty(*s, dtype=BF, device="meta")  # noqa: E731
+    with pytest.raises(ValueError, match="tokens"):
+        ops.qk_norm_rope(wide(1, 2 ** 32 + 5, 64), wide(1, 2 ** 32 + 5, 64), 64, None, None)
+    with pytest.raises(ValueError, match="tokens"):
+        ops.ranged_attn(wide(1, 3, 64), wide(1, 2 ** 32 + 5, 64), wide(1, 2 ** 32 + 5, 64), 1, 1, 64)
+    pw = ops.PackedWeight(wide(32, 64), None, 32, 64, 64, 64, 1, 1)
+    for x, index in ((wide(1, 2 ** 32 + 5, 64), 1), (wide(2 ** 16, 2 ** 15, 64), 2 ** 16)):
+        with pytest.raises(ValueError, match="rows"):
+            ops.linear_adapters(x, pw, wide(2, 4, 64), wide(2, 32, 4), torch.empty(index, dtype=I32, device="meta"))
