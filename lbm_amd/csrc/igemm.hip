@@ -1224,6 +1224,8 @@ extern "C" int lbmk_igemm(const lbmk_igemm_desc* dp, void* stream) {
     LBMK_REQUIRE(d.lr_t && d.lr_index && d.lr_count > 0 && d.lr_rows > 0 && d.M % d.lr_rows == 0, "igemm: adapters of %d rows per request over %d rows",
                  d.lr_rows, d.M);
     LBMK_REQUIRE(d.lr_rank > 0 && d.lr_rank <= 256 && d.lr_k % 32 == 0 && d.lr_k >= d.lr_rank, "igemm: adapter rank %d (t has %d columns)", d.lr_rank, d.lr_k);
+    // (a tile of at most 256 rows is addressed by 32-bit offsets from its first row; what lies past 2 GiB would read as zeros)
+    LBMK_REQUIRE(((int64_t)((d.M < 256 ? d.M : 256) - 1) * d.a_cs + d.K) * 2 < (1ll << 31), "igemm: adapters with rows %d elements apart", d.a_cs);
     LBMK_REQUIRE(lbmk_aligned(d.lr_t, 16) && lbmk_aligned(d.lr_up, d.lr_rank % 8 == 0 ? 16 : 2) && lbmk_aligned(d.lr_index, 4), "igemm: misaligned adapter");
   }
   int tile = d.tile;

@@ -1819,6 +1819,9 @@ def linear_adapters(x: torch.Tensor, pw: PackedWeight, down: torch.Tensor, up: t
     xp = x.data_ptr()
     if (unit != 1 or xp & 15 or ldx & 7 or ldx < K or ldx >> 31 or (rows > 1 and R > 1 and sr != rows * ldx)) and R * rows:
         raise ValueError(f"linear_adapters: strides {stride}: channels adjacent, one stride of a multiple of 8 between all rows")
+    few = tile < 0 and lib.lbmk_adapter_few_suits(R, rows)
+    if not few and R * rows and (min(R * rows, 256) - 1) * ldx + K >> 30:
+        raise ValueError(f"linear_adapters: row stride {ldx}: the tiled product takes 256 rows within 2 GiB")
     if device < 0:
         _need_gpu(x)
     T = R * rows
@@ -1829,7 +1832,7 @@ def linear_adapters(x: torch.Tensor, pw: PackedWeight, down: torch.Tensor, up: t
     t = torch.empty(T, tk, dtype=bf16, device=x.device)
     bias, ip, tp = _ptr(pw.bias), index.data_ptr(), t.data_ptr()
     _launch(device, "lbmk_adapter_down", lib.lbmk_adapter_down, xp, dp, ip, _ptr(scaling), tp, R, rows, K, ldx, rank, tk, count)
-    if tile < 0 and lib.lbmk_adapter_few_suits(R, rows):
+    if few:
         _launch(device, "lbmk_adapter_linear_few", lib.lbmk_adapter_linear_few, xp, w.data_ptr(), bias, tp, upp, ip, out.data_ptr(), R, rows, N, K,
                 ldx, pw.Kp, N, rank, tk, count)
         return out
