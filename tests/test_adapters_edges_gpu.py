@@ -42,3 +42,24 @@ def test_wide_row_strides(cuda, R, rows):
     args = on(cuda, w, b, down, up, index, scaling)
     y = ops.linear_adapters(view, ops.pack_linear_weight(args[0], args[1]), *args[2:])
     check(y, definition(x, w, b, down, up, scaling, index))
+
+
+# ---- many rows: two groups of 16 rows share one reading of the factor (from 512 groups of 16 rows on) --------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [
+    (18, 451, 128, 72, 3, 40, True),           # 29 groups of a request in 15 pairs, the last rows 3 of 32; two blocks of ranks
+    (33, 250, 320, 40, 5, 7, False),
+    (512, 17, 72, 200, 4, 16, True),           # the second group of a pair holds one row
+    (1, 8200, 64, 64, 1, 64, True),
+], ids=lambda c: "-".join(map(str, c)))
+def test_many_rows(cuda, case):
+    from lbm_amd import ops
+    *sizes, bias = case
+    x, w, b, down, up, scaling, index = make(32, *sizes, bias)
+    index[0] = 0
+    want = definition(x, w, b, down, up, scaling, index)
+    xd, wd, bd, dd, ud, sd, idx = on(cuda, x, w, b, down, up, scaling, index)
+    pw = ops.pack_linear_weight(wd, bd)
+    y = ops.linear_adapters(xd, pw, dd, ud, idx, sd)
+    check(y, want)
+    assert torch.equal(y, ops.linear_adapters(xd, pw, dd, ud, idx, sd))
