@@ -187,6 +187,14 @@ __device__ __forceinline__ float nr_sum(float v) {
   return v;
 }
 
+// the hardware's reciprocal root: off by one step of f32 where an exactly rounded one is off by half, which only the f32 form's
+// outputs can show, and a fifth of its instructions.  It takes subnormal arguments for zeros, so those are scaled
+__device__ __forceinline__ float nr_rsq(float v) {
+  const bool tiny = v < 0x1p-126f;
+  const float r = __builtin_amdgcn_rsqf(tiny ? v * 0x1p24f : v);
+  return tiny ? r * 0x1p12f : r;
+}
+
 // blockIdx.y: 0 the queries, 1 the keys
 template <typename T, int VEC, bool INTER, int L, bool BWD>
 __global__ __launch_bounds__(NR_THREADS) void norm_rope_kernel(NormRope d) {
@@ -271,7 +279,7 @@ __global__ __launch_bounds__(NR_THREADS) void norm_rope_kernel(NormRope d) {
         }
         // (a select, not a product: what an idle lane reads twice may be infinite)
         const float ms = nr_sum<L>((ca < 0 ? 0.f : qa) + (cb < 0 ? 0.f : qb)) * inv_d;
-        const float rstd = __builtin_amdgcn_rsqf(ms + d.eps);
+        const float rstd = nr_rsq(ms + d.eps);
         if constexpr (!BWD) {
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {

@@ -58,3 +58,36 @@ def test_more_tokens_than_a_step_of_the_grid(cuda, dtype, B, N, Hq, Hk, D, F, in
             assert bool((off <= half * want.abs() + n * one * want.abs().amax(-1, keepdim=True) + 1e-37).all())
         off = (dw.double() - rdw).abs()
         assert bool((off <= ((steps * min(H, 5) + 118) * one) * mag + one * rdw.abs()).all()), float((off / (one * mag)).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("eps", [0.0, 1e-40])
+def test_heads_whose_mean_square_is_a_subnormal_number(cuda, dtype, eps):
+    """values around 2^-65: squares around 2^-130, which f32 holds in 19 bits and fewer.  A square is off by half a step of 2^-149, so
+    the mean square by 2^-149 (of at least 2^-132: 2^-17 of it, and half of that in the root), and the outputs by 2^-17 of their
+    head's largest magnitude beside the usual roundings; the gradient's two terms likewise."""
+    from lbm_amd import ops
+    B, N, H, D, F = 1, 37, 3, 64, 32
+    gen = torch.Generator(device=cuda).manual_seed(42)
+    r = lambda *s: torch.randn(*s, generator=gen, device=cuda)  # noqa: E731
+    q, k = ((r(B, N, H * D) * 2.0 ** -64.5).to(dtype) for _ in range(2))
+    # (gradients as small as the heads: dx holds their quotient)
+    gq, gk = ((r(B, N, H * D) * 2.0 ** -60).to(dtype) for _ in range(2))
+    w = 1 + 0.2 * r(D)
+    table = ops.rope_table(300, F, device=cuda)
+    pos = torch.randint(0, 300, (B, N), generator=gen, device=cuda, dtype=I32)
+    y = ops.qk_norm_rope(q, k, D, w, w, table, pos, eps=eps)
+    d = ops.qk_norm_rope_bwd(q, k, gq, gk, D, w, w, table, pos, eps=eps)
+    half = torch.finfo(dtype).eps / 2
+    for x, g, got, dx in ((q, gq, y[0], d[0]), (k, gk, y[1], d[1])):
+        xd, wd, gd = x.double().unflatten(-1, (-1, D)).requires_grad_(True), w.double(), g.double().unflatten(-1, (-1, D))
+        c, s = (table.double()[pos.long()][..., i].unsqueeze(2) for i in (0, 1))
+        v = xd * (xd.square().mean(-1, keepdim=True) + eps).rsqrt() * wd
+        want = torch.cat((v[..., :F] * c - v[..., F:] * s, v[..., F:] * c + v[..., :F] * s), -1)
+        wdx = torch.autograd.grad(want, xd, gd)[0]
+        big = want.detach().abs().amax(-1, keepdim=True)
+        off = (got.double().unflatten(-1, (-1, D)) - want.detach()).abs()
+        assert bool((off <= half * want.detach().abs() + 2.0 ** -17 * big).all())
+        off = (dx.double().unflatten(-1, (-1, D)) - wdx).abs()
+        assert bool((off <= half * wdx.abs() + 2.0 ** -14 * wdx.abs().amax(-1, keepdim=True)).all())
