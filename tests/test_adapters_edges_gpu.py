@@ -63,3 +63,22 @@ def test_many_rows(cuda, case):
     y = ops.linear_adapters(xd, pw, dd, ud, idx, sd)
     check(y, want)
     assert torch.equal(y, ops.linear_adapters(xd, pw, dd, ud, idx, sd))
+
+
+# ---- more requests than a launch's grid takes ------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_more_requests_than_a_grid(cuda):
+    """70001 requests of one row: the factors' product in two launches, the second from request 65535 on"""
+    from lbm_amd import ops
+    R, K, N, rank = 70001, 64, 64, 8
+    x, w, b, down, up, scaling, index = make(33, R, 1, K, N, 3, rank)
+    has, a, x0 = (index >= 0).double()[:, None], index.clamp(min=0).long(), x[:, 0].double()
+    s = scaling.double()[a][:, None] * has
+    t = s * torch.stack([x0 @ d.double().t() for d in down])[a, torch.arange(R)]
+    each = torch.stack([t @ u.double().t() for u in up])[a, torch.arange(R)]
+    y = x0 @ w.double().t() + b.double() + each
+    mag = x0.abs() @ w.double().abs().t() + b.double().abs()
+    mag += torch.stack([(s * (x0.abs() @ d.double().abs().t())) @ u.double().abs().t() for d, u in zip(down, up)])[a, torch.arange(R)]
+    tol = 2.0 ** -8 * (y.abs() + torch.stack([t.abs() @ u.double().abs().t() for u in up])[a, torch.arange(R)]) + (K + rank + 16) * 2.0 ** -24 * mag
+    args = on(cuda, x[:, 0].contiguous(), w, b, down, up, index, scaling)
+    check(ops.linear_adapters(args[0], ops.pack_linear_weight(args[1], args[2]), *args[3:]), (y, tol))

@@ -239,3 +239,38 @@ def test_sizes_that_32_bits_do_not_hold():
     for x, index in ((wide(1, 2 ** 32 + 5, 64), 1), (wide(2 ** 16, 2 ** 15, 64), 2 ** 16)):
         with pytest.raises(ValueError, match="rows"):
             ops.linear_adapters(x, pw, wide(2, 4, 64), wide(2, 32, 4), torch.empty(index, dtype=I32, device="meta"))
+
+
+# ---- ranked workgroups (over 4096 keys) --------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,cap,bias,times", [(64, 0.0, False, 1), (64, 500.0, True, 20), (40, 8.0, False, 1), (128, 0.0, True, 1), (160, 0.0, False, 1), (96, 300.0, False, 10)])
+@pytest.mark.parametrize("hole", [None, float("nan"), -float("inf")])
+def test_ranked_workgroups_of_two_rows_with_padding_that_holds_anything(cuda, D, cap, bias, times, hole):
+    """two rows of a batch with documents of their own, causal inside them, and padding between that holds zeros or values that are not
+    finite: the second walk starts with the ranking again.  Many heads: the first ones again, in another order"""
+    from lbm_amd import ops
+    B, Nq, Nk, H = 2, 500, 4200, 2
+    q, k, v, g, gen = make(26, B, Nq, Nk, H, H, D)
+    ranges, pad = torch.zeros(B, Nq, 2, dtype=I32), torch.ones(B, Nk, dtype=torch.bool)
+    rows = torch.ones(B, Nq, dtype=torch.bool)
+    for b, docs in enumerate((((0, 120, 0, 900), (125, 300, 905, 4100), (300, 490, 4100, 4190)), ((3, 260, 10, 4000), (270, 500, 4005, 4200)))):
+        for a, e, lo, hi in docs:
+            for i in range(a, e):
+                ranges[b, i] = torch.tensor([lo, max(lo + 1, hi - (e - 1 - i) * (hi - lo) // (2 * (e - a)))])
+            pad[b, lo:hi] = False
+            rows[b, a:e] = False
+    clean = [t.clone() for t in (q, k, v, g)]
+    for t, p in zip((q, k, v, g), (rows, pad, pad, rows)):
+        t[p] = 0.0 if hole is None else hole
+    for t, p in zip(clean, (rows, pad, pad, rows)):
+        t[p] = 0.0
+    slopes = torch.tensor([0.5, 0.01]) if bias else None
+    want = definition(*clean[:3], H, H, D, seen_by(ranges, Nk), (torch.arange(Nq) + Nk - Nq).expand(B, Nq), D ** -0.5, cap, slopes, clean[3])
+    q, k, v, g = (t.to(cuda).repeat(1, 1, times) for t in (q, k, v, g))
+    kw = dict(cap=cap, slopes=None if slopes is None else slopes.to(cuda).repeat(times))
+    ranges = ranges.to(cuda)
+    o, lse, rest = ops.ranged_attn(q, k, v, H * times, H * times, D, ranges, return_lse=True, return_rest=True, **kw)
+    got = (o,) + ops.ranged_attn_bwd(q, k, v, o, g, lse, H * times, H * times, D, ranges, rest=rest, **kw)
+    for n, x in zip(("o", "dq", "dk", "dv"), got):
+        for part in (x[..., :H * D], x[..., -H * D:]):
+            check(n, part, want[n])
