@@ -10,8 +10,8 @@
 //     (lr_* fields), few rows here: the weight's bytes are the floor, so a workgroup of 8 waves takes
 //     16 output columns of 64 rows, its waves split K, and W goes from memory into MFMA operands without LDS.
 // Measured: 16 requests of one token, 1280 -> 1280, rank 16: 5.4 + 5.8 us, of which the weight's 3.3 MB are 0.7: latency of two
-// launches.  8 x 1024 rows, 1280 -> 3840, rank 32: adapter_down 7.7 us (21 MB of x; the factor, 80 KB, is read from L2 by each of
-// 256 workgroups), the whole call 86.5, the shared product alone 75.5.
+// launches.  8 x 1024 rows, 1280 -> 3840, rank 32: adapter_down 7.7 us (8.7 in a trace; 21 MB of x; the factor, 80 KB, is read from
+// L2 by each of 256 workgroups), the whole call 86.5 ... 90.5, the shared product alone 75.5.
 #include "common.h"
 
 namespace {

@@ -279,8 +279,11 @@ __global__ __launch_bounds__(256) void cached_join_kernel(const Cached a) {
 
 int cache_pad(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 160; }
 
-// parts of the keys: some four workgroups per CU over all requests, of at least 256 keys of a full cache each.  Two / four / eight
-// per CU, 20 over 5 heads of 64: 64 requests of 2400 ... 8200 keys 99 / 92 / 89 us, 8 of 1200 ... 4000 keys 14.3 / 15.2 / 16.6 us.
+// parts of the keys: some four workgroups per CU over all requests, of at least 256 keys of a full cache each.  One / two / four per
+// CU, 20 over 5 heads: 64 requests of 2000 ... 8200 keys, heads of 64 97 / 91 / 84 us, of 96 160 / 146 / 141, of 128 175 / 167 / 162
+// (5.0 TB/s), of 160 251 / 228 / 217; 8 requests of 1200 ... 4000 keys, 64 12.3 / 12.5 / 15.4, 128 21.3 / 23.5 / 25.5, 160 27 / 30 / 30;
+// one of 16000, 64 10.9 / 10.9 / 10.9, 128 17.5 / 22.8 / 22.6.  The rule is the many requests': from 72 channels on LDS holds one
+// workgroup per CU, and few requests would be 6 ... 30 % faster with one.
 int cache_splits(int B, int H, int Hk, int n, int cap_rows) {
   const int64_t blocks = (int64_t)B * Hk * (((int64_t)n * (H / Hk) + 31) / 32);
   int64_t s = (4ll * lbmk_num_cus() + blocks - 1) / (blocks > 0 ? blocks : 1);

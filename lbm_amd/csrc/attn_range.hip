@@ -14,7 +14,9 @@
 //
 // Bound by the vector ALU beside the matrix cores: a score costs 4 D operations of matrix work forward, and an exp2 (a quarter of
 // the rate), a fused multiply-add, a maximum, an addition and half a conversion of vector work, as long again at 64 channels; the
-// tiles come from L2.  Measured, 2 x 4096 tokens, 20 heads of 64: all keys 207 us forward (830 TFLOP/s), 715 us backward (600 TFLOP/s of its
+// tiles come from L2.  Counted over 2 x 4096 tokens, 20 heads of 64, matrix / vector units busy: forward 35 / 61 % of the cycles, dQ
+// 44 / 69, dK and dV 39 / 43; with a cap 23 / 81, 28 / 84, 26 / 67.  Short or uneven walks leave CUs without work instead: 69 ... 83 %
+// of the cycles with some over a prefix or 7 documents, 56 ... 61 % over short causal documents.  Measured, 2 x 4096 tokens, 20 heads of 64: all keys 207 us forward (830 TFLOP/s), 715 us backward (600 TFLOP/s of its
 // 5 products); causal 122 (700) and 386 us.  8 heads of 128, causal: 102 us (670), 366 us.  (A library product of 8192^3 reaches 1380 TFLOP/s on the same card.)
 #include "attn_tile.h"
 
@@ -69,8 +71,8 @@ __device__ __forceinline__ int2 row_range(const Ranged& a, int b, int q) {
 //
 // Two parts per block of queries: part 1 takes the queries whose keys start behind those of the block's first query, part 0 the
 // others.  A block across two documents would walk the keys of both, one half of it idle in each, and it alone would set the
-// kernel's time; as two parts it does not (the same documents in one part: 106 us instead of 67, 3000 keys with 4 heads of 160 63
-// instead of 32).  Under a causal mask every query is of part 0, and part 1 ends at once (2 ... 3 us of a short call).
+// kernel's time; as two parts it does not (9001 keys in 7 documents, 10 heads of 64, in one part: 106 us instead of 67 on one box, 3000
+// keys with 4 heads of 160 63 instead of 32).  Under a causal mask every query is of part 0, and part 1 ends at once (2 ... 3 us of a short call).
 //
 // Documents and causal masks give the blocks very different numbers of keys, and a launch is often no more workgroups than the
 // chip holds at once: in any fixed order some CUs get three long ones and others three short ones.  So, over long rows and with up
@@ -431,8 +433,8 @@ __device__ __forceinline__ void put_rows_f32(float* op, const f32x16 (&acc)[DT],
     }
 }
 
-// Two backward kernels, dQ by blocks of queries and dK / dV by blocks of keys: seven products instead of five, but no atomics and no
-// f32 partial sums of dQ, and each operand that an owner keeps stays in registers.  About as long as each other (2 x 2111 tokens,
+// Two backward kernels, dQ by blocks of queries and dK / dV by blocks of keys: S and dP are formed in both, and dS K twice (dS as two
+// operands), eight products instead of five, but no atomics and no f32 partial sums of dQ, and each operand that an owner keeps stays in registers.  About as long as each other (2 x 2111 tokens,
 // causal documents, 20 over 5 heads of 64: 55 and 57 us).
 //
 // dQ and delta; also writes, for the second kernel, what the ranges of each 32 queries have in common
@@ -689,7 +691,9 @@ __device__ __forceinline__ void keys_of(const Ranged& a, char* smem, int& b, int
   cut = __builtin_amdgcn_readfirstlane(cut);
 }
 
-// dK and dV of 128 keys (the heavier of the two per tile: four products, and dS and P as operands): walks the query tiles of every head that shares the key head.  With few workgroups the walk is cut
+// dK and dV of 128 keys (four products per tile, and dS and P as operands, one bf16 each: half a step per weight, of random sign over
+// the queries; a second operand for each, as dQ has for dS, would cost two products more.  dK and dV are 2.3 ... 2.5e-3 of their norm
+// off, where their own rounding is 1.7e-3): walks the query tiles of every head that shares the key head.  With few workgroups the walk is cut
 // into `splits` parts whose sums are added afterwards in their order.
 template <int DH, int KS, int MAP, class Form>
 __device__ __forceinline__ bool ranged_bwd_dkv_body(const Ranged& a, char* smem) {
@@ -1043,8 +1047,12 @@ int fwd_occupancy(int DHP, bool far) { return DHP <= 96 && !far ? 3 : DHP <= 128
 int dq_occupancy(int DHP) { return DHP <= 64 ? 3 : DHP <= 96 ? 2 : 1; }
 
 // Ranked workgroups: few enough for the order to matter and for the ranking to be cheap, and walks long enough to pay for it (every
-// workgroup ranks before it starts, 2 ... 4 us).  Both sides measured: 9001 keys in 7 unequal documents, 10 heads of 64, 84 -> 67 us
-// forward, 310 -> 282 backward; up to 4096 keys it gains nothing (2 x 2111, 20 heads, causal documents: 26 -> 30 us).
+// workgroup ranks before it starts, 2 ... 4 us).  Both sides measured, index order -> ranked, forward and backward us: unequal
+// documents, 9001 keys in 7, 10 heads of 64 86 -> 72 and 300 -> 278, 8 heads of 128 119 -> 93 and 524 -> 476; 12000 in 9, 8 of 64
+// 86 -> 73 and 327 -> 292; 6000 in 5, 10 of 64 55 -> 44 and 208 -> 178; 4600 in 5, 16 of 64 50 -> 40 and 187 -> 165.  It loses where
+// the launch is small or the spans fall evenly: 4200 in 6, 4 heads of 80 29 -> 32 and 98 -> 104, 8000 in 3 causal, 8 of 64 77 -> 80
+// and 254 -> 258; up to 4096 keys it gains little: 3500 in 5, 10 of 64 30 -> 29 and 108 -> 106 (2 x 2111, 20 heads, causal
+// documents: 26 -> 30 forward).
 constexpr int ORDER_KEYS = 4096;
 bool order_pays(const Ranged& a, int64_t n) { return a.ranges && a.Nk > ORDER_KEYS && n <= 4ll * a.cus; }
 void order_blocks(Ranged& a, int occupancy) {

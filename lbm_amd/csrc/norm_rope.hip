@@ -12,8 +12,8 @@
 // between lanes and the norm a log2(L)-step butterfly.  The lanes of a group walk heads of ONE token, so its cosines and
 // sines are read once and stay in registers; the next head is loaded, and kept as it lies in memory, while one is worked on.
 // All statistics and gradient sums are f32; each output is rounded once.
-// Measured, 4 x 4096 tokens, 20 + 20 heads of 64, bf16: 30 us forward (168 MB, 5.6 TB/s; a copy reaches 4.9), 63 us backward
-// (252 MB, 4.0 TB/s) and 4 us for the weights' gradients; a few tokens: 4.5 us, a launch's latency.
+// Measured in a trace, 4 x 4096 tokens, 20 + 20 heads of 64, bf16: 30 us forward (168 MB, 5.6 TB/s; a copy reaches 4.9), 63 us backward
+// (252 MB, 4.0 TB/s) and 4 us for the weights' gradients (both backward kernels 56 us when a graph replays them); a few tokens: 4.5 us, a launch's latency.
 #include "common.h"
 
 namespace {
@@ -402,7 +402,7 @@ int nr_run(NormRope& d, int f32, int interleaved, bool bwd, hipStream_t s) {
   const int vec = nr_vec(d.D, d.rot, interleaved), L = nr_lanes(d.D, vec), groups = NR_THREADS / L;
   // lane groups per token: with many tokens four or five heads per group, so that the token's angles are read once for several
   // heads; with few tokens as many groups as there are heads.  20 + 20 heads of 64, two axes, one head per group against four,
-  // forward / backward: 8 tokens 3.7 / 7.7 us against 4.6 / 8.9, 400 tokens 4.4 / 9.6 against 4.9 / 9.4, 1600 9.1 / 23.7 against
+  // forward / backward, replayed from a graph: 8 tokens 3.7 / 7.7 us against 4.6 / 8.9, 400 tokens 4.4 / 9.6 against 4.9 / 9.4, 1600 9.1 / 23.7 against
   // 6.5 / 12.4, 16384 44 / 81 against 31 / 57
   const int heads = d.H[0] > d.H[1] ? d.H[0] : d.H[1];
   const int per = (int64_t)d.tokens * heads >= 16384 ? NR_HEADS : 1;
