@@ -47,11 +47,18 @@ int main(int, char** argv) {
   pthread_barrier_init(&bar, 0, 4);
   pthread_t t[4];
   for (intptr_t w = 0; w < 4; ++w) pthread_create(&t[w], 0, wave_main, (void*)w);
-  usleep(1000000);                                       // a wave that left the others waiting does not keep the test
-  for (int w = 0; w < 4; ++w) {
-    void* r = 0;
-    printf("%%d ", pthread_tryjoin_np(t[w], &r) == 0 ? (int)(intptr_t)r : -1);
+  int got[4] = {-1, -1, -1, -1};                         // a wave that was left waiting ends the test, not the run: ten seconds
+  for (int i = 0, done = 0; i < 1000 && done < 4; ++i) {
+    usleep(10000);
+    for (int w = 0; w < 4; ++w) {
+      void* r = 0;
+      if (got[w] < 0 && pthread_tryjoin_np(t[w], &r) == 0) {
+        got[w] = (int)(intptr_t)r;
+        ++done;
+      }
+    }
   }
+  for (int w = 0; w < 4; ++w) printf("%%d ", got[w]);
   fflush(stdout);
   _exit(0);
 }
