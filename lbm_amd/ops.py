@@ -1475,6 +1475,17 @@ def _token_rows(name: str, t: torch.Tensor, heads: Optional[int], head_dim: int,
     return p, B, N, c, ld, sb
 
 
+def _rows_overlap(B: int, N: int, c: int, ld: int, sb: int) -> bool:
+    """whether two of the rows of c elements at b * sb + n * ld share an address (ld >= c)"""
+    if B * N == 0 or B == 1 or sb >= (N - 1) * ld + c or (sb >= c and ld >= (B - 1) * sb + c):
+        return False
+    for b in range(1, B):
+        n, r = divmod(b * sb, ld)
+        if (n < N and r < c) or (n + 1 < N and ld - r < c):
+            return True
+    return False
+
+
 def token_rows_ready(t: torch.Tensor) -> torch.Tensor:
     """``t``, or a contiguous copy where the kernels cannot read it in place (an output gradient that autograd expanded
     from a scalar or cut out of another tensor)"""
@@ -1547,7 +1558,7 @@ def _norm_rope(q, k, head_dim, q_weight, k_weight, table, positions, eps, interl
         gqp, _, _, _, lgq, sgq = _token_rows("dq_out", gq, None, head_dim)
         gkp, _, _, _, lgk, sgk = _token_rows("dk_out", gk, None, head_dim)
         _one_device(q, gq, gk)
-    if device < 0:
+    if device < 0 and out is None:
         _need_gpu(q)
     if out is None:
         qo, ko = torch.empty(q.shape, dtype=dt, device=q.device), torch.empty(k.shape, dtype=dt, device=q.device)
@@ -1559,8 +1570,10 @@ def _norm_rope(q, k, head_dim, q_weight, k_weight, table, positions, eps, interl
         _one_device(q, qo, ko)
         qop, _, _, _, ldqo, sqo = _token_rows("out[0]", qo, None, head_dim)
         kop, _, _, _, ldko, sko = _token_rows("out[1]", ko, None, head_dim)
-        if B > 1 and (sqo == 0 or sko == 0):
-            raise ValueError("out: a broadcast batch cannot be written")
+        if _rows_overlap(B, N, qc, ldqo, sqo) or _rows_overlap(B, N, kc, ldko, sko):
+            raise ValueError(f"out: strides {qo.stride()}, {ko.stride()}: rows that overlap (or a broadcast batch) cannot be written")
+        if device < 0:
+            _need_gpu(q)
     d = NormRopeDesc(qp, kp, _ptr(q_weight), _ptr(k_weight), gqp, gkp, qop, kop, _ptr(table), _ptr(positions), B, N, qc // head_dim,
                      kc // head_dim, head_dim, rot, axes, rows, ldq, ldk, ldqo, ldko, lgq, lgk, sq, sk, sqo, sko, sgq, sgk,
                      1 if dt == torch.float32 else 0, 1 if wdt == torch.float32 else 0, 1 if interleaved else 0, eps)

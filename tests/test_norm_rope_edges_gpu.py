@@ -91,3 +91,29 @@ def test_heads_whose_mean_square_is_a_subnormal_number(cuda, dtype, eps):
         assert bool((off <= half * want.detach().abs() + 2.0 ** -17 * big).all())
         off = (dx.double().unflatten(-1, (-1, D)) - wdx).abs()
         assert bool((off <= half * wdx.abs() + 2.0 ** -14 * wdx.abs().amax(-1, keepdim=True)).all())
+
+
+def test_destinations_whose_rows_overlap_are_refused():
+    """two groups would write one address; batches between the rows of a wider buffer do not"""
+    from lbm_amd import ops
+    B, N, C = 2, 4, 64
+    q, k = torch.zeros(B, N, C, dtype=BF), torch.zeros(B, N, C, dtype=BF)
+    good = torch.zeros(B, N, C, dtype=BF)
+    buf = torch.zeros(4096, dtype=BF)
+    for strides in ((0, C, 1), (C, C, 1), (3 * C, C, 1), (C // 2, 2 * C, 1), (4 * C, 2 * C, 1), (2 * C + 8, 2 * C, 1)):
+        bad = buf.as_strided((B, N, C), strides)
+        for out in ((bad, good), (good, bad)):
+            with pytest.raises(ValueError, match="out"):
+                ops.qk_norm_rope(q, k, 64, None, None, out=out)
+    for strides in ((N * C, C, 1), (N * C + 8, C, 1), (C, B * C, 1), (C, 3 * C, 1), (3 * C, 2 * C, 1)):
+        with pytest.raises(RuntimeError, match="GPU only"):
+            ops.qk_norm_rope(q, k, 64, None, None, out=(buf.as_strided((B, N, C), strides), good))
+
+
+def test_overlap_of_rows_against_every_address():
+    import itertools
+    from lbm_amd.ops import _rows_overlap
+    for B, N, c in itertools.product((0, 1, 2, 4), (0, 1, 2, 3), (1, 3)):
+        for ld, sb in itertools.product(range(c, 12), range(0, 26)):
+            rows = [set(range(b * sb + n * ld, b * sb + n * ld + c)) for b in range(B) for n in range(N)]
+            assert _rows_overlap(B, N, c, ld, sb) == (len(set().union(*rows)) < B * N * c), (B, N, c, ld, sb)
