@@ -258,6 +258,27 @@ class LayerNormFn(torch.autograd.Function):
         return (dx, *_cast_pair(dg, db, wdt), None, None, None)
 
 
+class _FirstGradients(torch.autograd.Function):
+    """Hands gradients on as functions of what they were computed from, and refuses the next derivative"""
+
+    @staticmethod
+    def forward(ctx, n, *tensors):
+        return tuple(t.view_as(t) for t in tensors[:n])
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise NotImplementedError("the token operators have no gradient of their gradients")
+
+
+def _first_gradients(grads, *inputs):
+    """``grads`` of a kernel; with a graph asked for (create_graph) a derivative through them raises instead of counting as zero"""
+    if not torch.is_grad_enabled():
+        return grads
+    given = [g for g in grads if g is not None]
+    out = iter(_FirstGradients.apply(len(given), *given, *(t for t in inputs if t is not None)))
+    return tuple(None if g is None else next(out) for g in grads)
+
+
 class QKNormRopeFn(torch.autograd.Function):
     """Head norms of q and k with the position rotation (ops.qk_norm_rope); the backward pass recomputes the statistics
     from the saved inputs."""
@@ -272,9 +293,9 @@ class QKNormRopeFn(torch.autograd.Function):
     def backward(ctx, dq_out, dk_out):
         q, k, wq, wk, table, positions = ctx.saved_tensors
         head_dim, eps, interleaved = ctx.cfg
-        dq, dk, dwq, dwk = ops.qk_norm_rope_bwd(q, k, ops.token_rows_ready(dq_out), ops.token_rows_ready(dk_out), head_dim, wq, wk, table,
-                                                positions, eps=eps, interleaved=interleaved)
-        return dq, dk, dwq, dwk, None, None, None, None, None
+        grads = ops.qk_norm_rope_bwd(q, k, ops.token_rows_ready(dq_out), ops.token_rows_ready(dk_out), head_dim, wq, wk, table, positions,
+                                     eps=eps, interleaved=interleaved)
+        return (*_first_gradients(grads, q, k, wq, wk, dq_out, dk_out), None, None, None, None, None)
 
 
 class SiluFn(torch.autograd.Function):
@@ -401,8 +422,9 @@ class RangedAttentionFn(torch.autograd.Function):
     def backward(ctx, do):
         q, k, v, o, lse, rest, ranges, slopes = ctx.saved_tensors
         heads, kv_heads, head_dim, scale, cap = ctx.cfg
-        return (*ops.ranged_attn_bwd(q, k, v, o, ops.token_rows_ready(do), lse, heads, kv_heads, head_dim, ranges, scale=scale, cap=cap,
-                                     slopes=slopes, rest=rest), None, None, None, None, None, None, None)
+        grads = ops.ranged_attn_bwd(q, k, v, o, ops.token_rows_ready(do), lse, heads, kv_heads, head_dim, ranges, scale=scale, cap=cap,
+                                    slopes=slopes, rest=rest)
+        return (*_first_gradients(grads, q, k, v, do), None, None, None, None, None, None, None)
 
 
 class SelfAttnQKVFn(torch.autograd.Function):
