@@ -71,7 +71,7 @@ __device__ __forceinline__ int2 row_range(const Ranged& a, int b, int q) {
 //
 // Two parts per block of queries: part 1 takes the queries whose keys start behind those of the block's first query, part 0 the
 // others.  A block across two documents would walk the keys of both, one half of it idle in each, and it alone would set the
-// kernel's time; as two parts it does not (9001 keys in 7 documents, 10 heads of 64, in one part: 106 us instead of 67 on one box, 3000
+// kernel's time; as two parts it does not (9001 keys in 7 documents, 10 heads of 64, in one part: 106 us instead of 67, 3000
 // keys with 4 heads of 160 63 instead of 32).  Under a causal mask every query is of part 0, and part 1 ends at once (2 ... 3 us of a short call).
 //
 // Documents and causal masks give the blocks very different numbers of keys, and a launch is often no more workgroups than the
